@@ -495,6 +495,87 @@ int qwc_pack_decode_batch(const uint32_t* row_slots, const uint8_t* slot_active,
                           int rows, int capacity, int max_blocks, int page_size,
                           qwc_stream stream);
 
+/* ------------------------------------------------------------------ */
+/* Chunks of new tokens and shared prefixes (additive)                  */
+/* ------------------------------------------------------------------ */
+
+/*
+ * Copies units (cache pages, state slots) inside arrays: for every array and every pair
+ * {source, target} of pairs u32[count][2] (device), unit `source` becomes unit `target`.  `arrays` is HOST
+ * memory, read during the call; each entry names device memory of `units` units of `unit_bytes` bytes
+ * (base 16-byte aligned, unit_bytes a multiple of 16).  One launch per 128 arrays: K and V of all attention
+ * layers (unit = page), or codes, scales and convolution history of all DeltaNet layers (unit = slot).
+ *
+ * No target may be named twice or be a source as well (a pair with source == target is skipped, which is
+ * also how a list is padded).  A pair beyond an array's units is not copied there, and the device
+ * status word reads 0x107.  count == 0 does nothing.
+ * Does for a list of pages what Executor::copy_kv_block (crates/qwc-engine/src/executor.rs:825-835) does for one.
+ */
+typedef struct qwc_copy_array {
+    void* base;
+    uint64_t unit_bytes;
+    uint64_t units;
+} qwc_copy_array;
+
+int qwc_cache_copy(const qwc_copy_array* arrays, int array_count, const uint32_t* pairs, int count,
+                   qwc_stream stream);
+
+/*
+ * The operators below take a ragged batch of chunks of new tokens, `sequences` of them (1..128), in
+ * `tokens` rows (1..65536): chunk s is rows chunk_begins[s] .. chunk_begins[s + 1] (u32[sequences + 1], device,
+ * ascending, cut at `tokens`; empty chunks are fine).  Rows of no chunk are left as they were.  state_slots
+ * u32[sequences] names each chunk's slot, no slot twice; a slot beyond the pool leaves its chunk out and the
+ * device status word reads 0x105.  continues u32[sequences] (NULL: all 1) is 0 where a sequence begins with its chunk:
+ * what the slot holds from before then counts as zeros.  The number of value heads comes from qwc_configure.
+ */
+
+/*
+ * Attention of the chunks' tokens over the paged e4m3 cache, which holds their own keys and values already:
+ * token i of a chunk of n stands at position context_lengths[s] - n + i (context_lengths u32[sequences] count the
+ * chunk) and sees the positions up to its own; a row that sees none is zero.  Heads, cache layout, scales, gate
+ * and gate_stride as qwc_paged_attention_packed_fp8_scaled, except that block_tables u32[sequences, max_blocks] has a
+ * row for each sequence.  query, output bf16[tokens, 24, 256].  num_blocks: pages of the cache; a page
+ * beyond it reads as zeros.  workspace: qwc_paged_attention_chunk_workspace_bytes() bytes; calls that overlap on
+ * the device must not share one.  Pointers of rows, caches and workspace 16-byte aligned.
+ * The segment shapes of crates/qwc-cuda/src/ffi.rs:520-537, for a whole batch.
+ */
+size_t qwc_paged_attention_chunk_workspace_bytes(void);
+int qwc_paged_attention_chunk_fp8(const void* query, const void* query_gate_projection, const void* key_cache,
+                                  const void* value_cache, const void* block_tables, const void* context_lengths,
+                                  const void* chunk_begins, const float* key_scales, const float* value_scales,
+                                  void* output, void* workspace, size_t workspace_bytes, int tokens, int sequences,
+                                  int max_blocks, int page_size, int num_blocks, int gate_stride, float softmax_scale,
+                                  qwc_stream stream);
+
+/*
+ * The step in front of the delta rule for chunks: convolution over the tokens, SiLU, L2 norm of q and k, decay and
+ * write strength.  Inputs as qwc_delta_prepare_decode (rows of mixed_stride and gate_stride elements,
+ * mixed_stride % 8 == 0); the convolution starts from the slot's history conv_state f32[capacity, channels, 3] and leaves
+ * the chunk's last rows there.  qkv bf16[tokens, channels]: q [16][128] (scaled by 128^-1/2) | k [16][128] |
+ * v [heads][128], each rounded once; alpha, beta f32[tokens, heads].  mixed_qkv, conv_weight and qkv 16-byte aligned.
+ */
+int qwc_delta_prepare_chunk(const void* mixed_qkv, const void* a_projection, const void* b_projection,
+                            const void* conv_weight, const void* a_log, const void* dt_bias, void* conv_state,
+                            const void* state_slots, const void* continues, const void* chunk_begins, void* qkv,
+                            void* alpha, void* beta, int state_capacity, int tokens, int sequences, int mixed_stride,
+                            int gate_stride, qwc_stream stream);
+
+/*
+ * The gated delta rule over chunks, on the slots' int8 state (layout of qwc_delta_decode_int8): per token
+ *   S <- alpha S;  u = beta (v - S k);  S <- S + u k^T;  o = S q
+ * The state is read from its eight bits at the start of a chunk, carried in fp32, and written back at its end.
+ * qkv, alpha, beta: what qwc_delta_prepare_chunk wrote.  out bf16[tokens, heads, 128].  With norm_weight
+ * bf16[128] and gate bf16 rows of gate_stride elements (0 = heads * 128; both or neither NULL), out is
+ * rmsnorm(o) * norm_weight * silu(gate) instead.  workspace: qwc_delta_chunk_workspace_bytes(tokens, sequences) bytes;
+ * calls that overlap on the device must not share one.  Row pointers, state and workspace 16-byte aligned.
+ */
+size_t qwc_delta_chunk_workspace_bytes(int tokens, int sequences);
+int qwc_delta_chunk_int8(void* state, float* state_scales, const void* state_slots, const void* continues,
+                         const void* chunk_begins, const void* qkv, const void* alpha, const void* beta, void* out,
+                         int state_capacity, int tokens, int sequences, const void* gate, int gate_stride,
+                         const void* norm_weight, float epsilon, void* workspace, size_t workspace_bytes,
+                         qwc_stream stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -114,6 +114,12 @@ KERNEL_SYMBOLS = {
     "qwc_fp8_max_batched_logits": (c_int, []),
     "qwc_argmax": (c_int, [P, P, P, P, c_int, c_int, c_int, P]),
     "qwc_page_table_apply": (c_int, [P, P, P, c_int, c_int, c_int, P]),
+    "qwc_cache_copy": (c_int, [P, c_int, P, c_int, P]),
+    "qwc_paged_attention_chunk_workspace_bytes": (c_size_t, []),
+    "qwc_paged_attention_chunk_fp8": (c_int, [P] * 11 + [c_size_t] + [c_int] * 6 + [c_float, P]),
+    "qwc_delta_prepare_chunk": (c_int, [P] * 13 + [c_int] * 5 + [P]),
+    "qwc_delta_chunk_workspace_bytes": (c_size_t, [c_int, c_int]),
+    "qwc_delta_chunk_int8": (c_int, [P] * 9 + [c_int] * 3 + [P, c_int, P, c_float, P, c_size_t, P]),
     "qwc_pack_decode_batch": (c_int, [P] * 18 + [c_int, c_int, c_int, c_int, P]),
 }
 

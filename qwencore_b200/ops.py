@@ -11,6 +11,7 @@ from __future__ import annotations
 
 import math
 
+import numpy as np
 import torch
 
 from . import abi
@@ -301,3 +302,115 @@ def pack_decode_batch(row_slots, slot_active, seq_tokens, seq_blocks, rope_table
         _p(state_slots), _p(positions), _p(context_lengths), _p(physical_blocks), _p(block_offsets), _p(block_tables),
         _p(block_table_offsets), _p(block_ids), _p(cosine), _p(sine), _p(status), rows, capacity, max_blocks,
         page_size, _stream()), "qwc_pack_decode_batch")
+
+
+# ---- chunks of new tokens and shared prefixes (additive entry points) ------------------------------
+
+def _check_here(*tensors) -> None:
+    """The launch goes to the current device: every tensor has to be there."""
+    device = torch.cuda.current_device()
+    for tensor in tensors:
+        assert tensor is None or (tensor.is_cuda and tensor.device.index == device and tensor.is_contiguous())
+
+
+def copy_table(tensors, units: int) -> np.ndarray:
+    """The arrays of `cache_copy`: one row (address, bytes of a unit, units) for each tensor of `units` units."""
+    for tensor in tensors:
+        assert tensor.is_contiguous() and tensor.numel() % units == 0
+    return np.array([[t.data_ptr(), t.numel() // units * t.element_size(), units] for t in tensors], dtype=np.uint64)
+
+
+def cache_copy(table: np.ndarray, pairs: torch.Tensor, count: int) -> None:
+    """Unit `source` of every array becomes unit `target` for the first `count` rows of `pairs` (source, target)."""
+    assert table.dtype == np.uint64 and table.ndim == 2 and table.shape[1] == 3 and table.flags.c_contiguous
+    assert pairs.numel() >= 2 * count and pairs.element_size() == 4
+    _check_here(pairs)
+    abi.check(abi.lib.qwc_cache_copy(table.ctypes.data, table.shape[0], _p(pairs), count, _stream()), "qwc_cache_copy")
+
+
+def attention_chunk_workspace_bytes() -> int:
+    return int(abi.lib.qwc_paged_attention_chunk_workspace_bytes())
+
+
+def paged_attention_chunk(query, query_gate_projection, key_cache, value_cache, block_tables, context_lengths,
+                          chunk_begins, max_blocks_per_sequence: int, output, tokens: int, sequences: int, workspace,
+                          page_size: int, num_blocks: int, key_scales=None, value_scales=None,
+                          gate_stride: int = 0) -> None:
+    """Attention of a ragged batch of chunks over the paged cache, which holds the chunks' own keys and values already.
+
+    Rows chunk_begins[s] .. chunk_begins[s + 1] are the newest tokens of sequence s; context_lengths count them.
+    """
+    assert query.numel() >= tokens * NUM_ATTN_HEADS * ATTN_HEAD_DIM and query.dtype == torch.bfloat16
+    assert output.numel() >= tokens * NUM_ATTN_HEADS * ATTN_HEAD_DIM and output.dtype == torch.bfloat16
+    assert context_lengths.numel() >= sequences and chunk_begins.numel() > sequences
+    assert block_tables.numel() >= sequences * max_blocks_per_sequence
+    for cache in (key_cache, value_cache):
+        assert cache.numel() * cache.element_size() >= num_blocks * NUM_KV_HEADS * page_size * ATTN_HEAD_DIM
+    if query_gate_projection is not None:
+        stride = gate_stride or NUM_ATTN_HEADS * 2 * ATTN_HEAD_DIM
+        assert query_gate_projection.numel() >= (tokens - 1) * stride + NUM_ATTN_HEADS * 2 * ATTN_HEAD_DIM
+    _check_here(query, query_gate_projection, key_cache, value_cache, block_tables, context_lengths, chunk_begins, output,
+                workspace, key_scales, value_scales)
+    workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    abi.check(abi.lib.qwc_paged_attention_chunk_fp8(
+        _p(query), _p(query_gate_projection), _p(key_cache), _p(value_cache), _p(block_tables), _p(context_lengths),
+        _p(chunk_begins), _p(key_scales), _p(value_scales), _p(output), _p(workspace), workspace_bytes, tokens, sequences,
+        max_blocks_per_sequence, page_size, num_blocks, gate_stride, 1.0 / math.sqrt(ATTN_HEAD_DIM), _stream()),
+        "qwc_paged_attention_chunk_fp8")
+
+
+def _delta_channels() -> tuple[int, int]:
+    heads = abi.get_shape()[0]
+    return heads, (2 * LA_NUM_K_HEADS + heads) * LA_HEAD_DIM
+
+
+def delta_prepare_chunk(mixed, a_offset: int, b_offset: int, conv_weight, a_log, dt_bias, conv_state, state_slots,
+                        continues, chunk_begins, qkv, alpha, beta, state_capacity: int, tokens: int, sequences: int,
+                        mixed_stride: int) -> None:
+    """Convolution, norms and gates for chunks; a/b are strided views of the mixed row, as in `delta_prepare_decode`."""
+    heads, channels = _delta_channels()
+    assert mixed.numel() >= (tokens - 1) * mixed_stride + max(channels, a_offset + heads, b_offset + heads)
+    assert qkv.numel() >= tokens * channels and alpha.numel() >= tokens * heads and beta.numel() >= tokens * heads
+    assert conv_state.numel() >= state_capacity * channels * 3 and conv_weight.numel() >= channels * 4
+    assert mixed.dtype == torch.bfloat16 and qkv.dtype == torch.bfloat16 and conv_state.dtype == torch.float32
+    assert state_slots.numel() >= sequences and chunk_begins.numel() > sequences
+    assert continues is None or continues.numel() >= sequences
+    _check_here(mixed, conv_weight, a_log, dt_bias, conv_state, state_slots, continues, chunk_begins, qkv, alpha, beta)
+    base = mixed.data_ptr()
+    abi.check(abi.lib.qwc_delta_prepare_chunk(base, base + 2 * a_offset, base + 2 * b_offset, _p(conv_weight), _p(a_log),
+                                              _p(dt_bias), _p(conv_state), _p(state_slots), _p(continues),
+                                              _p(chunk_begins), _p(qkv), _p(alpha), _p(beta), state_capacity, tokens,
+                                              sequences, mixed_stride, mixed_stride, _stream()),
+              "qwc_delta_prepare_chunk")
+
+
+def delta_chunk_workspace_bytes(tokens: int, sequences: int) -> int:
+    return int(abi.lib.qwc_delta_chunk_workspace_bytes(tokens, sequences))
+
+
+def delta_chunk(state, state_scales, state_slots, continues, chunk_begins, qkv, alpha, beta, out, state_capacity: int,
+                tokens: int, sequences: int, workspace, gate=None, gate_offset: int = 0, gate_stride: int = 0,
+                norm_weight=None, epsilon: float = 1e-6) -> None:
+    """The gated delta rule over chunks, on the rows that `delta_prepare_chunk` wrote.
+
+    With `gate` (bf16 rows, z at column gate_offset) and `norm_weight` the gated RMSNorm is applied to the result."""
+    heads, channels = _delta_channels()
+    assert state.dtype == torch.int8 and state_scales.dtype == torch.float32 and qkv.dtype == torch.bfloat16
+    assert state.numel() >= state_capacity * heads * LA_HEAD_DIM ** 2
+    assert state_scales.numel() >= state_capacity * heads * LA_HEAD_DIM
+    assert qkv.numel() >= tokens * channels and out.numel() >= tokens * heads * LA_HEAD_DIM
+    assert out.dtype == torch.bfloat16 and alpha.dtype == torch.float32 and beta.dtype == torch.float32
+    assert alpha.numel() >= tokens * heads and beta.numel() >= tokens * heads
+    assert state_slots.numel() >= sequences and chunk_begins.numel() > sequences
+    assert continues is None or continues.numel() >= sequences
+    if gate is not None:
+        stride = gate_stride or heads * LA_HEAD_DIM
+        assert gate.dtype == torch.bfloat16 and norm_weight.numel() >= LA_HEAD_DIM
+        assert gate.numel() >= (tokens - 1) * stride + gate_offset + heads * LA_HEAD_DIM
+    _check_here(state, state_scales, state_slots, continues, chunk_begins, qkv, alpha, beta, out, workspace, gate,
+                norm_weight)
+    workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    abi.check(abi.lib.qwc_delta_chunk_int8(
+        _p(state), _p(state_scales), _p(state_slots), _p(continues), _p(chunk_begins), _p(qkv), _p(alpha), _p(beta),
+        _p(out), state_capacity, tokens, sequences, 0 if gate is None else gate.data_ptr() + 2 * gate_offset, gate_stride,
+        _p(norm_weight), epsilon, _p(workspace), workspace_bytes, _stream()), "qwc_delta_chunk_int8")
