@@ -4,137 +4,998 @@
 // Heads, cache and gate as in the decode attention (cuda/paged_attention.cu:1299-1713); the chunk's own keys and values
 // are in the cache already.  A row that sees nothing is zero.
 //
-// A CTA has one token and one KV head, its warps take the positions w, w + 8, ... with the six query heads of the group in
-// registers, and their sums meet in shared memory.
+// Bound by the tensor cores once a chunk has more than a few dozen tokens: 4 * 256 flops for each (row, position).
+// Two SMs of a pair work on one item (chunk_plan.h), 42 tokens x 6 heads of a KV head: 126 rows each, of 128.  For every
+// unit of 128 positions tcgen05.mma.cta_group::2 computes S = Q K^T and O += P V for all 256 rows; an SM fetches and widens
+// half of the operands, 64 of the keys and 128 of the value's dims, which is why it is a pair: alone, an SM would have to
+// widen twice as much as its integer pipes do beside the softmax.
+//
+//   * operands are f16.  An e4m3 is moved bit by bit into an f16 that is 2^-8 of it, exactly (a shift and two masks for two of
+//     them; the factor goes into the scales).  A code that is no number becomes a finite one, so that it does no harm
+//     where a probability is zero.  Queries are brought to 2^15 by a power of two per row: a bf16's eight bits fit f16's
+//     eleven for 29 binades below the row's largest element.  The mask and the shifts take bytes 0 and 2, 1 and 3 of a
+//     word together, so the dims of K, Q and V lie in that order, and the columns of O are put right when it is stored;
+//   * a thread is a row of S: no shuffles.  Probabilities go back as f16 into the tensor memory of their scores, as the A
+//     operand of P V (rounded to eleven bits; their fp32 values are summed).  The running maximum that they refer to
+//     follows the scores only when these have grown by 2^8, so that O, which stays in tensor memory for the whole item, is
+//     hardly ever rescaled;
+//   * tensor memory: two buffers of scores (2 x 128 columns) and O (256 columns).  S of unit n + 1 is issued before P V of unit n.
+//
+//   warps 0-3   softmax, and the item's result
+//   warps 4-7   widen Q, K and V
+//   warp 8      fetches K and V, rings of two stages
+//   warp 9      issues the MMAs (in the pair's first CTA)
 
 #include "chunk.cuh"
+#include "chunk_plan.h"
+#include "tcgen05.cuh"
 
 namespace qwc {
 namespace {
 
-constexpr int kWarps = 8;
+constexpr int kThreads = 320;
+constexpr int kFirstWidenWarp = 4;
+constexpr int kWidenWarps = 4;
+constexpr int kFetchWarp = 8;
+constexpr int kMmaWarp = 9;
+constexpr int kRowTokens = kItemTokens / 2;              // of a CTA's rows
+constexpr int kRows = 128;                               // ... 126 of them used
+constexpr int kUnit = kPlanUnitTokens;
+constexpr int kKeyTokens = kUnit / 2;                    // of a unit that a CTA widens
+constexpr int kBoxTokens = 16;
+constexpr int kBoxBytes = kBoxTokens * 128;
+constexpr int kRawBytes = kKeyTokens * kHeadDim;         // K of a unit, or V: 16 KiB
+constexpr int kRawStages = 2;
+constexpr int kKeyBlock = kKeyTokens * 128;              // 64 dims of the widened keys
+constexpr int kValueBlock = kUnit * 128;
+constexpr int kQueryBlock = kRows * 128;
+constexpr int kTmemColumns = 512;
+constexpr int kOutputColumn = 2 * kUnit;
+constexpr int kMaxPairs = 96;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kRescaleAbove = 8.0f;                    // log2
+static_assert(kPlanHeads == kKvHeads && kRowTokens * kGqaGroup <= kRows, "the plan's items");
 
-__device__ __forceinline__ void e4m3x8_to_float(const uint2& codes, float (&out)[8]) {
-    const uint32_t words[2] = {codes.x, codes.y};
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        uint32_t lo, hi;
-        cvt_e4m3x4_to_f16x2(words[i], lo, hi);
-        const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-        const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-        out[4 * i] = a.x;
-        out[4 * i + 1] = a.y;
-        out[4 * i + 2] = b.x;
-        out[4 * i + 3] = b.y;
-    }
+struct Smem {
+    uint8_t q[4 * kQueryBlock];               // [64 dims][row][128 bytes], f16, 128-byte swizzle
+    uint8_t k[2][4 * kKeyBlock];              // [64 dims][token][128 bytes]
+    uint8_t v[2 * kValueBlock];               // [64 dims][token][128 bytes]
+    uint8_t raw_k[kRawStages][kRawBytes];     // [half of the dims][token][128 bytes], e4m3, 128-byte swizzle
+    uint8_t raw_v[kRawStages][kRawBytes];     // [token][128 bytes]
+    uint64_t raw_k_full[kRawStages], raw_k_empty[kRawStages];
+    uint64_t raw_v_full[kRawStages], raw_v_empty[kRawStages];
+    uint64_t k_full[2], k_empty[2], v_full, v_empty;  // (k_full, v_full, q_full, p_full, o_free: the first CTA's count for both)
+    uint64_t q_full, q_free, scales_ready;
+    uint64_t s_full[2], p_full[2];
+    uint64_t o_done[2], o_free;
+    float row_scale[kRows];                   // what the row's query has been divided by
+    long long sequence_line[kMaxChunkSequences];
+    ChunkWalk start;
+    long long total;
+    uint32_t tmem_base;
+    int stop;    // nothing is done: an earlier kernel has given up
+    int failed;  // a wait gave up
+};
+static_assert(sizeof(Smem) + 1024 <= 232448, "shared memory of a CTA");
+
+// What a pair leaves of an item that is cut: statistics and normalised rows of both CTAs, two slots for each pair.
+struct PartialStats {
+    float maximum;  // log2
+    float sum;
+};
+struct MergeItem {
+    int sequence;  // -1: nothing to merge
+    int head;
+    int tile;
+    int last_pair;
+    int first_row;
+    int rows;      // tokens
+};
+constexpr size_t kSlotRows = 2 * kRows;
+constexpr size_t kOutBytes = static_cast<size_t>(kMaxPairs) * 2 * kSlotRows * kHeadDim * sizeof(__half);
+constexpr size_t kStatsBytes = static_cast<size_t>(kMaxPairs) * 2 * kSlotRows * sizeof(PartialStats);
+constexpr size_t kWorkspaceBytes = kOutBytes + kStatsBytes + kMaxPairs * sizeof(MergeItem);
+
+struct Params {
+    const __nv_bfloat16* query;
+    const __nv_bfloat16* gate;
+    const uint32_t* block_tables;
+    const uint32_t* context_lengths;
+    const uint32_t* begins;
+    const float* key_scales;
+    const float* value_scales;
+    __nv_bfloat16* output;
+    __half* partial_out;
+    PartialStats* partial_stats;
+    MergeItem* merge;
+    int tokens, sequences, max_blocks, page_size, num_blocks, gate_stride;
+    float softmax_scale;
+    int* status;
+};
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t rank;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    return rank;
 }
 
-__global__ void __launch_bounds__(kWarps * 32) chunk_attention_kernel(
-    const __nv_bfloat16* __restrict__ query, const __nv_bfloat16* __restrict__ gate, const uint8_t* __restrict__ keys,
-    const uint8_t* __restrict__ values, const uint32_t* __restrict__ block_tables,
-    const uint32_t* __restrict__ context_lengths, const uint32_t* __restrict__ begins,
-    const float* __restrict__ key_scales, const float* __restrict__ value_scales, __nv_bfloat16* __restrict__ output,
-    int tokens, int sequences, int max_blocks, int page_size, int num_blocks, int gate_stride, float softmax_scale) {
-    pdl_launch_dependents();
-    __shared__ float maxima[kWarps][kGqaGroup], sums[kWarps][kGqaGroup];
-    __shared__ float partial[kWarps][kHeadDim];
+__device__ __forceinline__ void pair_sync() {
+    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
+// An arrival at the barrier of the pair's first CTA.
+__device__ __forceinline__ void arrive_first(uint64_t* bar) {
+    asm volatile(
+        "{\n"
+        ".reg .b32 remote;\n"
+        "mapa.shared::cluster.u32 remote, %0, 0;\n"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [remote];\n"
+        "}\n" ::"r"(smem_u32(bar))
+        : "memory");
+}
+
+__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        "selp.u32 %0, 1, 0, p;\n"
+        "}\n"
+        : "=r"(done)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
+// Every role marches unit by unit with the others, so no wait is long: it gives up after 20 ms.
+__device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, Smem& sm, int* status) {
+    const long long start = clock64();
+    for (;;) {
+#pragma unroll 1
+        for (int spin = 0; spin < 64; ++spin) {
+            if (try_wait_cluster(bar, parity)) {
+                return true;
+            }
+        }
+        if (*reinterpret_cast<volatile int*>(&sm.failed) != 0) {
+            return false;
+        }
+        if (clock64() - start > 40000000ll) {
+            break;
+        }
+    }
+    atomicCAS(status, 0, kStatusChunkAttentionWait);
+    *reinterpret_cast<volatile int*>(&sm.failed) = 1;
+    return false;
+}
+
+// For a converged warp: the same answer in every lane.
+__device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Smem& sm, int* status) {
+    const bool ok = try_wait_cluster(bar, parity) || wait_slow(bar, parity, sm, status);
+    return __all_sync(0xffffffffu, ok);
+}
+
+// D[2 x 128][N] (+)= A[2 x 128][16] x B[N][16], f16, fp32 accumulate, both SMs of the pair: A from shared memory ...
+__device__ __forceinline__ void pair_mma_ss(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// ... or tensor memory.
+__device__ __forceinline__ void pair_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
+                                            uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// One arrival at the barrier of both CTAs when every MMA issued so far has completed.
+__device__ __forceinline__ void pair_commit(uint64_t* bar) {
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(
+            smem_u32(bar)),
+        "h"(static_cast<uint16_t>(3))
+        : "memory");
+}
+
+// Operand of 128-byte rows with the 128-byte swizzle, eight rows to an atom.  K-major: a row is one of M or N, its bytes 64
+// of the contracted elements.  MN-major: a row is one of the contracted, its bytes 64 of M or N, the next 64 `block` bytes on.
+__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t block) {
+    const uint64_t lo = ((address >> 4) & 0x3FFFu) | (static_cast<uint64_t>((block >> 4) & 0x3FFFu) << 16);
+    const uint64_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
+    return lo | (hi << 32);
+}
+
+__device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,"
+        "%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Largest of three; a NaN counts as nothing.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    uint32_t out;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(out) : "f"(hi), "f"(lo));
+    return out;
+}
+
+// Four e4m3 -> two f16x2 of 2^-8 their value: bytes 0 and 2, bytes 1 and 3.
+__device__ __forceinline__ void widen4(uint32_t word, uint32_t& even, uint32_t& odd) {
+    even = ((word << 7) & 0x3f803f80u) | ((word << 8) & 0x80008000u);
+    odd = ((word >> 1) & 0x3f803f80u) | (word & 0x80008000u);
+}
+
+// 64 bytes of eight raw rows of 128 bytes -> f16, by a warp: `half` of the row.  Sixteen bytes per lane; lanes 0-3 and 4-7 of
+// a phase read rows that differ in bits 0 and 2, so that neither the loads nor the stores meet in a bank.
+__device__ __forceinline__ void widen_rows(const uint8_t* raw, uint8_t* wide, int half, int lane) {
+    const int group = lane >> 3;
+    const int row = (lane & 4) != 0 ? group ^ 5 : group;
+    const int piece = lane & 3;
+    const uint4 codes = *reinterpret_cast<const uint4*>(raw + row * 128 + (((half * 4 + piece) ^ row) << 4));
+    uint4 lo, hi;
+    widen4(codes.x, lo.x, lo.y);
+    widen4(codes.y, lo.z, lo.w);
+    widen4(codes.z, hi.x, hi.y);
+    widen4(codes.w, hi.z, hi.w);
+    *reinterpret_cast<uint4*>(wide + row * 128 + (((2 * piece) ^ row) << 4)) = lo;
+    *reinterpret_cast<uint4*>(wide + row * 128 + (((2 * piece + 1) ^ row) << 4)) = hi;
+}
+
+// Cache pages as rows of 256 bytes, fetched in boxes of 16 tokens x 128 bytes.  A row beyond the cache arrives as zeros.
+cudaError_t encode_pages(CUtensorMap* map, const void* cache, long long rows) {
+    const EncodeTiled encode = tensor_map_encoder();
+    if (encode == nullptr) {
+        return cudaErrorNotSupported;
+    }
+    const cuuint64_t dims[2] = {kHeadDim, static_cast<cuuint64_t>(rows)};
+    const cuuint64_t strides[1] = {kHeadDim};
+    const cuuint32_t box[2] = {128, kBoxTokens};
+    const cuuint32_t element_strides[2] = {1, 1};
+    const CUresult result =
+        encode(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(cache), dims, strides, box, element_strides,
+               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return result == CUDA_SUCCESS ? cudaSuccess : cudaErrorInvalidValue;
+}
+
+__device__ __forceinline__ ChunkSequence sequence_info(const Params& p, int sequence) {
+    const ChunkSpan span = chunk_span(p.begins, sequence, p.tokens);
+    const uint32_t capacity = static_cast<uint32_t>(p.max_blocks) * static_cast<uint32_t>(p.page_size);
+    return {span.begin, span.length, static_cast<int>(min(__ldcg(p.context_lengths + sequence), capacity))};
+}
+
+// Where this pair's share of the line begins, by the whole CTA.
+__device__ __forceinline__ void find_start(const Params& p, Smem& sm, int pair, int pairs) {
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
-    const int kv_head = blockIdx.y;
-    pdl_wait();
-    const ChunkTile tile = find_chunk_tile(begins, sequences, tokens, 1, blockIdx.x);
-    if (tile.sequence < 0) {
-        return;
-    }
-    const size_t row = static_cast<size_t>(tile.span.begin) + tile.index;
-    const uint32_t context =
-        min(__ldcg(context_lengths + tile.sequence), static_cast<uint32_t>(max_blocks) * static_cast<uint32_t>(page_size));
-    const int hidden_behind = tile.span.length - 1 - tile.index;  // later tokens of the chunk
-    const int visible = static_cast<int>(context) - hidden_behind;
-    const uint32_t* table = block_tables + static_cast<size_t>(tile.sequence) * max_blocks;
-    const float scale = softmax_scale * kLog2e * (key_scales ? key_scales[kv_head] : 1.0f);
-    float q[kGqaGroup][8], acc[kGqaGroup][8], running_max[kGqaGroup], running_sum[kGqaGroup];
-#pragma unroll
-    for (int h = 0; h < kGqaGroup; ++h) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(query + (row * kQueryHeads + kv_head * kGqaGroup + h) * kHeadDim + 8 * lane);
-        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            q[h][2 * i] = __uint_as_float(words[i] << 16) * scale;
-            q[h][2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u) * scale;
-            acc[h][2 * i] = acc[h][2 * i + 1] = 0.0f;
+    // a head's length of line for every sequence
+    for (int s = warp; s < p.sequences; s += kThreads / 32) {
+        const ChunkSequence info = sequence_info(p, s);
+        const int tiles = item_tiles(info);
+        long long sum = 0;
+        for (int tile = lane; tile < tiles; tile += 32) {
+            sum += item_units(info, tile) + kItemLead;
         }
-        running_max[h] = -INFINITY;
-        running_sum[h] = 0.0f;
-    }
-    for (int position = warp; position < visible; position += kWarps) {
-        const uint32_t page = __ldg(table + position / page_size);
-        const bool exists = page < static_cast<uint32_t>(num_blocks);
-        const size_t at = ((static_cast<size_t>(page) * kKvHeads + kv_head) * page_size + position % page_size) * kHeadDim + 8 * lane;
-        float k[8], v[8];
-        e4m3x8_to_float(exists ? *reinterpret_cast<const uint2*>(keys + at) : make_uint2(0, 0), k);
-        e4m3x8_to_float(exists ? *reinterpret_cast<const uint2*>(values + at) : make_uint2(0, 0), v);
 #pragma unroll
-        for (int h = 0; h < kGqaGroup; ++h) {
-            float score = 0.0f;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                score = fmaf(q[h][i], k[i], score);
-            }
-            score = warp_sum(score);
-            const float new_max = fmaxf(running_max[h], score);
-            const float factor = exp2f(running_max[h] - new_max);
-            const float weight = exp2f(score - new_max);
-            running_sum[h] = fmaf(running_sum[h], factor, weight);
-            running_max[h] = new_max;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                acc[h][i] = fmaf(acc[h][i], factor, weight * v[i]);
-            }
+        for (int offset = 16; offset > 0; offset >>= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, offset);
         }
-    }
-    if (lane == 0) {
-#pragma unroll
-        for (int h = 0; h < kGqaGroup; ++h) {
-            maxima[warp][h] = running_max[h];
-            sums[warp][h] = running_sum[h];
+        if (lane == 0) {
+            sm.sequence_line[s] = sum;
         }
     }
     __syncthreads();
-    const float v_scale = value_scales ? value_scales[kv_head] : 1.0f;
-    const int dim = threadIdx.x;
-#pragma unroll
-    for (int h = 0; h < kGqaGroup; ++h) {
-        float highest = -INFINITY;
-        for (int w = 0; w < kWarps; ++w) {
-            highest = fmaxf(highest, maxima[w][h]);
-        }
-        const float factor = running_sum[h] > 0.0f ? exp2f(running_max[h] - highest) : 0.0f;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            partial[warp][8 * lane + i] = acc[h][i] * factor;
-        }
-        __syncthreads();
-        float total = 0.0f, denominator = 0.0f;
-        for (int w = 0; w < kWarps; ++w) {
-            total += partial[w][dim];
-            denominator += sums[w][h] > 0.0f ? sums[w][h] * exp2f(maxima[w][h] - highest) : 0.0f;
-        }
-        float value = denominator > 0.0f ? total * v_scale / denominator : 0.0f;
-        const int head = kv_head * kGqaGroup + h;
-        if (gate != nullptr) {
-            value *= 1.0f / (1.0f + __expf(-__bfloat162float(gate[row * gate_stride + head * (2 * kHeadDim) + kHeadDim + dim])));
-        }
-        output[(row * kQueryHeads + head) * kHeadDim + dim] = __float2bfloat16(value);
-        __syncthreads();
+    if (warp != 0) {
+        return;
     }
+    long long total = 0;
+    for (int s = lane; s < p.sequences; s += 32) {
+        total += kPlanHeads * sm.sequence_line[s];
+    }
+#pragma unroll
+    for (int offset = 16; offset > 0; offset >>= 1) {
+        total += __shfl_xor_sync(0xffffffffu, total, offset);
+    }
+    const int workers = plan_workers(total, pairs);
+    const long long begin = share_begin(total, pair, workers);
+    ChunkWalk walk = {};
+    walk.left = pair < workers ? share_begin(total, pair + 1, workers) - begin : 0;
+    // the sequence: a warp scan for 32 of them
+    long long carry = 0;
+    for (int base = 0; base < p.sequences && walk.left > 0; base += 32) {
+        const long long mine = base + lane < p.sequences ? kPlanHeads * sm.sequence_line[base + lane] : 0;
+        long long inclusive = mine;
+#pragma unroll
+        for (int offset = 1; offset < 32; offset <<= 1) {
+            const long long other = __shfl_up_sync(0xffffffffu, inclusive, offset);
+            if (lane >= offset) {
+                inclusive += other;
+            }
+        }
+        const uint32_t past = __ballot_sync(0xffffffffu, begin < carry + inclusive);
+        if (past != 0) {
+            const int at = __ffs(past) - 1;
+            walk.sequence = base + at;
+            carry += __shfl_sync(0xffffffffu, inclusive - mine, at);
+            break;
+        }
+        carry += __shfl_sync(0xffffffffu, inclusive, 31);
+    }
+    if (walk.left > 0) {
+        walk.info = sequence_info(p, walk.sequence);
+        const long long head_line = sm.sequence_line[walk.sequence];
+        walk.head = static_cast<int>((begin - carry) / head_line);
+        carry += walk.head * head_line;
+        // ... and the tile
+        const int tiles = item_tiles(walk.info);
+        for (int base = 0; base < tiles; base += 32) {
+            const long long mine = base + lane < tiles ? item_units(walk.info, base + lane) + kItemLead : 0;
+            long long inclusive = mine;
+#pragma unroll
+            for (int offset = 1; offset < 32; offset <<= 1) {
+                const long long other = __shfl_up_sync(0xffffffffu, inclusive, offset);
+                if (lane >= offset) {
+                    inclusive += other;
+                }
+            }
+            const uint32_t past = __ballot_sync(0xffffffffu, begin < carry + inclusive);
+            if (past != 0) {
+                const int at = __ffs(past) - 1;
+                walk.tile = base + at;
+                carry += __shfl_sync(0xffffffffu, inclusive - mine, at);
+                break;
+            }
+            carry += __shfl_sync(0xffffffffu, inclusive, 31);
+        }
+        walk.skip = begin - carry;
+        walk.at = carry;
+    }
+    if (lane == 0) {
+        sm.start = walk;
+        sm.total = total;
+    }
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+    chunk_attention_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map,
+                           const __grid_constant__ Params p) {
+    extern __shared__ unsigned char smem_raw[];
+    Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+    const int lane = threadIdx.x & 31;
+    const int warp = threadIdx.x >> 5;
+    const int rank = static_cast<int>(cluster_rank());
+    const int pair = blockIdx.x >> 1;
+    const int pairs = gridDim.x >> 1;
+
+    pdl_launch_dependents();
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
+                     "r"(kTmemColumns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+    if (threadIdx.x == kFetchWarp * 32) {
+        for (int i = 0; i < kRawStages; ++i) {
+            mbar_init(&sm.raw_k_full[i], 1);
+            mbar_init(&sm.raw_k_empty[i], kWidenWarps);
+            mbar_init(&sm.raw_v_full[i], 1);
+            mbar_init(&sm.raw_v_empty[i], kWidenWarps);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&sm.k_full[i], 2 * kWidenWarps);
+            mbar_init(&sm.k_empty[i], 1);
+            mbar_init(&sm.s_full[i], 1);
+            mbar_init(&sm.p_full[i], 2 * 4);
+            mbar_init(&sm.o_done[i], 1);
+        }
+        mbar_init(&sm.v_full, 2 * kWidenWarps);
+        mbar_init(&sm.v_empty, 1);
+        mbar_init(&sm.q_full, 2 * kWidenWarps);
+        mbar_init(&sm.q_free, 1 + 4);
+        mbar_init(&sm.scales_ready, kWidenWarps);
+        mbar_init(&sm.o_free, 2 * 4);
+        sm.failed = 0;
+        mbar_fence_init();
+    }
+    fence_proxy_async();
+    __syncthreads();
+    pair_sync();  // (the other CTA's shared memory is there)
+    pdl_wait();
+    if (rank == 0 && threadIdx.x < 2) {
+        // both CTAs of a pair go by what the first one finds in the status word
+        const uint32_t stop = status_is_set(p.status) ? 1u : 0u;
+        asm volatile(
+            "{\n"
+            ".reg .b32 remote;\n"
+            "mapa.shared::cluster.u32 remote, %0, %1;\n"
+            "st.shared::cluster.u32 [remote], %2;\n"
+            "}\n" ::"r"(smem_u32(&sm.stop)),
+            "r"(threadIdx.x), "r"(stop)
+            : "memory");
+    }
+    find_start(p, sm, pair, pairs);
+    __syncthreads();
+    pair_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sm.tmem_base);
+    const auto info = [&](int sequence) { return sequence_info(p, sequence); };
+    ChunkWalk walk = sm.start;
+    if (*reinterpret_cast<volatile int*>(&sm.stop) != 0) {
+        walk.left = 0;
+    }
+    ChunkPiece piece;
+    bool ok = true;
+    int g = 0;     // units so far
+    int item = 0;  // pieces so far
+
+    if (warp == kFetchWarp) {
+        // ---------------- lanes 0-7: K, 16 tokens x 128 bytes each; lanes 8-15: V ------------------
+        const bool keys = lane < 8;
+        const int token = keys ? rank * kKeyTokens + (lane >> 1) * kBoxTokens : (lane - 8) * kBoxTokens;  // of the unit
+        const int x = keys ? (lane & 1) * 128 : rank * 128;
+        const int offset = keys ? (lane & 1) * kKeyTokens * 128 + (lane >> 1) * kBoxBytes : (lane - 8) * kBoxBytes;
+        for (bool first = true; ok && next_piece(walk, first, p.sequences, info, piece); first = false) {
+            const uint32_t* table = p.block_tables + static_cast<size_t>(walk.sequence) * p.max_blocks;
+            for (int unit = piece.unit_begin; unit < piece.unit_end; ++unit, ++g) {
+                const int slot = g % kRawStages;
+                const uint32_t parity = ((g / kRawStages) & 1) ^ 1;
+                const long long position = static_cast<long long>(unit) * kUnit + token;
+                int row = -kBoxTokens;  // in front of the cache: zeros
+                if (lane < 16 && position < walk.info.context) {
+                    const uint32_t page = __ldg(table + position / p.page_size);
+                    if (page < static_cast<uint32_t>(p.num_blocks)) {
+                        row = (static_cast<int>(page) * kKvHeads + walk.head) * p.page_size +
+                              static_cast<int>(position % p.page_size);
+                    }
+                }
+                ok = wait(&sm.raw_k_empty[slot], parity, sm, p.status);
+                if (!ok) {
+                    break;
+                }
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&sm.raw_k_full[slot], kRawBytes);
+                }
+                __syncwarp();
+                if (lane < 8) {
+                    tma_box_g2s(sm.raw_k[slot] + offset, &key_map, x, row, &sm.raw_k_full[slot]);
+                }
+                __syncwarp();
+                ok = wait(&sm.raw_v_empty[slot], parity, sm, p.status);
+                if (lane == 0) {
+                    // (asked for or not: what is left out on giving up is not waited for)
+                    if (ok) {
+                        mbar_arrive_expect_tx(&sm.raw_v_full[slot], kRawBytes);
+                    }
+                }
+                __syncwarp();
+                if (ok && lane >= 8 && lane < 16) {
+                    tma_box_g2s(sm.raw_v[slot] + offset, &value_map, x, row, &sm.raw_v_full[slot]);
+                }
+                __syncwarp();
+                if (!ok) {
+                    ++g;  // its keys are on their way
+                    break;
+                }
+            }
+        }
+    } else if (warp == kMmaWarp) {
+        // ---------------- tensor-core issue, for both CTAs ------------------------------------------
+        if (rank == 0) {
+            const uint32_t idesc_scores = (1u << 4) | (static_cast<uint32_t>(kUnit >> 3) << 17) | (16u << 24);
+            const uint32_t idesc_output = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(kHeadDim >> 3) << 17) | (16u << 24);
+            const uint32_t q_base = smem_u32(sm.q), v_base = smem_u32(sm.v);
+            // P V of unit n of the piece, number `number` of all
+            const auto issue_output = [&](int number, bool first_unit) {
+                const int buffer = number & 1;
+                if (!wait(&sm.p_full[buffer], (number >> 1) & 1, sm, p.status) ||
+                    !wait(&sm.v_full, number & 1, sm, p.status)) {
+                    return false;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (elect_one()) {
+#pragma unroll
+                    for (int ks = 0; ks < kUnit / 16; ++ks) {
+                        pair_mma_ts(tmem_base + kOutputColumn, tmem_base + buffer * kUnit + ks * 8,
+                                    operand(v_base + ks * 2048, kValueBlock), idesc_output, first_unit && ks == 0 ? 0u : 1u);
+                    }
+                    pair_commit(&sm.v_empty);
+                    pair_commit(&sm.o_done[buffer]);
+                }
+                __syncwarp();
+                return true;
+            };
+            for (bool first = true; ok && next_piece(walk, first, p.sequences, info, piece); first = false) {
+                ok = wait(&sm.q_full, item & 1, sm, p.status);
+                for (int unit = piece.unit_begin; ok && unit < piece.unit_end; ++unit, ++g) {
+                    const int buffer = g & 1;
+                    ok = wait(&sm.k_full[buffer], (g >> 1) & 1, sm, p.status);
+                    if (!ok) {
+                        break;
+                    }
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (elect_one()) {
+                        const uint32_t k_base = smem_u32(sm.k[buffer]);
+#pragma unroll
+                        for (int ks = 0; ks < kHeadDim / 16; ++ks) {
+                            pair_mma_ss(tmem_base + buffer * kUnit, operand(q_base + (ks >> 2) * kQueryBlock + (ks & 3) * 32, 16),
+                                        operand(k_base + (ks >> 2) * kKeyBlock + (ks & 3) * 32, 16), idesc_scores, ks > 0 ? 1u : 0u);
+                        }
+                        pair_commit(&sm.s_full[buffer]);
+                        pair_commit(&sm.k_empty[buffer]);
+                        if (unit == piece.unit_end - 1) {
+                            pair_commit(&sm.q_free);
+                        }
+                    }
+                    __syncwarp();
+                    if (unit == piece.unit_begin) {
+                        // O of the item before has been read
+                        ok = wait(&sm.o_free, (item & 1) ^ 1, sm, p.status);
+                    } else {
+                        ok = issue_output(g - 1, unit == piece.unit_begin + 1);
+                    }
+                }
+                if (ok) {
+                    ok = issue_output(g - 1, piece.unit_end - piece.unit_begin == 1);
+                }
+                ++item;
+            }
+        }
+    } else if (warp >= kFirstWidenWarp) {
+        // ---------------- Q, K and V to f16 -------------------------------------------------------------
+        const int me = warp - kFirstWidenWarp;
+        const auto widen_keys = [&](int number) {
+            const int slot = number % kRawStages;
+            const int buffer = number & 1;
+            if (!wait(&sm.raw_k_full[slot], (number / kRawStages) & 1, sm, p.status) ||
+                !wait(&sm.k_empty[buffer], ((number >> 1) & 1) ^ 1, sm, p.status)) {
+                return false;
+            }
+#pragma unroll 4
+            for (int i = me; i < 32; i += kWidenWarps) {  // half of the dims, eight tokens, half of a raw row
+                const int block = i >> 3, rows = (i & 7) * 8;
+                widen_rows(sm.raw_k[slot] + (block >> 1) * (kKeyTokens * 128) + rows * 128,
+                           sm.k[buffer] + block * kKeyBlock + rows * 128, block & 1, lane);
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.raw_k_empty[slot]);
+                arrive_first(&sm.k_full[buffer]);
+            }
+            return true;
+        };
+        const auto widen_values = [&](int number) {
+            const int slot = number % kRawStages;
+            if (!wait(&sm.raw_v_full[slot], (number / kRawStages) & 1, sm, p.status) ||
+                !wait(&sm.v_empty, (number & 1) ^ 1, sm, p.status)) {
+                return false;
+            }
+#pragma unroll 4
+            for (int i = me; i < 32; i += kWidenWarps) {
+                const int block = i & 1, rows = (i >> 1) * 8;
+                widen_rows(sm.raw_v[slot] + rows * 128, sm.v + block * kValueBlock + rows * 128, block, lane);
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.raw_v_empty[slot]);
+                arrive_first(&sm.v_full);
+            }
+            return true;
+        };
+        for (bool first = true; ok && next_piece(walk, first, p.sequences, info, piece); first = false) {
+            ok = wait(&sm.q_free, (item & 1) ^ 1, sm, p.status);
+            if (!ok) {
+                break;
+            }
+            // eight dims per lane, 32 rows per warp
+            const int first_token = walk.tile * kItemTokens + rank * kRowTokens;
+#pragma unroll 1
+            for (int base = 0; base < kRows / kWidenWarps; base += 4) {
+                uint4 raw[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = me * (kRows / kWidenWarps) + base + j;
+                    const int token = first_token + r / kGqaGroup;
+                    raw[j] = make_uint4(0, 0, 0, 0);
+                    if (r < kRowTokens * kGqaGroup && token < walk.info.length) {
+                        raw[j] = __ldg(reinterpret_cast<const uint4*>(
+                                           p.query + ((static_cast<size_t>(walk.info.begin) + token) * kQueryHeads +
+                                                      walk.head * kGqaGroup + r % kGqaGroup) * kHeadDim) + lane);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int r = me * (kRows / kWidenWarps) + base + j;
+                    const uint32_t words[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+                    uint32_t highest = 0;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        highest = max(highest, max(words[i] & 0x7fffu, (words[i] >> 16) & 0x7fffu));
+                    }
+                    highest = __reduce_max_sync(0xffffffffu, highest);
+                    // the largest element to [2^14, 2^15); infinities and NaN stay what they are, and rows that are
+                    // (nearly) zero are not blown up without end
+                    const uint32_t exponent = max(highest >> 7, 64u);
+                    const float up = exponent == 255u ? 1.0f : __uint_as_float((127u + 14u + 127u - exponent) << 23);
+                    float x[8];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        x[2 * i] = __uint_as_float(words[i] << 16) * up;
+                        x[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u) * up;
+                    }
+                    *reinterpret_cast<uint4*>(sm.q + (lane >> 3) * kQueryBlock + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) =
+                        make_uint4(pack_f16(x[0], x[2]), pack_f16(x[1], x[3]), pack_f16(x[4], x[6]), pack_f16(x[5], x[7]));
+                    if (lane == 0) {
+                        sm.row_scale[r] = exponent == 255u ? 1.0f : __uint_as_float((exponent - 14u) << 23);
+                    }
+                }
+            }
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.scales_ready);
+                arrive_first(&sm.q_full);
+            }
+            ok = widen_keys(g);
+            for (int unit = piece.unit_begin; ok && unit < piece.unit_end; ++unit, ++g) {
+                if (unit + 1 < piece.unit_end) {
+                    ok = widen_keys(g + 1);
+                }
+                ok = ok && widen_values(g);
+            }
+            ++item;
+        }
+        // the last commits have arrived in this CTA's shared memory before it ends
+        if (ok && g > 0) {
+            ok = (g < 2 || wait(&sm.k_empty[g & 1], ((g - 2) >> 1) & 1, sm, p.status)) &&
+                 wait(&sm.k_empty[(g - 1) & 1], ((g - 1) >> 1) & 1, sm, p.status) && wait(&sm.v_empty, (g - 1) & 1, sm, p.status) && wait(&sm.q_free, (item - 1) & 1, sm, p.status);
+        }
+    } else {
+        // ---------------- softmax: thread = row -----------------------------------------------------
+        const int r = threadIdx.x;
+        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+        const int row_token = r / kGqaGroup;
+        if (r == 0 && rank == 0) {
+            p.merge[pair].sequence = -1;  // nothing to merge, until an item turns out to be cut
+        }
+        for (bool first = true; ok && next_piece(walk, first, p.sequences, info, piece); first = false) {
+            ok = wait(&sm.scales_ready, item & 1, sm, p.status);
+            if (!ok) {
+                break;
+            }
+            const int token = walk.tile * kItemTokens + rank * kRowTokens + row_token;  // of the chunk
+            const bool live = r < kRowTokens * kGqaGroup && token < walk.info.length;
+            // positions that the row sees, and that every live row of the CTA sees
+            const int visible = live ? walk.info.context - walk.info.length + token + 1 : 0;
+            const int visible_to_all = walk.info.context - walk.info.length + walk.tile * kItemTokens + rank * kRowTokens + 1;
+            // scores in log2 (keys have been widened to 2^-8 of themselves)
+            const float scale = fmaxf(
+                p.softmax_scale * kLog2e * (p.key_scales ? p.key_scales[walk.head] : 1.0f) * 256.0f * sm.row_scale[r], 1e-37f);
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.q_free);
+            }
+            float reference = -INFINITY;  // log2
+            float sum = 0.0f;
+            for (int unit = piece.unit_begin; unit < piece.unit_end; ++unit, ++g) {
+                const int buffer = g & 1;
+                ok = wait(&sm.s_full[buffer], (g >> 1) & 1, sm, p.status);
+                if (!ok) {
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                uint32_t loaded[kUnit / 32][32];
+#pragma unroll
+                for (int c = 0; c < kUnit / 32; ++c) {
+                    tmem_load32_issue(t_lane + buffer * kUnit + c * 32, loaded[c]);
+                }
+                tmem_load_wait();
+                float s[kUnit];
+#pragma unroll
+                for (int i = 0; i < kUnit; ++i) {
+                    asm volatile("" : "+r"(loaded[i / 32][i % 32]));  // (not to be taken before the wait)
+                    s[i] = __uint_as_float(loaded[i / 32][i % 32]);
+                }
+                if ((unit + 1) * static_cast<long long>(kUnit) > visible_to_all) {
+                    const long long limit = static_cast<long long>(visible) - static_cast<long long>(unit) * kUnit;
+                    const int seen = limit > kUnit ? kUnit : limit < 0 ? 0 : static_cast<int>(limit);
+#pragma unroll
+                    for (int i = 0; i < kUnit; ++i) {
+                        s[i] = i < seen ? s[i] : -INFINITY;
+                    }
+                }
+                float highest[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                for (int i = 4; i < kUnit; i += 8) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        highest[j] = i + 4 + j < kUnit ? max3(highest[j], s[i + j], s[i + 4 + j]) : fmaxf(highest[j], s[i + j]);
+                    }
+                }
+                const float top = fmaxf(fmaxf(highest[0], highest[1]), fmaxf(highest[2], highest[3])) * scale;
+                // (a row without any score keeps its reference, and none at all counts as 0)
+                const bool grown = top > reference + kRescaleAbove;
+                if (__any_sync(0xffffffffu, grown)) {
+                    const float factor = grown ? exp2_fast(reference - top) : 1.0f;
+                    if (unit > piece.unit_begin) {
+                        // the first unit's O is not added to anything; after it, wait for the one before this
+                        ok = wait(&sm.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, sm, p.status);
+                        if (!ok) {
+                            break;
+                        }
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                        for (int c = 0; c < kHeadDim / 32; ++c) {
+                            uint32_t part[32];
+                            tmem_load32_issue(t_lane + kOutputColumn + c * 32, part);
+                            tmem_load_wait();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                asm volatile("" : "+r"(part[i]));
+                                part[i] = __float_as_uint(__uint_as_float(part[i]) * factor);
+                            }
+                            tmem_store32(t_lane + kOutputColumn + c * 32, part);
+                        }
+                        tmem_store_wait();
+                    }
+                    sum *= factor;
+                    reference = grown ? top : reference;
+                }
+                const float minus = reference == -INFINITY ? 0.0f : -reference;
+                float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    uint32_t packed[32];
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int at = c * 64 + 2 * i;
+                        const float lo = exp2_fast(fmaf(s[at], scale, minus));
+                        const float hi = exp2_fast(fmaf(s[at + 1], scale, minus));
+                        sums[i & 3] += lo + hi;
+                        packed[i] = pack_f16(lo, hi);
+                    }
+                    tmem_store32(t_lane + buffer * kUnit + c * 32, packed);
+                }
+                sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
+                tmem_store_wait();
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    arrive_first(&sm.p_full[buffer]);
+                }
+            }
+            if (!ok) {
+                break;
+            }
+            // ---- the piece's result
+            const bool whole = piece.unit_begin == 0 && piece.unit_end == piece.units;
+            const int slot = 2 * pair + (piece.unit_begin == 0 ? 1 : 0);
+            const size_t partial_row = static_cast<size_t>(slot) * kSlotRows + rank * kRows + r;
+            if (!whole && piece.unit_begin == 0 && r == 0 && rank == 0) {
+                MergeItem merge;
+                merge.sequence = walk.sequence;
+                merge.head = walk.head;
+                merge.tile = walk.tile;
+                merge.last_pair = worker_of(sm.total, walk.item_end - 1, plan_workers(sm.total, pairs));
+                merge.first_row = walk.info.begin + walk.tile * kItemTokens;
+                merge.rows = min(kItemTokens, walk.info.length - walk.tile * kItemTokens);
+                p.merge[pair] = merge;
+            }
+            const float inverse = sum > 0.0f || isnan(sum) ? 256.0f / sum : 0.0f;  // (values are 2^-8 of themselves, too)
+            const size_t row = static_cast<size_t>(walk.info.begin) + token;
+            const int head = walk.head * kGqaGroup + r % kGqaGroup;
+            const float v_scale = inverse * (p.value_scales ? p.value_scales[walk.head] : 1.0f);
+            const __nv_bfloat16* gate_row = p.gate + row * p.gate_stride + head * (2 * kHeadDim) + kHeadDim;
+            // (a barrier for every second unit: P V of the unit before may still run, and on one barrier the parity of
+            // this one would be that of the one before it)
+            ok = wait(&sm.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, sm, p.status);
+            if (!ok) {
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+            for (int c = 0; c < kHeadDim / 32; ++c) {
+                uint32_t part[32];
+                uint4 gates[4] = {};
+                if (whole && p.gate != nullptr && live) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        gates[i] = __ldg(reinterpret_cast<const uint4*>(gate_row + c * 32) + i);
+                    }
+                }
+                __syncwarp();
+                tmem_load32_issue(t_lane + kOutputColumn + c * 32, part);
+                tmem_load_wait();
+                float value[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    asm volatile("" : "+r"(part[i]));
+                    // columns 4 i .. + 3 are dims 4 i + 0, 2, 1, 3
+                    value[(i & ~3) | ((i & 1) << 1) | ((i >> 1) & 1)] = __uint_as_float(part[i]);
+                }
+                if (live && !whole) {
+                    uint4* to = reinterpret_cast<uint4*>(p.partial_out + partial_row * kHeadDim + c * 32);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        to[i] = make_uint4(pack_f16(value[8 * i] * inverse, value[8 * i + 1] * inverse),
+                                           pack_f16(value[8 * i + 2] * inverse, value[8 * i + 3] * inverse),
+                                           pack_f16(value[8 * i + 4] * inverse, value[8 * i + 5] * inverse),
+                                           pack_f16(value[8 * i + 6] * inverse, value[8 * i + 7] * inverse));
+                    }
+                } else if (live) {
+                    uint4* to = reinterpret_cast<uint4*>(p.output + (row * kQueryHeads + head) * kHeadDim + c * 32);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t words[4];
+                        const uint32_t gate_words[4] = {gates[i].x, gates[i].y, gates[i].z, gates[i].w};
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            float lo = value[8 * i + 2 * j] * v_scale, hi = value[8 * i + 2 * j + 1] * v_scale;
+                            if (p.gate != nullptr) {
+                                lo *= 1.0f / (1.0f + __expf(-__uint_as_float(gate_words[j] << 16)));
+                                hi *= 1.0f / (1.0f + __expf(-__uint_as_float(gate_words[j] & 0xffff0000u)));
+                            }
+                            const __nv_bfloat162 both = __floats2bfloat162_rn(lo, hi);
+                            words[j] = *reinterpret_cast<const uint32_t*>(&both);
+                        }
+                        to[i] = make_uint4(words[0], words[1], words[2], words[3]);
+                    }
+                }
+                __syncwarp();
+            }
+            if (!whole && live) {
+                p.partial_stats[partial_row] = {reference, sum};
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                arrive_first(&sm.o_free);
+            }
+            ++item;
+        }
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (*reinterpret_cast<volatile int*>(&sm.failed) != 0) {
+        // A wait gave up somewhere.  What was asked for and arrives by itself is waited for, 0.2 ms at most for each.
+        const auto arrived = [](uint64_t* bar, uint32_t parity) {
+            const long long start = clock64();
+            while (!try_wait_cluster(bar, parity) && clock64() - start < 400000ll) {
+            }
+        };
+        if (warp == kFetchWarp) {
+            for (int i = g > kRawStages ? g - kRawStages : 0; i < g; ++i) {
+                arrived(&sm.raw_k_full[i % kRawStages], (i / kRawStages) & 1);
+                arrived(&sm.raw_v_full[i % kRawStages], (i / kRawStages) & 1);
+            }
+        } else if (warp == kMmaWarp && rank == 0 && g > 0) {
+            arrived(&sm.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1);
+            arrived(&sm.v_empty, (g - 1) & 1);
+            if (g > 1) {
+                arrived(&sm.v_empty, g & 1);
+            }
+        }
+    }
+    __syncthreads();
+    pair_sync();  // nobody leaves while the other may still arrive at its barriers, or while MMAs read its memory
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemColumns) : "memory");
+    }
+}
+
+// Items that were cut: a pair's last item began there and went on with the pairs after it.  A warp per row, eight dims
+// per lane, the pieces in order.
+constexpr int kMergeWarps = 8;
+
+__global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const __grid_constant__ Params p) {
+    pdl_launch_dependents();
+    pdl_wait();
+    const int pair = blockIdx.x;
+    const MergeItem item = p.merge[pair];
+    if (item.sequence < 0) {
+        return;
+    }
+    const int lane = threadIdx.x & 31;
+    const int index = blockIdx.y * kMergeWarps + (threadIdx.x >> 5);  // token and head of the group
+    const int token = index / kGqaGroup;
+    if (token >= item.rows) {
+        return;
+    }
+    const int r = (token / kRowTokens) * kRows + (token % kRowTokens) * kGqaGroup + index % kGqaGroup;
+    float maximum = -INFINITY;
+    for (int w = pair + lane; w <= item.last_pair; w += 32) {
+        const PartialStats stats = p.partial_stats[(2 * static_cast<size_t>(w) + (w == pair ? 1 : 0)) * kSlotRows + r];
+        if (!(stats.sum <= 0.0f)) {
+            maximum = fmaxf(maximum, stats.maximum);
+        }
+    }
+#pragma unroll
+    for (int offset = 16; offset > 0; offset >>= 1) {
+        maximum = fmaxf(maximum, __shfl_xor_sync(0xffffffffu, maximum, offset));
+    }
+    float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+    float denominator = 0.0f;
+#pragma unroll 4
+    for (int w = pair; w <= item.last_pair; ++w) {
+        const size_t at = (2 * static_cast<size_t>(w) + (w == pair ? 1 : 0)) * kSlotRows + r;
+        const PartialStats stats = p.partial_stats[at];
+        const uint4 raw = reinterpret_cast<const uint4*>(p.partial_out + at * kHeadDim)[lane];
+        const float weight = !(stats.sum <= 0.0f) ? stats.sum * exp2f(stats.maximum - maximum) : 0.0f;
+        denominator += weight;
+        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&words[i]));
+            acc[2 * i] = fmaf(weight, f.x, acc[2 * i]);
+            acc[2 * i + 1] = fmaf(weight, f.y, acc[2 * i + 1]);
+        }
+    }
+    const float v_scale = p.value_scales ? p.value_scales[item.head] : 1.0f;
+    const float inverse = denominator > 0.0f || isnan(denominator) ? v_scale / denominator : 0.0f;
+    const size_t row = static_cast<size_t>(item.first_row) + token;
+    const int head = item.head * kGqaGroup + index % kGqaGroup;
+    uint32_t gate_words[4] = {0, 0, 0, 0};
+    if (p.gate != nullptr) {
+        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p.gate + row * p.gate_stride + head * (2 * kHeadDim) + kHeadDim) + lane);
+        gate_words[0] = raw.x;
+        gate_words[1] = raw.y;
+        gate_words[2] = raw.z;
+        gate_words[3] = raw.w;
+    }
+    uint32_t words[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        float lo = acc[2 * j] * inverse, hi = acc[2 * j + 1] * inverse;
+        if (p.gate != nullptr) {
+            lo *= 1.0f / (1.0f + __expf(-__uint_as_float(gate_words[j] << 16)));
+            hi *= 1.0f / (1.0f + __expf(-__uint_as_float(gate_words[j] & 0xffff0000u)));
+        }
+        const __nv_bfloat162 both = __floats2bfloat162_rn(lo, hi);
+        words[j] = *reinterpret_cast<const uint32_t*>(&both);
+    }
+    reinterpret_cast<uint4*>(p.output + (row * kQueryHeads + head) * kHeadDim)[lane] = make_uint4(words[0], words[1], words[2], words[3]);
 }
 
 }  // namespace
 }  // namespace qwc
 
-extern "C" size_t qwc_paged_attention_chunk_workspace_bytes(void) { return 0; }
+extern "C" size_t qwc_paged_attention_chunk_workspace_bytes(void) { return qwc::kWorkspaceBytes; }
 
 extern "C" int qwc_paged_attention_chunk_fp8(const void* query, const void* query_gate_projection, const void* key_cache,
                                              const void* value_cache, const void* block_tables,
@@ -149,21 +1010,77 @@ extern "C" int qwc_paged_attention_chunk_fp8(const void* query, const void* quer
         gate_stride = kQueryHeads * 2 * kHeadDim;
     }
     if (query == nullptr || key_cache == nullptr || value_cache == nullptr || block_tables == nullptr ||
-        context_lengths == nullptr || chunk_begins == nullptr || output == nullptr || tokens <= 0 ||
+        context_lengths == nullptr || chunk_begins == nullptr || output == nullptr || workspace == nullptr || tokens <= 0 ||
         tokens > kMaxChunkTokens || sequences <= 0 || sequences > kMaxChunkSequences || max_blocks <= 0 ||
         (page_size != 16 && page_size != 64) || static_cast<long long>(max_blocks) * page_size > 0x7fffffffll ||
         num_blocks <= 0 || static_cast<long long>(num_blocks) * kKvHeads * page_size > 0x7fffffffll ||
         gate_stride < kQueryHeads * 2 * kHeadDim || gate_stride % 8 != 0 || !isfinite(softmax_scale) ||
         softmax_scale <= 0.0f || !aligned(query) || !aligned(query_gate_projection) || !aligned(key_cache) ||
-        !aligned(value_cache) || !aligned(output) || !aligned(workspace) ||
-        workspace_bytes < qwc_paged_attention_chunk_workspace_bytes()) {
+        !aligned(value_cache) || !aligned(output) || !aligned(workspace) || workspace_bytes < kWorkspaceBytes) {
         return cudaErrorInvalidValue;
     }
-    return launch_chained(chunk_attention_kernel, dim3(tokens, kKvHeads), dim3(kWarps * 32), 0, stream,
-                          static_cast<const __nv_bfloat16*>(query), static_cast<const __nv_bfloat16*>(query_gate_projection),
-                          static_cast<const uint8_t*>(key_cache), static_cast<const uint8_t*>(value_cache),
-                          static_cast<const uint32_t*>(block_tables), static_cast<const uint32_t*>(context_lengths),
-                          static_cast<const uint32_t*>(chunk_begins), key_scales, value_scales,
-                          static_cast<__nv_bfloat16*>(output), tokens, sequences, max_blocks, page_size, num_blocks,
-                          gate_stride, softmax_scale);
+    int* status = status_ptr();
+    if (status == nullptr) {
+        return cudaErrorInvalidValue;
+    }
+    const int shared = static_cast<int>(sizeof(Smem)) + 1024;
+    struct Setup {
+        cudaError_t error;
+        int pairs;
+    };
+    static PerDevice<Setup> per_device;
+    const Setup* setup = per_device.get([shared]() {
+        Setup found = {cudaSuccess, 0};
+        int device = 0, sms = 0;
+        found.error = cudaFuncSetAttribute(chunk_attention_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, shared);
+        if (found.error == cudaSuccess) {
+            found.error = cudaGetDevice(&device);
+        }
+        if (found.error == cudaSuccess) {
+            found.error = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+        }
+        found.pairs = sms / 2 < 1 ? 1 : sms / 2 > kMaxPairs ? kMaxPairs : sms / 2;
+        return found;
+    });
+    if (setup == nullptr) {
+        return cudaErrorInvalidDevice;
+    }
+    if (setup->error != cudaSuccess) {
+        return setup->error;
+    }
+    CUtensorMap key_map, value_map;
+    const long long rows = static_cast<long long>(num_blocks) * kKvHeads * page_size;
+    cudaError_t error = encode_pages(&key_map, key_cache, rows);
+    if (error == cudaSuccess) {
+        error = encode_pages(&value_map, value_cache, rows);
+    }
+    if (error != cudaSuccess) {
+        return error;
+    }
+    Params p;
+    p.query = static_cast<const __nv_bfloat16*>(query);
+    p.gate = static_cast<const __nv_bfloat16*>(query_gate_projection);
+    p.block_tables = static_cast<const uint32_t*>(block_tables);
+    p.context_lengths = static_cast<const uint32_t*>(context_lengths);
+    p.begins = static_cast<const uint32_t*>(chunk_begins);
+    p.key_scales = key_scales;
+    p.value_scales = value_scales;
+    p.output = static_cast<__nv_bfloat16*>(output);
+    p.partial_out = static_cast<__half*>(workspace);
+    p.partial_stats = reinterpret_cast<PartialStats*>(static_cast<char*>(workspace) + kOutBytes);
+    p.merge = reinterpret_cast<MergeItem*>(static_cast<char*>(workspace) + kOutBytes + kStatsBytes);
+    p.tokens = tokens;
+    p.sequences = sequences;
+    p.max_blocks = max_blocks;
+    p.page_size = page_size;
+    p.num_blocks = num_blocks;
+    p.gate_stride = gate_stride;
+    p.softmax_scale = softmax_scale;
+    p.status = status;
+    error = launch_chained(chunk_attention_kernel, dim3(2 * setup->pairs), dim3(kThreads), shared, stream, key_map, value_map, p);
+    if (error != cudaSuccess) {
+        return error;
+    }
+    return launch_chained(chunk_merge_kernel, dim3(setup->pairs, (kItemTokens * kGqaGroup + kMergeWarps - 1) / kMergeWarps),
+                          dim3(kMergeWarps * 32), 0, stream, p);
 }
