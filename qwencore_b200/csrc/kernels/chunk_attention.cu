@@ -6,25 +6,29 @@
 //
 // Bound by the tensor cores once a chunk has more than a few dozen tokens: 4 * 256 flops for each (row, position).
 // Two SMs of a pair work on one item (chunk_plan.h), 42 tokens x 6 heads of a KV head: 126 rows each, of 128.  For every
-// unit of 128 positions tcgen05.mma.cta_group::2 computes S = Q K^T and O += P V for all 256 rows; an SM fetches and widens
-// half of the operands, 64 of the keys and 128 of the value's dims, which is why it is a pair: alone, an SM would have to
-// widen twice as much as its integer pipes do beside the softmax.
+// unit of 128 positions tcgen05.mma.cta_group::2 computes S = Q K^T and O += P V for all 256 rows; an SM fetches half of
+// the operands, 64 of the keys and 128 of the value's dims, which is why it is a pair: alone, an SM would widen twice as
+// many values, and read twice as much shared memory for the tensor cores.
 //
-//   * operands are f16.  An e4m3 is moved bit by bit into an f16 that is 2^-8 of it, exactly (a shift and two masks for two of
-//     them; the factor goes into the scales).  A code that is no number becomes a finite one, so that it does no harm
-//     where a probability is zero.  Queries are brought to 2^15 by a power of two per row: a bf16's eight bits fit f16's
-//     eleven for 29 binades below the row's largest element.  The mask and the shifts take bytes 0 and 2, 1 and 3 of a
-//     word together, so the dims of K, Q and V lie in that order, and the columns of O are put right when it is stored;
-//   * a thread is a row of S: no shuffles.  Probabilities go back as f16 into the tensor memory of their scores, as the A
-//     operand of P V (rounded to eleven bits; their fp32 values are summed).  The running maximum that they refer to
-//     follows the scores only when these have grown by 2^8, so that O, which stays in tensor memory for the whole item, is
-//     hardly ever rescaled;
+//   * keys enter as they are stored (kind::f8f6f4).  A row's query is brought to [128, 256) by a power of two and becomes the
+//     sum of an e4m3 and an e5m2, one multiplication each: four bits, and then what they leave in three, which holds a
+//     bf16's eight bits for 14 binades below the row's largest element.  What is lost below, times the largest key there can
+//     be, bounds the error of a score; where that is more than 2^-13 for any row of an item, the item's keys are
+//     widened to f16 like the values, and its queries are f16, which hold eight bits for 29 binades;
+//   * values are widened: an e4m3 is moved bit by bit into an f16 that is 2^-8 of it, exactly (a shift and two masks for two
+//     of them; the factor goes into the scales).  A code that is no number becomes a finite one, so that it does no harm
+//     where a probability is zero.  The masks take bytes 0 and 2, 1 and 3 of a word together, so the columns of O lie in
+//     that order, and are put right when it is stored;
+//   * two threads share a row of S, 64 columns each.  Probabilities go back as f16 into the tensor memory of their scores, as
+//     the A operand of P V (rounded to eleven bits; their fp32 values are summed).  The running maximum that they refer to
+//     follows the scores only when these have grown by 2^8, so that O, which stays in tensor memory for the whole
+//     item, is hardly ever rescaled;
 //   * tensor memory: two buffers of scores (2 x 128 columns) and O (256 columns).  S of unit n + 1 is issued before P V of unit n.
 //
-//   warps 0-3   softmax, and the item's result
-//   warps 4-7   widen Q, K and V
-//   warp 8      fetches K and V, rings of two stages
-//   warp 9      issues the MMAs (in the pair's first CTA)
+//   warps 0-7   softmax, and the item's result
+//   warps 8-11  the query's digits, widening
+//   warp 12     fetches K and V, rings of three and two stages
+//   warp 13     issues the MMAs (in the pair's first CTA)
 
 #include "chunk.cuh"
 #include "chunk_plan.h"
@@ -33,11 +37,12 @@
 namespace qwc {
 namespace {
 
-constexpr int kThreads = 320;
-constexpr int kFirstWidenWarp = 4;
+constexpr int kSoftmaxWarps = 8;
+constexpr int kFirstWidenWarp = kSoftmaxWarps;
 constexpr int kWidenWarps = 4;
-constexpr int kFetchWarp = 8;
-constexpr int kMmaWarp = 9;
+constexpr int kFetchWarp = kFirstWidenWarp + kWidenWarps;
+constexpr int kMmaWarp = kFetchWarp + 1;
+constexpr int kThreads = (kMmaWarp + 1) * 32;
 constexpr int kRowTokens = kItemTokens / 2;              // of a CTA's rows
 constexpr int kRows = 128;                               // ... 126 of them used
 constexpr int kUnit = kPlanUnitTokens;
@@ -45,30 +50,37 @@ constexpr int kKeyTokens = kUnit / 2;                    // of a unit that a CTA
 constexpr int kBoxTokens = 16;
 constexpr int kBoxBytes = kBoxTokens * 128;
 constexpr int kRawBytes = kKeyTokens * kHeadDim;         // K of a unit, or V: 16 KiB
-constexpr int kRawStages = 2;
+constexpr int kKeyStages = 3;                           // (values leave theirs when they are widened, keys when they have been used)
+constexpr int kValueStages = 2;
 constexpr int kKeyBlock = kKeyTokens * 128;              // 64 dims of the widened keys
 constexpr int kValueBlock = kUnit * 128;
 constexpr int kQueryBlock = kRows * 128;
+constexpr int kDigitBytes = 2 * kQueryBlock;             // a digit of the queries: [half of the dims][row][128 bytes]
 constexpr int kTmemColumns = 512;
 constexpr int kOutputColumn = 2 * kUnit;
 constexpr int kMaxPairs = 96;
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kRescaleAbove = 8.0f;                    // log2
+constexpr float kScoreError = 1.0f / 8192.0f;            // of a score, by digits that leave something
 static_assert(kPlanHeads == kKvHeads && kRowTokens * kGqaGroup <= kRows, "the plan's items");
 
 struct Smem {
-    uint8_t q[4 * kQueryBlock];               // [64 dims][row][128 bytes], f16, 128-byte swizzle
-    uint8_t k[2][4 * kKeyBlock];              // [64 dims][token][128 bytes]
-    uint8_t v[2 * kValueBlock];               // [64 dims][token][128 bytes]
-    uint8_t raw_k[kRawStages][kRawBytes];     // [half of the dims][token][128 bytes], e4m3, 128-byte swizzle
-    uint8_t raw_v[kRawStages][kRawBytes];     // [token][128 bytes]
-    uint64_t raw_k_full[kRawStages], raw_k_empty[kRawStages];
-    uint64_t raw_v_full[kRawStages], raw_v_empty[kRawStages];
-    uint64_t k_full[2], k_empty[2], v_full, v_empty;  // (k_full, v_full, q_full, p_full, o_free: the first CTA's count for both)
-    uint64_t q_full, q_free, scales_ready;
+    uint8_t q[4 * kQueryBlock];               // two digits, or f16 [64 dims][row][128 bytes]; 128-byte swizzle
+    uint8_t wide[2][2 * kValueBlock];         // V of a unit: [64 dims][token][128 bytes]; or V and K ([64 dims][token][128 bytes])
+    uint8_t raw_k[kKeyStages][kRawBytes];     // [half of the dims][token][128 bytes], e4m3, 128-byte swizzle
+    uint8_t raw_v[kValueStages][kRawBytes];     // [token][128 bytes]
+    uint64_t raw_k_full[kKeyStages], raw_k_empty[kKeyStages];
+    uint64_t raw_v_full[kValueStages], raw_v_empty[kValueStages];
+    // (those that the MMAs wait for, k_full, v_full, q_full, p_full, o_free: the first CTA's count for both)
+    uint64_t k_full[2], k_empty, v_full[2], v_empty[2];
+    uint64_t q_full, q_free, scales_ready, mode_ready;
     uint64_t s_full[2], p_full[2];
+    uint64_t max_ready[2][4], sum_ready[4];   // of the two warps that share 32 rows
     uint64_t o_done[2], o_free;
-    float row_scale[kRows];                   // what the row's query has been divided by
+    float row_max[2][2][kRows];
+    float row_sum[2][kRows];
+    float row_scale[kRows];                   // what the row's query times key has been divided by
+    uint32_t inexact[2 * kWidenWarps];        // rows whose digits leave too much, by warp of the pair
     long long sequence_line[kMaxChunkSequences];
     ChunkWalk start;
     long long total;
@@ -135,6 +147,20 @@ __device__ __forceinline__ void arrive_first(uint64_t* bar) {
         : "memory");
 }
 
+// ... of either CTA, after a word at the same place of its shared memory.
+__device__ __forceinline__ void tell(uint32_t* word, uint32_t value, uint64_t* bar, uint32_t rank) {
+    asm volatile(
+        "{\n"
+        ".reg .b32 remote;\n"
+        "mapa.shared::cluster.u32 remote, %0, %3;\n"
+        "st.shared::cluster.u32 [remote], %1;\n"
+        "mapa.shared::cluster.u32 remote, %2, %3;\n"
+        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [remote];\n"
+        "}\n" ::"r"(smem_u32(word)),
+        "r"(value), "r"(smem_u32(bar)), "r"(rank)
+        : "memory");
+}
+
 __device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
     uint32_t done;
     asm volatile(
@@ -190,7 +216,20 @@ __device__ __forceinline__ void pair_mma_ss(uint32_t d_tmem, uint64_t a_desc, ui
         : "memory");
 }
 
-// ... or tensor memory.
+// ... 32 eight-bit elements each ...
+__device__ __forceinline__ void pair_mma_fp8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                             uint32_t accumulate) {
+    asm volatile(
+        "{\n"
+        ".reg .pred p;\n"
+        "setp.ne.b32 p, %4, 0;\n"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n"
+        "}\n" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+
+// ... or A from tensor memory.
 __device__ __forceinline__ void pair_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc,
                                             uint32_t accumulate) {
     asm volatile(
@@ -251,6 +290,22 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     uint32_t out;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(out) : "f"(hi), "f"(lo));
     return out;
+}
+
+// Two numbers as e4m3 and, of what that leaves, as e5m2; the numbers become what is left at last.
+__device__ __forceinline__ void take_digits(float& lo, float& hi, uint32_t& d0, uint32_t& d1) {
+    uint16_t first, second;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(first) : "f"(hi), "f"(lo));
+    const uint32_t held = cvt_e4m3x2_to_f16x2(first);
+    const float2 value = __half22float2(*reinterpret_cast<const __half2*>(&held));
+    lo -= value.x;
+    hi -= value.y;
+    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(second) : "f"(hi), "f"(lo));
+    d0 = first;
+    d1 = second;
+    // an e5m2 is the upper byte of an f16
+    lo -= __half2float(__ushort_as_half(static_cast<unsigned short>(second << 8)));
+    hi -= __half2float(__ushort_as_half(static_cast<unsigned short>(second & 0xff00)));
 }
 
 // Four e4m3 -> two f16x2 of 2^-8 their value: bytes 0 and 2, bytes 1 and 3.
@@ -410,25 +465,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     }
     if (threadIdx.x == kFetchWarp * 32) {
-        for (int i = 0; i < kRawStages; ++i) {
+        for (int i = 0; i < kKeyStages; ++i) {
             mbar_init(&sm.raw_k_full[i], 1);
-            mbar_init(&sm.raw_k_empty[i], kWidenWarps);
+            mbar_init(&sm.raw_k_empty[i], 1 + kWidenWarps);
+        }
+        for (int i = 0; i < kValueStages; ++i) {
             mbar_init(&sm.raw_v_full[i], 1);
             mbar_init(&sm.raw_v_empty[i], kWidenWarps);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm.k_full[i], 2 * kWidenWarps);
-            mbar_init(&sm.k_empty[i], 1);
+            mbar_init(&sm.v_full[i], 2 * kWidenWarps);
+            mbar_init(&sm.v_empty[i], 1);
             mbar_init(&sm.s_full[i], 1);
-            mbar_init(&sm.p_full[i], 2 * 4);
+            mbar_init(&sm.p_full[i], 2 * kSoftmaxWarps);
             mbar_init(&sm.o_done[i], 1);
+            for (int j = 0; j < 4; ++j) {
+                mbar_init(&sm.max_ready[i][j], 2);
+            }
         }
-        mbar_init(&sm.v_full, 2 * kWidenWarps);
-        mbar_init(&sm.v_empty, 1);
+        for (int j = 0; j < 4; ++j) {
+            mbar_init(&sm.sum_ready[j], 2);
+        }
+        mbar_init(&sm.k_empty, 1);
         mbar_init(&sm.q_full, 2 * kWidenWarps);
-        mbar_init(&sm.q_free, 1 + 4);
+        mbar_init(&sm.q_free, 1 + kSoftmaxWarps);
         mbar_init(&sm.scales_ready, kWidenWarps);
-        mbar_init(&sm.o_free, 2 * 4);
+        mbar_init(&sm.mode_ready, 2 * kWidenWarps);
+        mbar_init(&sm.o_free, 2 * kSoftmaxWarps);
         sm.failed = 0;
         mbar_fence_init();
     }
@@ -468,43 +532,43 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         const bool keys = lane < 8;
         const int token = keys ? rank * kKeyTokens + (lane >> 1) * kBoxTokens : (lane - 8) * kBoxTokens;  // of the unit
         const int x = keys ? (lane & 1) * 128 : rank * 128;
+        const int page_shift = p.page_size == 16 ? 4 : 6;
         const int offset = keys ? (lane & 1) * kKeyTokens * 128 + (lane >> 1) * kBoxBytes : (lane - 8) * kBoxBytes;
         for (bool first = true; ok && next_piece(walk, first, p.sequences, info, piece); first = false) {
             const uint32_t* table = p.block_tables + static_cast<size_t>(walk.sequence) * p.max_blocks;
             for (int unit = piece.unit_begin; unit < piece.unit_end; ++unit, ++g) {
-                const int slot = g % kRawStages;
-                const uint32_t parity = ((g / kRawStages) & 1) ^ 1;
+                const int k_slot = g % kKeyStages, v_slot = g % kValueStages;
                 const long long position = static_cast<long long>(unit) * kUnit + token;
                 int row = -kBoxTokens;  // in front of the cache: zeros
                 if (lane < 16 && position < walk.info.context) {
-                    const uint32_t page = __ldg(table + position / p.page_size);
+                    const uint32_t page = __ldg(table + (position >> page_shift));
                     if (page < static_cast<uint32_t>(p.num_blocks)) {
-                        row = (static_cast<int>(page) * kKvHeads + walk.head) * p.page_size +
-                              static_cast<int>(position % p.page_size);
+                        row = (((static_cast<int>(page) * kKvHeads + walk.head) << page_shift) |
+                              static_cast<int>(position & (p.page_size - 1)));
                     }
                 }
-                ok = wait(&sm.raw_k_empty[slot], parity, sm, p.status);
+                ok = wait(&sm.raw_k_empty[k_slot], ((g / kKeyStages) & 1) ^ 1, sm, p.status);
                 if (!ok) {
                     break;
                 }
                 if (lane == 0) {
-                    mbar_arrive_expect_tx(&sm.raw_k_full[slot], kRawBytes);
+                    mbar_arrive_expect_tx(&sm.raw_k_full[k_slot], kRawBytes);
                 }
                 __syncwarp();
                 if (lane < 8) {
-                    tma_box_g2s(sm.raw_k[slot] + offset, &key_map, x, row, &sm.raw_k_full[slot]);
+                    tma_box_g2s(sm.raw_k[k_slot] + offset, &key_map, x, row, &sm.raw_k_full[k_slot]);
                 }
                 __syncwarp();
-                ok = wait(&sm.raw_v_empty[slot], parity, sm, p.status);
+                ok = wait(&sm.raw_v_empty[v_slot], ((g / kValueStages) & 1) ^ 1, sm, p.status);
                 if (lane == 0) {
                     // (asked for or not: what is left out on giving up is not waited for)
                     if (ok) {
-                        mbar_arrive_expect_tx(&sm.raw_v_full[slot], kRawBytes);
+                        mbar_arrive_expect_tx(&sm.raw_v_full[v_slot], kRawBytes);
                     }
                 }
                 __syncwarp();
                 if (ok && lane >= 8 && lane < 16) {
-                    tma_box_g2s(sm.raw_v[slot] + offset, &value_map, x, row, &sm.raw_v_full[slot]);
+                    tma_box_g2s(sm.raw_v[v_slot] + offset, &value_map, x, row, &sm.raw_v_full[v_slot]);
                 }
                 __syncwarp();
                 if (!ok) {
@@ -517,23 +581,26 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         // ---------------- tensor-core issue, for both CTAs ------------------------------------------
         if (rank == 0) {
             const uint32_t idesc_scores = (1u << 4) | (static_cast<uint32_t>(kUnit >> 3) << 17) | (16u << 24);
+            const uint32_t idesc_rest = idesc_scores | (1u << 7);  // A is e5m2
             const uint32_t idesc_output = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(kHeadDim >> 3) << 17) | (16u << 24);
-            const uint32_t q_base = smem_u32(sm.q), v_base = smem_u32(sm.v);
-            // P V of unit n of the piece, number `number` of all
+            const uint32_t q_base = smem_u32(sm.q);
+            bool widened = false;
+            // P V of unit number `number`
             const auto issue_output = [&](int number, bool first_unit) {
                 const int buffer = number & 1;
                 if (!wait(&sm.p_full[buffer], (number >> 1) & 1, sm, p.status) ||
-                    !wait(&sm.v_full, number & 1, sm, p.status)) {
+                    !wait(&sm.v_full[buffer], (number >> 1) & 1, sm, p.status)) {
                     return false;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 if (elect_one()) {
+                    const uint32_t v_base = smem_u32(sm.wide[widened ? 0 : buffer]);
 #pragma unroll
                     for (int ks = 0; ks < kUnit / 16; ++ks) {
                         pair_mma_ts(tmem_base + kOutputColumn, tmem_base + buffer * kUnit + ks * 8,
                                     operand(v_base + ks * 2048, kValueBlock), idesc_output, first_unit && ks == 0 ? 0u : 1u);
                     }
-                    pair_commit(&sm.v_empty);
+                    pair_commit(&sm.v_empty[buffer]);
                     pair_commit(&sm.o_done[buffer]);
                 }
                 __syncwarp();
@@ -541,6 +608,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             };
             for (bool first = true; ok && next_piece(walk, first, p.sequences, info, piece); first = false) {
                 ok = wait(&sm.q_full, item & 1, sm, p.status);
+                widened = __any_sync(0xffffffffu, lane < 2 * kWidenWarps && sm.inexact[lane & (2 * kWidenWarps - 1)] != 0);
                 for (int unit = piece.unit_begin; ok && unit < piece.unit_end; ++unit, ++g) {
                     const int buffer = g & 1;
                     ok = wait(&sm.k_full[buffer], (g >> 1) & 1, sm, p.status);
@@ -549,14 +617,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     if (elect_one()) {
-                        const uint32_t k_base = smem_u32(sm.k[buffer]);
+                        const uint32_t d = tmem_base + buffer * kUnit;
+                        if (!widened) {
+                            const uint32_t k_base = smem_u32(sm.raw_k[g % kKeyStages]);
 #pragma unroll
-                        for (int ks = 0; ks < kHeadDim / 16; ++ks) {
-                            pair_mma_ss(tmem_base + buffer * kUnit, operand(q_base + (ks >> 2) * kQueryBlock + (ks & 3) * 32, 16),
-                                        operand(k_base + (ks >> 2) * kKeyBlock + (ks & 3) * 32, 16), idesc_scores, ks > 0 ? 1u : 0u);
+                            for (int ks = 0; ks < kHeadDim / 32; ++ks) {
+                                const uint64_t keys = operand(k_base + (ks >> 2) * (kKeyTokens * 128) + (ks & 3) * 32, 16);
+                                const uint32_t a = q_base + (ks >> 2) * kQueryBlock + (ks & 3) * 32;
+                                pair_mma_fp8(d, operand(a, 16), keys, idesc_scores, ks > 0 ? 1u : 0u);
+                                pair_mma_fp8(d, operand(a + kDigitBytes, 16), keys, idesc_rest, 1u);
+                            }
+                        } else {
+                            const uint32_t k_base = smem_u32(sm.wide[1]);
+#pragma unroll
+                            for (int ks = 0; ks < kHeadDim / 16; ++ks) {
+                                pair_mma_ss(d, operand(q_base + (ks >> 2) * kQueryBlock + (ks & 3) * 32, 16),
+                                            operand(k_base + (ks >> 2) * kKeyBlock + (ks & 3) * 32, 16), idesc_scores, ks > 0 ? 1u : 0u);
+                            }
                         }
                         pair_commit(&sm.s_full[buffer]);
-                        pair_commit(&sm.k_empty[buffer]);
+                        pair_commit(&sm.raw_k_empty[g % kKeyStages]);
+                        pair_commit(&sm.k_empty);
                         if (unit == piece.unit_end - 1) {
                             pair_commit(&sm.q_free);
                         }
@@ -576,61 +657,65 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
         }
     } else if (warp >= kFirstWidenWarp) {
-        // ---------------- Q, K and V to f16 -------------------------------------------------------------
+        // ---------------- the query's digits; V (and K) to f16 ------------------------------------------
         const int me = warp - kFirstWidenWarp;
-        const auto widen_keys = [&](int number) {
-            const int slot = number % kRawStages;
-            const int buffer = number & 1;
-            if (!wait(&sm.raw_k_full[slot], (number / kRawStages) & 1, sm, p.status) ||
-                !wait(&sm.k_empty[buffer], ((number >> 1) & 1) ^ 1, sm, p.status)) {
+        constexpr int kWarpRows = kRows / kWidenWarps;
+        constexpr int kBatch = 16;  // rows in flight: eight dims per lane
+        bool widened = false, was_widened = false;
+        // keys of a unit: as they came, or widened
+        const auto pass_keys = [&](int number) {
+            const int slot = number % kKeyStages;
+            if (!wait(&sm.raw_k_full[slot], (number / kKeyStages) & 1, sm, p.status)) {
                 return false;
             }
+            if (widened) {
+                if (!wait(&sm.k_empty, (number & 1) ^ 1, sm, p.status)) {
+                    return false;
+                }
 #pragma unroll 4
-            for (int i = me; i < 32; i += kWidenWarps) {  // half of the dims, eight tokens, half of a raw row
-                const int block = i >> 3, rows = (i & 7) * 8;
-                widen_rows(sm.raw_k[slot] + (block >> 1) * (kKeyTokens * 128) + rows * 128,
-                           sm.k[buffer] + block * kKeyBlock + rows * 128, block & 1, lane);
+                for (int i = me; i < 32; i += kWidenWarps) {  // half of the dims, eight tokens, half of a raw row
+                    const int block = i >> 3, rows = (i & 7) * 8;
+                    widen_rows(sm.raw_k[slot] + (block >> 1) * (kKeyTokens * 128) + rows * 128,
+                               sm.wide[1] + block * kKeyBlock + rows * 128, block & 1, lane);
+                }
+                fence_proxy_async();
             }
-            fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&sm.raw_k_empty[slot]);
-                arrive_first(&sm.k_full[buffer]);
+                arrive_first(&sm.k_full[number & 1]);
             }
             return true;
         };
         const auto widen_values = [&](int number) {
-            const int slot = number % kRawStages;
-            if (!wait(&sm.raw_v_full[slot], (number / kRawStages) & 1, sm, p.status) ||
-                !wait(&sm.v_empty, (number & 1) ^ 1, sm, p.status)) {
+            const int slot = number % kValueStages;
+            const int buffer = number & 1;
+            if (!wait(&sm.raw_v_full[slot], (number / kValueStages) & 1, sm, p.status) ||
+                !wait(&sm.v_empty[buffer], ((number >> 1) & 1) ^ 1, sm, p.status) ||
+                // (all units in one buffer: the unit before, too)
+                (widened && number > 0 && !wait(&sm.v_empty[buffer ^ 1], ((number - 1) >> 1) & 1, sm, p.status))) {
                 return false;
             }
+            uint8_t* to = sm.wide[widened ? 0 : buffer];
 #pragma unroll 4
             for (int i = me; i < 32; i += kWidenWarps) {
                 const int block = i & 1, rows = (i >> 1) * 8;
-                widen_rows(sm.raw_v[slot] + rows * 128, sm.v + block * kValueBlock + rows * 128, block, lane);
+                widen_rows(sm.raw_v[slot] + rows * 128, to + block * kValueBlock + rows * 128, block, lane);
             }
             fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&sm.raw_v_empty[slot]);
-                arrive_first(&sm.v_full);
+                arrive_first(&sm.v_full[buffer]);
             }
             return true;
         };
         for (bool first = true; ok && next_piece(walk, first, p.sequences, info, piece); first = false) {
-            ok = wait(&sm.q_free, (item & 1) ^ 1, sm, p.status);
-            if (!ok) {
-                break;
-            }
-            // eight dims per lane, 32 rows per warp
             const int first_token = walk.tile * kItemTokens + rank * kRowTokens;
-#pragma unroll 1
-            for (int base = 0; base < kRows / kWidenWarps; base += 4) {
-                uint4 raw[4];
+            const auto fetch_rows = [&](int base, uint4 (&raw)[kBatch]) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = me * (kRows / kWidenWarps) + base + j;
+                for (int j = 0; j < kBatch; ++j) {
+                    const int r = me * kWarpRows + base + j;
                     const int token = first_token + r / kGqaGroup;
                     raw[j] = make_uint4(0, 0, 0, 0);
                     if (r < kRowTokens * kGqaGroup && token < walk.info.length) {
@@ -639,31 +724,97 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                                       walk.head * kGqaGroup + r % kGqaGroup) * kHeadDim) + lane);
                     }
                 }
+            };
+            // The row's numbers with its largest in [2^top, 2^(top + 1)), and what they are multiplied with to be what they
+            // were; infinities and NaN stay what they are, and rows that are (nearly) zero are not blown up without end.
+            const auto scale_row = [&](const uint4& raw, int top, float (&x)[8]) {
+                const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+                uint32_t highest = 0;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int r = me * (kRows / kWidenWarps) + base + j;
-                    const uint32_t words[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
-                    uint32_t highest = 0;
+                for (int i = 0; i < 4; ++i) {
+                    highest = max(highest, max(words[i] & 0x7fffu, (words[i] >> 16) & 0x7fffu));
+                }
+                highest = __reduce_max_sync(0xffffffffu, highest);
+                const uint32_t exponent = max(highest >> 7, 64u);
+                const float up = exponent == 255u ? 1.0f : __uint_as_float((254u + top - exponent) << 23);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        highest = max(highest, max(words[i] & 0x7fffu, (words[i] >> 16) & 0x7fffu));
-                    }
-                    highest = __reduce_max_sync(0xffffffffu, highest);
-                    // the largest element to [2^14, 2^15); infinities and NaN stay what they are, and rows that are
-                    // (nearly) zero are not blown up without end
-                    const uint32_t exponent = max(highest >> 7, 64u);
-                    const float up = exponent == 255u ? 1.0f : __uint_as_float((127u + 14u + 127u - exponent) << 23);
+                for (int i = 0; i < 4; ++i) {
+                    x[2 * i] = __uint_as_float(words[i] << 16) * up;
+                    x[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u) * up;
+                }
+                return exponent == 255u ? 1.0f : __uint_as_float((exponent - top) << 23);
+            };
+            uint4 raw[kBatch];
+            fetch_rows(0, raw);
+            ok = wait(&sm.q_free, (item & 1) ^ 1, sm, p.status);
+            if (!ok) {
+                break;
+            }
+            const float largest_key = 448.0f * p.softmax_scale * (p.key_scales ? fabsf(p.key_scales[walk.head]) : 1.0f);
+            bool exact = true;
+#pragma unroll 1
+            for (int base = 0; base < kWarpRows; base += kBatch) {
+                if (base > 0) {
+                    fetch_rows(base, raw);
+                }
+#pragma unroll
+                for (int j = 0; j < kBatch; ++j) {
+                    const int r = me * kWarpRows + base + j;
                     float x[8];
+                    const float scale = scale_row(raw[j], 7, x);
+                    uint32_t d0[4], d1[4];
+                    float left = 0.0f;
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        x[2 * i] = __uint_as_float(words[i] << 16) * up;
-                        x[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u) * up;
+                        take_digits(x[2 * i], x[2 * i + 1], d0[i], d1[i]);
+                        left += fabsf(x[2 * i]) + fabsf(x[2 * i + 1]);
                     }
-                    *reinterpret_cast<uint4*>(sm.q + (lane >> 3) * kQueryBlock + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) =
-                        make_uint4(pack_f16(x[0], x[2]), pack_f16(x[1], x[3]), pack_f16(x[4], x[6]), pack_f16(x[5], x[7]));
+                    // (in steps of 2^-26: what is left of an element is below 2^-13; a NaN or more counts as a lot)
+                    const uint32_t steps = left < 1.0f ? static_cast<uint32_t>(left * 67108864.0f) + 1u : 0x3ffffffu;
+                    const float lost = static_cast<float>(__reduce_add_sync(0xffffffffu, left == 0.0f ? 0u : steps)) * 1.4901161193847656e-8f;
+                    exact = exact && lost < 0.5f && lost * scale * largest_key <= kScoreError;
+                    uint8_t* to = sm.q + (lane >> 4) * kQueryBlock + r * 128 + ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
+                    *reinterpret_cast<uint2*>(to) = make_uint2(d0[0] | d0[1] << 16, d0[2] | d0[3] << 16);
+                    *reinterpret_cast<uint2*>(to + kDigitBytes) = make_uint2(d1[0] | d1[1] << 16, d1[2] | d1[3] << 16);
                     if (lane == 0) {
-                        sm.row_scale[r] = exponent == 255u ? 1.0f : __uint_as_float((exponent - 14u) << 23);
+                        sm.row_scale[r] = scale;
                     }
+                }
+            }
+            // the pair agrees
+            if (lane < 2) {
+                tell(&sm.inexact[rank * kWidenWarps + me], exact ? 0u : 1u, &sm.mode_ready, lane);
+            }
+            __syncwarp();
+            ok = wait(&sm.mode_ready, item & 1, sm, p.status);
+            if (!ok) {
+                break;
+            }
+            was_widened = widened;
+            widened = __any_sync(0xffffffffu, lane < 2 * kWidenWarps && sm.inexact[lane & (2 * kWidenWarps - 1)] != 0);
+            if (widened) {
+#pragma unroll 1
+                for (int base = 0; base < kWarpRows; base += kBatch) {
+                    fetch_rows(base, raw);
+#pragma unroll
+                    for (int j = 0; j < kBatch; ++j) {
+                        const int r = me * kWarpRows + base + j;
+                        float x[8];
+                        const float scale = scale_row(raw[j], 14, x);
+                        // (the dims in the order in which widened keys have them)
+                        *reinterpret_cast<uint4*>(sm.q + (lane >> 3) * kQueryBlock + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) =
+                            make_uint4(pack_f16(x[0], x[2]), pack_f16(x[1], x[3]), pack_f16(x[4], x[6]), pack_f16(x[5], x[7]));
+                        if (lane == 0) {
+                            sm.row_scale[r] = scale * 256.0f;
+                        }
+                    }
+                }
+            }
+            if ((widened || was_widened) && g > 0) {
+                // the buffers change their use: what has been issued has read them
+                ok = wait(&sm.v_empty[(g - 1) & 1], ((g - 1) >> 1) & 1, sm, p.status);
+                if (!ok) {
+                    break;
                 }
             }
             fence_proxy_async();
@@ -672,10 +823,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 mbar_arrive(&sm.scales_ready);
                 arrive_first(&sm.q_full);
             }
-            ok = widen_keys(g);
+            ok = pass_keys(g);
             for (int unit = piece.unit_begin; ok && unit < piece.unit_end; ++unit, ++g) {
                 if (unit + 1 < piece.unit_end) {
-                    ok = widen_keys(g + 1);
+                    ok = pass_keys(g + 1);
                 }
                 ok = ok && widen_values(g);
             }
@@ -683,15 +834,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
         // the last commits have arrived in this CTA's shared memory before it ends
         if (ok && g > 0) {
-            ok = (g < 2 || wait(&sm.k_empty[g & 1], ((g - 2) >> 1) & 1, sm, p.status)) &&
-                 wait(&sm.k_empty[(g - 1) & 1], ((g - 1) >> 1) & 1, sm, p.status) && wait(&sm.v_empty, (g - 1) & 1, sm, p.status) && wait(&sm.q_free, (item - 1) & 1, sm, p.status);
+            ok = (g < 2 || wait(&sm.v_empty[g & 1], ((g - 2) >> 1) & 1, sm, p.status)) &&
+                 wait(&sm.v_empty[(g - 1) & 1], ((g - 1) >> 1) & 1, sm, p.status) &&
+                 wait(&sm.q_free, (item - 1) & 1, sm, p.status);
+            for (int i = g > kKeyStages ? g - kKeyStages : 0; i < g && ok; ++i) {
+                ok = wait(&sm.raw_k_empty[i % kKeyStages], (i / kKeyStages) & 1, sm, p.status);
+            }
+            ok = ok && wait(&sm.k_empty, (g - 1) & 1, sm, p.status);
         }
     } else {
-        // ---------------- softmax: thread = row -----------------------------------------------------
-        const int r = threadIdx.x;
-        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+        // ---------------- softmax: two threads for a row ----------------------------------------------
+        constexpr int kColumns = kUnit / 2;  // of a thread
+        const int half = warp >> 2;
+        const int quarter = warp & 3;
+        const int r = quarter * 32 + lane;
+        const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
         const int row_token = r / kGqaGroup;
-        if (r == 0 && rank == 0) {
+        if (threadIdx.x == 0 && rank == 0) {
             p.merge[pair].sequence = -1;  // nothing to merge, until an item turns out to be cut
         }
         for (bool first = true; ok && next_piece(walk, first, p.sequences, info, piece); first = false) {
@@ -704,9 +863,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // positions that the row sees, and that every live row of the CTA sees
             const int visible = live ? walk.info.context - walk.info.length + token + 1 : 0;
             const int visible_to_all = walk.info.context - walk.info.length + walk.tile * kItemTokens + rank * kRowTokens + 1;
-            // scores in log2 (keys have been widened to 2^-8 of themselves)
-            const float scale = fmaxf(
-                p.softmax_scale * kLog2e * (p.key_scales ? p.key_scales[walk.head] : 1.0f) * 256.0f * sm.row_scale[r], 1e-37f);
+            // scores in log2
+            const float scale =
+                fmaxf(p.softmax_scale * kLog2e * (p.key_scales ? p.key_scales[walk.head] : 1.0f) * sm.row_scale[r], 1e-37f);
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&sm.q_free);
@@ -720,35 +879,45 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     break;
                 }
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                uint32_t loaded[kUnit / 32][32];
-#pragma unroll
-                for (int c = 0; c < kUnit / 32; ++c) {
-                    tmem_load32_issue(t_lane + buffer * kUnit + c * 32, loaded[c]);
-                }
+                uint32_t loaded[2][32];
+                tmem_load32_issue(t_lane + buffer * kUnit + half * kColumns, loaded[0]);
+                tmem_load32_issue(t_lane + buffer * kUnit + half * kColumns + 32, loaded[1]);
                 tmem_load_wait();
-                float s[kUnit];
+                float s[kColumns];
 #pragma unroll
-                for (int i = 0; i < kUnit; ++i) {
+                for (int i = 0; i < kColumns; ++i) {
                     asm volatile("" : "+r"(loaded[i / 32][i % 32]));  // (not to be taken before the wait)
                     s[i] = __uint_as_float(loaded[i / 32][i % 32]);
                 }
                 if ((unit + 1) * static_cast<long long>(kUnit) > visible_to_all) {
-                    const long long limit = static_cast<long long>(visible) - static_cast<long long>(unit) * kUnit;
-                    const int seen = limit > kUnit ? kUnit : limit < 0 ? 0 : static_cast<int>(limit);
+                    const long long limit = static_cast<long long>(visible) - static_cast<long long>(unit) * kUnit - half * kColumns;
+                    const int seen = limit > kColumns ? kColumns : limit < 0 ? 0 : static_cast<int>(limit);
 #pragma unroll
-                    for (int i = 0; i < kUnit; ++i) {
+                    for (int i = 0; i < kColumns; ++i) {
                         s[i] = i < seen ? s[i] : -INFINITY;
                     }
                 }
                 float highest[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                for (int i = 4; i < kUnit; i += 8) {
+                for (int i = 4; i < kColumns; i += 8) {
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        highest[j] = i + 4 + j < kUnit ? max3(highest[j], s[i + j], s[i + 4 + j]) : fmaxf(highest[j], s[i + j]);
+                        highest[j] = i + 4 + j < kColumns ? max3(highest[j], s[i + j], s[i + 4 + j]) : fmaxf(highest[j], s[i + j]);
                     }
                 }
-                const float top = fmaxf(fmaxf(highest[0], highest[1]), fmaxf(highest[2], highest[3])) * scale;
+                const float mine = fmaxf(fmaxf(highest[0], highest[1]), fmaxf(highest[2], highest[3]));
+                sm.row_max[buffer][half][r] = mine;
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&sm.max_ready[buffer][quarter]);
+                }
+                ok = wait(&sm.max_ready[buffer][quarter], (g >> 1) & 1, sm, p.status);
+                if (!ok) {
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const float top = fmaxf(mine, sm.row_max[buffer][half ^ 1][r]) * scale;
                 // (a row without any score keeps its reference, and none at all counts as 0)
                 const bool grown = top > reference + kRescaleAbove;
                 if (__any_sync(0xffffffffu, grown)) {
@@ -761,7 +930,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         }
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-                        for (int c = 0; c < kHeadDim / 32; ++c) {
+                        for (int c = half * 4; c < half * 4 + 4; ++c) {
                             uint32_t part[32];
                             tmem_load32_issue(t_lane + kOutputColumn + c * 32, part);
                             tmem_load_wait();
@@ -779,19 +948,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
                 const float minus = reference == -INFINITY ? 0.0f : -reference;
                 float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                uint32_t packed[32];
 #pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    uint32_t packed[32];
-#pragma unroll
-                    for (int i = 0; i < 32; ++i) {
-                        const int at = c * 64 + 2 * i;
-                        const float lo = exp2_fast(fmaf(s[at], scale, minus));
-                        const float hi = exp2_fast(fmaf(s[at + 1], scale, minus));
-                        sums[i & 3] += lo + hi;
-                        packed[i] = pack_f16(lo, hi);
-                    }
-                    tmem_store32(t_lane + buffer * kUnit + c * 32, packed);
+                for (int i = 0; i < 32; ++i) {
+                    const float lo = exp2_fast(fmaf(s[2 * i], scale, minus));
+                    const float hi = exp2_fast(fmaf(s[2 * i + 1], scale, minus));
+                    sums[i & 3] += lo + hi;
+                    packed[i] = pack_f16(lo, hi);
                 }
+                // (over scores of either half: both warps have read theirs when they met)
+                tmem_store32(t_lane + buffer * kUnit + half * 32, packed);
                 sum += (sums[0] + sums[1]) + (sums[2] + sums[3]);
                 tmem_store_wait();
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -807,7 +973,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const bool whole = piece.unit_begin == 0 && piece.unit_end == piece.units;
             const int slot = 2 * pair + (piece.unit_begin == 0 ? 1 : 0);
             const size_t partial_row = static_cast<size_t>(slot) * kSlotRows + rank * kRows + r;
-            if (!whole && piece.unit_begin == 0 && r == 0 && rank == 0) {
+            if (!whole && piece.unit_begin == 0 && threadIdx.x == 0 && rank == 0) {
                 MergeItem merge;
                 merge.sequence = walk.sequence;
                 merge.head = walk.head;
@@ -817,11 +983,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 merge.rows = min(kItemTokens, walk.info.length - walk.tile * kItemTokens);
                 p.merge[pair] = merge;
             }
-            const float inverse = sum > 0.0f || isnan(sum) ? 256.0f / sum : 0.0f;  // (values are 2^-8 of themselves, too)
+            sm.row_sum[half][r] = sum;
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.sum_ready[quarter]);
+            }
             const size_t row = static_cast<size_t>(walk.info.begin) + token;
             const int head = walk.head * kGqaGroup + r % kGqaGroup;
+            const int first_dim = half * (kHeadDim / 2);
+            const bool gated = whole && p.gate != nullptr && live;
+            const __nv_bfloat16* gate_row = p.gate + row * p.gate_stride + head * (2 * kHeadDim) + kHeadDim + first_dim;
+            uint4 gates[2][4] = {};
+            if (gated) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    gates[0][i] = __ldg(reinterpret_cast<const uint4*>(gate_row) + i);
+                }
+            }
+            ok = wait(&sm.sum_ready[quarter], item & 1, sm, p.status);
+            if (!ok) {
+                break;
+            }
+            sum += sm.row_sum[half ^ 1][r];
+            const float inverse = sum > 0.0f || isnan(sum) ? 256.0f / sum : 0.0f;  // (values are 2^-8 of themselves)
             const float v_scale = inverse * (p.value_scales ? p.value_scales[walk.head] : 1.0f);
-            const __nv_bfloat16* gate_row = p.gate + row * p.gate_stride + head * (2 * kHeadDim) + kHeadDim;
             // (a barrier for every second unit: P V of the unit before may still run, and on one barrier the parity of
             // this one would be that of the one before it)
             ok = wait(&sm.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, sm, p.status);
@@ -829,18 +1014,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll 1
-            for (int c = 0; c < kHeadDim / 32; ++c) {
+#pragma unroll
+            for (int c = 0; c < kHeadDim / 64; ++c) {
                 uint32_t part[32];
-                uint4 gates[4] = {};
-                if (whole && p.gate != nullptr && live) {
+                if (gated && c + 1 < kHeadDim / 64) {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        gates[i] = __ldg(reinterpret_cast<const uint4*>(gate_row + c * 32) + i);
+                        gates[(c + 1) & 1][i] = __ldg(reinterpret_cast<const uint4*>(gate_row + (c + 1) * 32) + i);
                     }
                 }
                 __syncwarp();
-                tmem_load32_issue(t_lane + kOutputColumn + c * 32, part);
+                tmem_load32_issue(t_lane + kOutputColumn + first_dim + c * 32, part);
                 tmem_load_wait();
                 float value[32];
 #pragma unroll
@@ -850,7 +1034,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     value[(i & ~3) | ((i & 1) << 1) | ((i >> 1) & 1)] = __uint_as_float(part[i]);
                 }
                 if (live && !whole) {
-                    uint4* to = reinterpret_cast<uint4*>(p.partial_out + partial_row * kHeadDim + c * 32);
+                    uint4* to = reinterpret_cast<uint4*>(p.partial_out + partial_row * kHeadDim + first_dim + c * 32);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         to[i] = make_uint4(pack_f16(value[8 * i] * inverse, value[8 * i + 1] * inverse),
@@ -859,17 +1043,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                            pack_f16(value[8 * i + 6] * inverse, value[8 * i + 7] * inverse));
                     }
                 } else if (live) {
-                    uint4* to = reinterpret_cast<uint4*>(p.output + (row * kQueryHeads + head) * kHeadDim + c * 32);
+                    uint4* to = reinterpret_cast<uint4*>(p.output + (row * kQueryHeads + head) * kHeadDim + first_dim + c * 32);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         uint32_t words[4];
-                        const uint32_t gate_words[4] = {gates[i].x, gates[i].y, gates[i].z, gates[i].w};
+                        const uint4 here = gates[c & 1][i];
+                        const uint32_t gate_words[4] = {here.x, here.y, here.z, here.w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             float lo = value[8 * i + 2 * j] * v_scale, hi = value[8 * i + 2 * j + 1] * v_scale;
-                            if (p.gate != nullptr) {
-                                lo *= 1.0f / (1.0f + __expf(-__uint_as_float(gate_words[j] << 16)));
-                                hi *= 1.0f / (1.0f + __expf(-__uint_as_float(gate_words[j] & 0xffff0000u)));
+                            if (gated) {
+                                lo = __fdividef(lo, 1.0f + __expf(-__uint_as_float(gate_words[j] << 16)));
+                                hi = __fdividef(hi, 1.0f + __expf(-__uint_as_float(gate_words[j] & 0xffff0000u)));
                             }
                             const __nv_bfloat162 both = __floats2bfloat162_rn(lo, hi);
                             words[j] = *reinterpret_cast<const uint32_t*>(&both);
@@ -879,7 +1064,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
                 __syncwarp();
             }
-            if (!whole && live) {
+            if (!whole && live && half == 0) {
                 p.partial_stats[partial_row] = {reference, sum};
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -900,15 +1085,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
         };
         if (warp == kFetchWarp) {
-            for (int i = g > kRawStages ? g - kRawStages : 0; i < g; ++i) {
-                arrived(&sm.raw_k_full[i % kRawStages], (i / kRawStages) & 1);
-                arrived(&sm.raw_v_full[i % kRawStages], (i / kRawStages) & 1);
+            for (int i = g > kKeyStages ? g - kKeyStages : 0; i < g; ++i) {
+                arrived(&sm.raw_k_full[i % kKeyStages], (i / kKeyStages) & 1);
+            }
+            for (int i = g > kValueStages ? g - kValueStages : 0; i < g; ++i) {
+                arrived(&sm.raw_v_full[i % kValueStages], (i / kValueStages) & 1);
             }
         } else if (warp == kMmaWarp && rank == 0 && g > 0) {
             arrived(&sm.s_full[(g - 1) & 1], ((g - 1) >> 1) & 1);
-            arrived(&sm.v_empty, (g - 1) & 1);
+            arrived(&sm.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1);
             if (g > 1) {
-                arrived(&sm.v_empty, g & 1);
+                arrived(&sm.o_done[g & 1], ((g - 2) >> 1) & 1);
             }
         }
     }

@@ -195,6 +195,28 @@ def test_attention_chunk_flat_and_steep_scores(cuda, ops, std):
     assert ((got - want).abs() <= bound).all()
 
 
+@pytest.mark.parametrize("rows", [slice(None), slice(50, 51), slice(0, 300, 90)])
+def test_attention_chunk_queries_with_an_outlier(cuda, ops, rows):
+    # one element of a million times the others, where all keys are zero: the others decide
+    case = Attention(cuda, 14, [300, 40], [700, 90], 16)
+    case.caches[0][..., 17] = 0
+    case.query[rows, :, 17] = 1.0e6
+    case.check(ops)
+
+
+def test_attention_chunk_queries_that_are_no_numbers(cuda, ops):
+    case = Attention(cuda, 15, [100, 50], [300, 0], 16)
+    want, spread = case.want()
+    case.query[30, 7, 5] = float("nan")
+    case.query[120, 3, 9] = float("inf")
+    got = case.run(ops).double()
+    broken = cuda.zeros((150, HEADS), dtype=cuda.bool, device="cuda")
+    broken[30, 7] = broken[120, 3] = True
+    assert got[30, 7].isnan().all()
+    close = (got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * spread
+    assert close[~broken].all()
+
+
 def test_attention_chunk_one_large_weight_and_many_small(cuda, ops):
     # a first token that draws half of every row's weight, the rest spread over thousands
     case = Attention(cuda, 12, [40], [8000], 16, gated=False)
