@@ -71,16 +71,19 @@ struct Smem {
     uint8_t raw_v[kValueStages][kRawBytes];     // [token][128 bytes]
     uint64_t raw_k_full[kKeyStages], raw_k_empty[kKeyStages];
     uint64_t raw_v_full[kValueStages], raw_v_empty[kValueStages];
-    // (those that the MMAs wait for, k_full, v_full, q_full, p_full, o_free: the first CTA's count for both)
-    uint64_t k_full[kKeyStages], k_empty, v_full[2], v_empty[2];
-    uint64_t q_full, q_free, scales_ready, mode_ready;
+    // (those that the MMAs wait for, k_peer, k_wide, v_full, q_full, q_wide, p_full, o_free: the first CTA's count)
+    uint64_t k_peer[kKeyStages];              // the other CTA's keys are there
+    uint64_t k_wide, k_empty, v_full[2], v_empty[2];
+    uint64_t q_full, q_wide, q_free, scales_ready;
+    uint64_t flags_ready, mode_ready;         // of the words inexact and mode
     uint64_t s_full[2], p_full[2];
     uint64_t max_ready[2][4], sum_ready[4];   // of the two warps that share 32 rows
     uint64_t o_done[2], o_free;
     float row_max[2][2][kRows];
     float row_sum[2][kRows];
     float row_scale[kRows];                   // what the row's query times key has been divided by
-    uint32_t inexact[2 * kWidenWarps];        // rows whose digits leave too much, by warp of the pair
+    uint32_t inexact[2 * kWidenWarps];        // rows whose digits leave too much, by warp of the pair (first CTA)
+    uint32_t mode;                            // what follows from that: queries and keys are widened
     long long sequence_line[kMaxChunkSequences];
     ChunkWalk start;
     long long total;
@@ -121,6 +124,7 @@ struct Params {
     PartialStats* partial_stats;
     MergeItem* merge;
     int tokens, sequences, max_blocks, page_size, num_blocks, gate_stride;
+    int wide_rows;  // gate, output and partial rows begin on 32-byte boundaries
     float softmax_scale;
     int* status;
 };
@@ -149,32 +153,17 @@ __device__ __forceinline__ void arrive_first(uint64_t* bar) {
         : "memory");
 }
 
-// ... of either CTA, after a word at the same place of its shared memory.
+// A word for the same place of a CTA's shared memory; its four bytes count at the barrier beside it.
 __device__ __forceinline__ void tell(uint32_t* word, uint32_t value, uint64_t* bar, uint32_t rank) {
     asm volatile(
         "{\n"
-        ".reg .b32 remote;\n"
+        ".reg .b32 remote, barrier;\n"
         "mapa.shared::cluster.u32 remote, %0, %3;\n"
-        "st.shared::cluster.u32 [remote], %1;\n"
-        "mapa.shared::cluster.u32 remote, %2, %3;\n"
-        "mbarrier.arrive.release.cluster.shared::cluster.b64 _, [remote];\n"
+        "mapa.shared::cluster.u32 barrier, %2, %3;\n"
+        "st.async.shared::cluster.mbarrier::complete_tx::bytes.u32 [remote], %1, [barrier];\n"
         "}\n" ::"r"(smem_u32(word)),
         "r"(value), "r"(smem_u32(bar)), "r"(rank)
         : "memory");
-}
-
-__device__ __forceinline__ bool try_wait_cluster(uint64_t* bar, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        "selp.u32 %0, 1, 0, p;\n"
-        "}\n"
-        : "=r"(done)
-        : "r"(smem_u32(bar)), "r"(parity)
-        : "memory");
-    return done != 0;
 }
 
 // Every role marches unit by unit with the others, so no wait is long: it gives up after 20 ms.
@@ -294,20 +283,20 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     return out;
 }
 
-// Two numbers as e4m3 and, of what that leaves, as e5m2; the numbers become what is left at last.
-__device__ __forceinline__ void take_digits(float& lo, float& hi, uint32_t& d0, uint32_t& d1) {
+// Two numbers below 256 as e4m3 and, of what that leaves, as e5m2, in f16 arithmetic; returns the magnitudes of what is left
+// at last.  (A warp has its scheduler's attention for an instruction every three or four cycles here: what counts is how
+// few there are.  Rounding to e5m2 with integer operations instead of conversions was slower, fp32 arithmetic too.)
+__device__ __forceinline__ __half2 take_digits(float lo, float hi, uint32_t& d0, uint32_t& d1) {
+    const uint32_t bits = pack_f16(lo, hi);
     uint16_t first, second;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(first) : "f"(hi), "f"(lo));
+    asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(first) : "r"(bits));
     const uint32_t held = cvt_e4m3x2_to_f16x2(first);
-    const float2 value = __half22float2(*reinterpret_cast<const __half2*>(&held));
-    lo -= value.x;
-    hi -= value.y;
-    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(second) : "f"(hi), "f"(lo));
+    const __half2 rest = __hsub2(*reinterpret_cast<const __half2*>(&bits), *reinterpret_cast<const __half2*>(&held));
+    asm("cvt.rn.satfinite.e5m2x2.f16x2 %0, %1;" : "=h"(second) : "r"(*reinterpret_cast<const uint32_t*>(&rest)));
     d0 = first;
     d1 = second;
-    // an e5m2 is the upper byte of an f16
-    lo -= __half2float(__ushort_as_half(static_cast<unsigned short>(second << 8)));
-    hi -= __half2float(__ushort_as_half(static_cast<unsigned short>(second & 0xff00)));
+    const uint32_t upper = __byte_perm(d1, 0u, 0x1404);  // an e5m2 is the upper byte of an f16
+    return __habs2(__hsub2(rest, *reinterpret_cast<const __half2*>(&upper)));
 }
 
 // Four e4m3 -> two f16x2 of 2^-8 their value: bytes 0 and 2, bytes 1 and 3.
@@ -330,6 +319,42 @@ __device__ __forceinline__ void widen_rows(const uint8_t* raw, uint8_t* wide, in
     widen4(codes.w, hi.z, hi.w);
     *reinterpret_cast<uint4*>(wide + row * 128 + (((2 * piece) ^ row) << 4)) = lo;
     *reinterpret_cast<uint4*>(wide + row * 128 + (((2 * piece + 1) ^ row) << 4)) = hi;
+}
+
+// 64 bytes of a row, half of it at a time where the rows begin on 32-byte boundaries (`wide`): whole sectors, of 32 rows
+// in one instruction.
+__device__ __forceinline__ void load64(const void* from, int wide, uint4 (&to)[4]) {
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            asm volatile("ld.global.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+                         : "=r"(to[2 * i].x), "=r"(to[2 * i].y), "=r"(to[2 * i].z), "=r"(to[2 * i].w), "=r"(to[2 * i + 1].x),
+                           "=r"(to[2 * i + 1].y), "=r"(to[2 * i + 1].z), "=r"(to[2 * i + 1].w)
+                         : "l"(static_cast<const char*>(from) + 32 * i));
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            to[i] = reinterpret_cast<const uint4*>(from)[i];
+        }
+    }
+}
+
+__device__ __forceinline__ void store64(void* to, int wide, const uint4 (&from)[4]) {
+    if (wide) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(static_cast<char*>(to) + 32 * i),
+                         "r"(from[2 * i].x), "r"(from[2 * i].y), "r"(from[2 * i].z), "r"(from[2 * i].w), "r"(from[2 * i + 1].x),
+                         "r"(from[2 * i + 1].y), "r"(from[2 * i + 1].z), "r"(from[2 * i + 1].w)
+                         : "memory");
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            reinterpret_cast<uint4*>(to)[i] = from[i];
+        }
+    }
 }
 
 // Cache pages as rows of 256 bytes, fetched in boxes of 16 tokens x 128 bytes.  A row beyond the cache arrives as zeros.
@@ -469,8 +494,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (threadIdx.x == kFetchWarp * 32) {
         for (int i = 0; i < kKeyStages; ++i) {
             mbar_init(&sm.raw_k_full[i], 1);
-            mbar_init(&sm.raw_k_empty[i], 1 + kWidenWarps);
-            mbar_init(&sm.k_full[i], 2 * kWidenWarps);
+            mbar_init(&sm.raw_k_empty[i], 1);
+            mbar_init(&sm.k_peer[i], 1);
         }
         for (int i = 0; i < kValueStages; ++i) {
             mbar_init(&sm.raw_v_full[i], 1);
@@ -489,11 +514,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         for (int j = 0; j < 4; ++j) {
             mbar_init(&sm.sum_ready[j], 2);
         }
+        mbar_init(&sm.k_wide, 2 * kWidenWarps);
         mbar_init(&sm.k_empty, 1);
         mbar_init(&sm.q_full, 2 * kWidenWarps);
+        mbar_init(&sm.q_wide, 2 * kWidenWarps);
         mbar_init(&sm.q_free, 1 + kSoftmaxWarps);
         mbar_init(&sm.scales_ready, kWidenWarps);
-        mbar_init(&sm.mode_ready, 2 * kWidenWarps);
+        mbar_init(&sm.flags_ready, 1);
+        mbar_init(&sm.mode_ready, 1);
         mbar_init(&sm.o_free, 2 * kSoftmaxWarps);
         sm.failed = 0;
         mbar_fence_init();
@@ -587,6 +615,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const uint32_t idesc_output = (1u << 4) | (1u << 16) | (static_cast<uint32_t>(kHeadDim >> 3) << 17) | (16u << 24);
             const uint32_t q_base = smem_u32(sm.q);
             bool widened = false;
+            int wide_items = 0, wide_units = 0;
             // P V of unit number `number`
             const auto issue_output = [&](int number, bool first_unit) {
                 const int buffer = number & 1;
@@ -609,11 +638,29 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 return true;
             };
             for (bool first = true; ok && next_piece(walk, first, p.sequences, info, piece); first = false) {
-                ok = wait(&sm.q_full, item & 1, sm, p.status);
+                if (lane == 0) {
+                    mbar_arrive_expect_tx(&sm.flags_ready, 2 * kWidenWarps * 4);
+                }
+                __syncwarp();
+                ok = wait(&sm.q_full, item & 1, sm, p.status) && wait(&sm.flags_ready, item & 1, sm, p.status);
                 widened = __any_sync(0xffffffffu, lane < 2 * kWidenWarps && sm.inexact[lane & (2 * kWidenWarps - 1)] != 0);
+                if (ok && lane < 2) {
+                    tell(&sm.mode, widened ? 1u : 0u, &sm.mode_ready, lane);
+                }
+                __syncwarp();
+                if (ok && widened) {
+                    ok = wait(&sm.q_wide, wide_items & 1, sm, p.status);
+                    ++wide_items;
+                }
                 for (int unit = piece.unit_begin; ok && unit < piece.unit_end; ++unit, ++g) {
                     const int buffer = g & 1;
-                    ok = wait(&sm.k_full[g % kKeyStages], (g / kKeyStages) & 1, sm, p.status);
+                    if (!widened) {
+                        ok = wait(&sm.raw_k_full[g % kKeyStages], (g / kKeyStages) & 1, sm, p.status) &&
+                             wait(&sm.k_peer[g % kKeyStages], (g / kKeyStages) & 1, sm, p.status);
+                    } else {
+                        ok = wait(&sm.k_wide, wide_units & 1, sm, p.status);
+                        ++wide_units;
+                    }
                     if (!ok) {
                         break;
                     }
@@ -657,36 +704,40 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
                 ++item;
             }
+        } else {
+            // the second CTA's keys, told to the first
+            for (bool first = true; ok && next_piece(walk, first, p.sequences, info, piece); first = false) {
+                for (int unit = piece.unit_begin; ok && unit < piece.unit_end; ++unit, ++g) {
+                    ok = wait(&sm.raw_k_full[g % kKeyStages], (g / kKeyStages) & 1, sm, p.status);
+                    if (ok && lane == 0) {
+                        arrive_first(&sm.k_peer[g % kKeyStages]);
+                    }
+                    __syncwarp();
+                }
+            }
         }
     } else if (warp >= kFirstWidenWarp) {
         // ---------------- the query's digits; V (and K) to f16 ------------------------------------------
         const int me = warp - kFirstWidenWarp;
         constexpr int kWarpRows = kRows / kWidenWarps;
-        constexpr int kBatch = 16;  // rows in flight: eight dims per lane
+        constexpr int kAhead = 8;  // rows in flight, eight dims per lane
         bool widened = false, was_widened = false;
-        // keys of a unit: as they came, or widened
-        const auto pass_keys = [&](int number) {
+        const auto widen_keys = [&](int number) {
             const int slot = number % kKeyStages;
-            if (!wait(&sm.raw_k_full[slot], (number / kKeyStages) & 1, sm, p.status)) {
+            if (!wait(&sm.raw_k_full[slot], (number / kKeyStages) & 1, sm, p.status) ||
+                !wait(&sm.k_empty, (number & 1) ^ 1, sm, p.status)) {
                 return false;
             }
-            if (widened) {
-                if (!wait(&sm.k_empty, (number & 1) ^ 1, sm, p.status)) {
-                    return false;
-                }
 #pragma unroll 4
-                for (int i = me; i < 32; i += kWidenWarps) {  // half of the dims, eight tokens, half of a raw row
-                    const int block = i >> 3, rows = (i & 7) * 8;
-                    widen_rows(sm.raw_k[slot] + (block >> 1) * (kKeyTokens * 128) + rows * 128,
-                               sm.wide[1] + block * kKeyBlock + rows * 128, block & 1, lane);
-                }
-                fence_proxy_async();
+            for (int i = me; i < 32; i += kWidenWarps) {  // half of the dims, eight tokens, half of a raw row
+                const int block = i >> 3, rows = (i & 7) * 8;
+                widen_rows(sm.raw_k[slot] + (block >> 1) * (kKeyTokens * 128) + rows * 128,
+                           sm.wide[1] + block * kKeyBlock + rows * 128, block & 1, lane);
             }
+            fence_proxy_async();
             __syncwarp();
             if (lane == 0) {
-                // (as many barriers as stages: a warp comes back to one only when every other has been there)
-                mbar_arrive(&sm.raw_k_empty[slot]);
-                arrive_first(&sm.k_full[slot]);
+                arrive_first(&sm.k_wide);
             }
             return true;
         };
@@ -715,18 +766,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         };
         for (bool first = true; ok && next_piece(walk, first, p.sequences, info, piece); first = false) {
             const int first_token = walk.tile * kItemTokens + rank * kRowTokens;
-            const auto fetch_rows = [&](int base, uint4 (&raw)[kBatch]) {
-#pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
-                    const int r = me * kWarpRows + base + j;
-                    const int token = first_token + r / kGqaGroup;
-                    raw[j] = make_uint4(0, 0, 0, 0);
-                    if (r < kRowTokens * kGqaGroup && token < walk.info.length) {
-                        raw[j] = __ldg(reinterpret_cast<const uint4*>(
-                                           p.query + ((static_cast<size_t>(walk.info.begin) + token) * kQueryHeads +
-                                                      walk.head * kGqaGroup + r % kGqaGroup) * kHeadDim) + lane);
-                    }
+            const auto fetch_row = [&](int index) {
+                const int r = me * kWarpRows + index;
+                const int token = first_token + r / kGqaGroup;
+                uint4 raw = make_uint4(0, 0, 0, 0);
+                if (index < kWarpRows && r < kRowTokens * kGqaGroup && token < walk.info.length) {
+                    raw = __ldg(reinterpret_cast<const uint4*>(
+                                    p.query + ((static_cast<size_t>(walk.info.begin) + token) * kQueryHeads +
+                                               walk.head * kGqaGroup + r % kGqaGroup) * kHeadDim) + lane);
                 }
+                return raw;
             };
             // The row's numbers with its largest in [2^top, 2^(top + 1)), and what they are multiplied with to be what they
             // were; infinities and NaN stay what they are, and rows that are (nearly) zero are not blown up without end.
@@ -747,35 +796,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
                 return exponent == 255u ? 1.0f : __uint_as_float((exponent - top) << 23);
             };
-            uint4 raw[kBatch];
-            fetch_rows(0, raw);
+            uint4 raw[kAhead];
+#pragma unroll
+            for (int j = 0; j < kAhead; ++j) {
+                raw[j] = fetch_row(j);
+            }
             ok = wait(&sm.q_free, (item & 1) ^ 1, sm, p.status);
             if (!ok) {
                 break;
             }
             const float largest_key = 448.0f * p.softmax_scale * (p.key_scales ? fabsf(p.key_scales[walk.head]) : 1.0f);
-            bool exact = true;
+            // (Four rows at a time.  With all of them unrolled the warps waited for instructions: 30000 to 45000 cycles an
+            // item, now 13000.)
+            float lost = 0.0f;  // by this lane's elements, over all rows
+            float largest_scale = 0.0f;
 #pragma unroll 1
-            for (int base = 0; base < kWarpRows; base += kBatch) {
-                if (base > 0) {
-                    fetch_rows(base, raw);
+            for (int base = 0; base < kWarpRows; base += 4) {
+                const uint4 now[4] = {raw[0], raw[1], raw[2], raw[3]};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    raw[j] = raw[j + 4];
+                    raw[j + 4] = fetch_row(base + kAhead + j);
                 }
 #pragma unroll
-                for (int j = 0; j < kBatch; ++j) {
+                for (int j = 0; j < 4; ++j) {
                     const int r = me * kWarpRows + base + j;
                     float x[8];
-                    const float scale = scale_row(raw[j], 7, x);
+                    const float scale = scale_row(now[j], 7, x);
                     uint32_t d0[4], d1[4];
-                    float left = 0.0f;
+                    __half2 left = __float2half2_rn(0.0f);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        take_digits(x[2 * i], x[2 * i + 1], d0[i], d1[i]);
-                        left += fabsf(x[2 * i]) + fabsf(x[2 * i + 1]);
+                        left = __hadd2(left, take_digits(x[2 * i], x[2 * i + 1], d0[i], d1[i]));
                     }
-                    // (in steps of 2^-26: what is left of an element is below 2^-13; a NaN or more counts as a lot)
-                    const uint32_t steps = left < 1.0f ? static_cast<uint32_t>(left * 67108864.0f) + 1u : 0x3ffffffu;
-                    const float lost = static_cast<float>(__reduce_add_sync(0xffffffffu, left == 0.0f ? 0u : steps)) * 1.4901161193847656e-8f;
-                    exact = exact && lost < 0.5f && lost * scale * largest_key <= kScoreError;
+                    lost = fmaf(__low2float(left) + __high2float(left), scale, lost);
+                    largest_scale = fmaxf(largest_scale, scale);
                     uint8_t* to = sm.q + (lane >> 4) * kQueryBlock + r * 128 + ((((lane & 15) >> 1) ^ (r & 7)) << 4) + (lane & 1) * 8;
                     *reinterpret_cast<uint2*>(to) = make_uint2(d0[0] | d0[1] << 16, d0[2] | d0[3] << 16);
                     *reinterpret_cast<uint2*>(to + kDigitBytes) = make_uint2(d1[0] | d1[1] << 16, d1[2] | d1[3] << 16);
@@ -784,36 +839,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     }
                 }
             }
-            // the pair agrees
-            if (lane < 2) {
-                tell(&sm.inexact[rank * kWidenWarps + me], exact ? 0u : 1u, &sm.mode_ready, lane);
+            // A score of any row is off by no more than all rows' losses, and what f16 leaves of 256 elements (2^-25 of
+            // each at most), times the largest key.  (A NaN or an infinity among the queries: too much.)  The pair's first
+            // CTA decides.
+            const bool exact = __all_sync(0xffffffffu, lost < INFINITY) &&
+                               fmaf(largest_scale, 7.62939453125e-6f, warp_sum(lost)) * largest_key <= kScoreError;
+            fence_proxy_async();
+            __syncwarp();
+            if (lane == 0) {
+                arrive_first(&sm.q_full);
+                tell(&sm.inexact[rank * kWidenWarps + me], exact ? 0u : 1u, &sm.flags_ready, 0);
+                if (me == 0) {
+                    mbar_arrive_expect_tx(&sm.mode_ready, 4);
+                }
             }
             __syncwarp();
             ok = wait(&sm.mode_ready, item & 1, sm, p.status);
             if (!ok) {
                 break;
             }
-            try_wait_cluster(&sm.mode_ready, item & 1);  // (the other CTA's words: acquired at the pair's scope)
             was_widened = widened;
-            widened = __any_sync(0xffffffffu, lane < 2 * kWidenWarps && sm.inexact[lane & (2 * kWidenWarps - 1)] != 0);
-            if (widened) {
-#pragma unroll 1
-                for (int base = 0; base < kWarpRows; base += kBatch) {
-                    fetch_rows(base, raw);
-#pragma unroll
-                    for (int j = 0; j < kBatch; ++j) {
-                        const int r = me * kWarpRows + base + j;
-                        float x[8];
-                        const float scale = scale_row(raw[j], 14, x);
-                        // (the dims in the order in which widened keys have them)
-                        *reinterpret_cast<uint4*>(sm.q + (lane >> 3) * kQueryBlock + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) =
-                            make_uint4(pack_f16(x[0], x[2]), pack_f16(x[1], x[3]), pack_f16(x[4], x[6]), pack_f16(x[5], x[7]));
-                        if (lane == 0) {
-                            sm.row_scale[r] = scale * 256.0f;
-                        }
-                    }
-                }
-            }
+            widened = *reinterpret_cast<volatile uint32_t*>(&sm.mode) != 0;
             if ((widened || was_widened) && g > 0) {
                 // the buffers change their use: what has been issued has read them
                 ok = wait(&sm.v_empty[(g - 1) & 1], ((g - 1) >> 1) & 1, sm, p.status);
@@ -821,16 +867,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     break;
                 }
             }
-            fence_proxy_async();
+            if (widened) {
+#pragma unroll 2
+                for (int j = 0; j < kWarpRows; ++j) {
+                    const int r = me * kWarpRows + j;
+                    float x[8];
+                    const float scale = scale_row(fetch_row(j), 14, x);
+                    // (the dims in the order in which widened keys have them)
+                    *reinterpret_cast<uint4*>(sm.q + (lane >> 3) * kQueryBlock + r * 128 + (((lane & 7) ^ (r & 7)) << 4)) =
+                        make_uint4(pack_f16(x[0], x[2]), pack_f16(x[1], x[3]), pack_f16(x[4], x[6]), pack_f16(x[5], x[7]));
+                    if (lane == 0) {
+                        sm.row_scale[r] = scale * 256.0f;
+                    }
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) {
+                    arrive_first(&sm.q_wide);
+                }
+            }
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&sm.scales_ready);
-                arrive_first(&sm.q_full);
             }
-            ok = pass_keys(g);
+            // Into L2: the gates that this item ends with, 512 bytes of a row ...
+            if (p.gate != nullptr) {
+                const int r = me * kWarpRows + lane;
+                const int token = first_token + r / kGqaGroup;
+                if (r < kRowTokens * kGqaGroup && token < walk.info.length) {
+                    bulk_prefetch_l2(p.gate + (static_cast<size_t>(walk.info.begin) + token) * p.gate_stride +
+                                         (walk.head * kGqaGroup + r % kGqaGroup) * (2 * kHeadDim) + kHeadDim,
+                                     kHeadDim * 2);
+                }
+                __syncwarp();
+            }
+            {
+                // ... and the next item's queries, 6 heads of a token together
+                ChunkWalk ahead = walk;
+                ChunkPiece next;
+                if (me == 0 && next_piece(ahead, false, p.sequences, info, next)) {
+                    const int token = ahead.tile * kItemTokens + rank * kRowTokens + lane;
+                    if (lane < kRowTokens && token < ahead.info.length) {
+                        bulk_prefetch_l2(p.query + ((static_cast<size_t>(ahead.info.begin) + token) * kQueryHeads +
+                                                    ahead.head * kGqaGroup) * kHeadDim, kGqaGroup * kHeadDim * 2);
+                    }
+                    __syncwarp();
+                }
+            }
+            ok = !widened || widen_keys(g);
             for (int unit = piece.unit_begin; ok && unit < piece.unit_end; ++unit, ++g) {
-                if (unit + 1 < piece.unit_end) {
-                    ok = pass_keys(g + 1);
+                if (widened && unit + 1 < piece.unit_end) {
+                    ok = widen_keys(g + 1);
                 }
                 ok = ok && widen_values(g);
             }
@@ -997,12 +1084,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int first_dim = half * (kHeadDim / 2);
             const bool gated = whole && p.gate != nullptr && live;
             const __nv_bfloat16* gate_row = p.gate + row * p.gate_stride + head * (2 * kHeadDim) + kHeadDim + first_dim;
-            uint4 gates[2][4] = {};
+            uint4 gates[4] = {};
             if (gated) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    gates[0][i] = __ldg(reinterpret_cast<const uint4*>(gate_row) + i);
-                }
+                load64(gate_row, p.wide_rows, gates);
             }
             ok = wait(&sm.sum_ready[quarter], item & 1, sm, p.status);
             if (!ok) {
@@ -1018,14 +1102,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < kHeadDim / 64; ++c) {
                 uint32_t part[32];
+                const uint4 here[4] = {gates[0], gates[1], gates[2], gates[3]};
                 if (gated && c + 1 < kHeadDim / 64) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        gates[(c + 1) & 1][i] = __ldg(reinterpret_cast<const uint4*>(gate_row + (c + 1) * 32) + i);
-                    }
+                    load64(gate_row + (c + 1) * 32, p.wide_rows, gates);
                 }
                 __syncwarp();
                 tmem_load32_issue(t_lane + kOutputColumn + first_dim + c * 32, part);
@@ -1038,33 +1120,34 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     value[(i & ~3) | ((i & 1) << 1) | ((i >> 1) & 1)] = __uint_as_float(part[i]);
                 }
                 if (live && !whole) {
-                    uint4* to = reinterpret_cast<uint4*>(p.partial_out + partial_row * kHeadDim + first_dim + c * 32);
+                    uint4 out[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        to[i] = make_uint4(pack_f16(value[8 * i] * inverse, value[8 * i + 1] * inverse),
+                        out[i] = make_uint4(pack_f16(value[8 * i] * inverse, value[8 * i + 1] * inverse),
                                            pack_f16(value[8 * i + 2] * inverse, value[8 * i + 3] * inverse),
                                            pack_f16(value[8 * i + 4] * inverse, value[8 * i + 5] * inverse),
                                            pack_f16(value[8 * i + 6] * inverse, value[8 * i + 7] * inverse));
                     }
+                    store64(p.partial_out + partial_row * kHeadDim + first_dim + c * 32, p.wide_rows, out);
                 } else if (live) {
-                    uint4* to = reinterpret_cast<uint4*>(p.output + (row * kQueryHeads + head) * kHeadDim + first_dim + c * 32);
+                    uint4 out[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         uint32_t words[4];
-                        const uint4 here = gates[c & 1][i];
-                        const uint32_t gate_words[4] = {here.x, here.y, here.z, here.w};
+                        const uint32_t gate_words[4] = {here[i].x, here[i].y, here[i].z, here[i].w};
 #pragma unroll
                         for (int j = 0; j < 4; ++j) {
                             float lo = value[8 * i + 2 * j] * v_scale, hi = value[8 * i + 2 * j + 1] * v_scale;
                             if (gated) {
-                                lo = __fdividef(lo, 1.0f + __expf(-__uint_as_float(gate_words[j] << 16)));
-                                hi = __fdividef(hi, 1.0f + __expf(-__uint_as_float(gate_words[j] & 0xffff0000u)));
+                                lo = __fdividef(lo, 1.0f + exp2_fast(__uint_as_float(gate_words[j] << 16) * -kLog2e));
+                                hi = __fdividef(hi, 1.0f + exp2_fast(__uint_as_float(gate_words[j] & 0xffff0000u) * -kLog2e));
                             }
                             const __nv_bfloat162 both = __floats2bfloat162_rn(lo, hi);
                             words[j] = *reinterpret_cast<const uint32_t*>(&both);
                         }
-                        to[i] = make_uint4(words[0], words[1], words[2], words[3]);
+                        out[i] = make_uint4(words[0], words[1], words[2], words[3]);
                     }
+                    store64(p.output + (row * kQueryHeads + head) * kHeadDim + first_dim + c * 32, p.wide_rows, out);
                 }
                 __syncwarp();
             }
@@ -1113,6 +1196,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // Items that were cut: a pair's last item began there and went on with the pairs after it.  A warp per row, eight dims
 // per lane, the pieces in order.
 constexpr int kMergeWarps = 8;
+constexpr int kMergeDepth = 8;  // pieces in flight
 
 __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const __grid_constant__ Params p) {
     pdl_launch_dependents();
@@ -1129,11 +1213,21 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const __g
         return;
     }
     const int r = (token / kRowTokens) * kRows + (token % kRowTokens) * kGqaGroup + index % kGqaGroup;
+    const auto slot = [&](int piece) {
+        return (2 * static_cast<size_t>(pair + piece) + (piece == 0 ? 1 : 0)) * kSlotRows + r;
+    };
+    const int pieces = item.last_pair - pair + 1;
+    // a piece per lane: its weight (at most 96 pieces)
     float maximum = -INFINITY;
-    for (int w = pair + lane; w <= item.last_pair; w += 32) {
-        const PartialStats stats = p.partial_stats[(2 * static_cast<size_t>(w) + (w == pair ? 1 : 0)) * kSlotRows + r];
-        if (!(stats.sum <= 0.0f)) {
-            maximum = fmaxf(maximum, stats.maximum);
+    PartialStats stats[(kMaxPairs + 31) / 32];
+#pragma unroll
+    for (int i = 0; i < (kMaxPairs + 31) / 32; ++i) {
+        stats[i] = {-INFINITY, 0.0f};
+        if (32 * i + lane < pieces) {
+            stats[i] = p.partial_stats[slot(32 * i + lane)];
+        }
+        if (!(stats[i].sum <= 0.0f)) {
+            maximum = fmaxf(maximum, stats[i].maximum);
         }
     }
 #pragma unroll
@@ -1142,19 +1236,34 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const __g
     }
     float acc[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
     float denominator = 0.0f;
-#pragma unroll 4
-    for (int w = pair; w <= item.last_pair; ++w) {
-        const size_t at = (2 * static_cast<size_t>(w) + (w == pair ? 1 : 0)) * kSlotRows + r;
-        const PartialStats stats = p.partial_stats[at];
-        const uint4 raw = reinterpret_cast<const uint4*>(p.partial_out + at * kHeadDim)[lane];
-        const float weight = !(stats.sum <= 0.0f) ? stats.sum * exp2f(stats.maximum - maximum) : 0.0f;
-        denominator += weight;
-        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&words[i]));
-            acc[2 * i] = fmaf(weight, f.x, acc[2 * i]);
-            acc[2 * i + 1] = fmaf(weight, f.y, acc[2 * i + 1]);
+    for (int i = 0; i < (kMaxPairs + 31) / 32; ++i) {
+        const float mine = !(stats[i].sum <= 0.0f) ? stats[i].sum * exp2f(stats[i].maximum - maximum) : 0.0f;
+        const int count = min(32, pieces - 32 * i);
+#pragma unroll 1
+        for (int first = 0; first < count; first += kMergeDepth) {
+            uint4 raw[kMergeDepth];
+#pragma unroll
+            for (int j = 0; j < kMergeDepth; ++j) {
+                raw[j] = make_uint4(0, 0, 0, 0);
+                if (first + j < count) {
+                    raw[j] = reinterpret_cast<const uint4*>(p.partial_out + slot(32 * i + first + j) * kHeadDim)[lane];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < kMergeDepth; ++j) {
+                const float weight = __shfl_sync(0xffffffffu, mine, (first + j) & 31);
+                if (first + j < count) {
+                    denominator += weight;
+                    const uint32_t words[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
+#pragma unroll
+                    for (int d = 0; d < 4; ++d) {
+                        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&words[d]));
+                        acc[2 * d] = fmaf(weight, f.x, acc[2 * d]);
+                        acc[2 * d + 1] = fmaf(weight, f.y, acc[2 * d + 1]);
+                    }
+                }
+            }
         }
     }
     const float v_scale = p.value_scales ? p.value_scales[item.head] : 1.0f;
@@ -1267,6 +1376,8 @@ extern "C" int qwc_paged_attention_chunk_fp8(const void* query, const void* quer
     p.num_blocks = num_blocks;
     p.gate_stride = gate_stride;
     p.softmax_scale = softmax_scale;
+    p.wide_rows = ((reinterpret_cast<uintptr_t>(query_gate_projection) | reinterpret_cast<uintptr_t>(output) |
+                    reinterpret_cast<uintptr_t>(workspace)) & 31) == 0 && gate_stride % 16 == 0;
     p.status = status;
     error = launch_chained(chunk_attention_kernel, dim3(2 * setup->pairs), dim3(kThreads), shared, stream, key_map, value_map, p);
     if (error != cudaSuccess) {
