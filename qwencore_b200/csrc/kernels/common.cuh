@@ -61,6 +61,7 @@ constexpr int kStatusStateSlotRange = 0x105;         // a row named a DeltaNet s
 constexpr int kStatusPeerWait = 0x106;               // a peer rank's slice of an activation row did not arrive
 constexpr int kStatusCopyRange = 0x107;              // a copy named a page or slot beyond its array
 constexpr int kStatusChunkAttentionWait = 0x108;
+constexpr int kStatusChunkDeltaWait = 0x109;
 
 // What a caller said about the projection its stream runs after the next one it launches
 // (qwc_nvfp4_prefetch_next): kept per host thread, taken (and cleared) by the next projection launch.

@@ -5,7 +5,9 @@ Tolerances, all from the types: an output rounded to bf16 is off by up to 2^-8 o
               less than 2^-12): 2^-10 of the weighted mean of |v|;
   delta rule  the operands of its products carry 16 bits or more: each of about six products in a row leaves 2^-16 of the
               sum of its terms' magnitudes, which for 64 or 128 terms of either sign is about 11 times the result:
-              2^-10 of the largest output of the sequence and head.  State values: half a code, and 2^-10 of the row's peak;
+              2^-10 of the largest output of the sequence and head.  State values: half a code, and 2^-10 of the largest
+              of the head's state (a row is a sum of u k over the tokens, off by 2^-16 of the terms; the terms of a row that
+              happens to cancel are as large as those of the others, so its own peak says nothing about them);
   gates       decay exp(-x), x = exp(a_log) softplus(a + dt) from two functions and a product in fp32, each off by an ulp
               or two: x is off by at most five of its 2^-23, which moves exp(-x) by |x| 5 2^-23 < |x| 2^-20 of itself, and
               the functions' own roundings 2^-20.  (Until x reaches 104, where fp32 underflows.)
@@ -338,7 +340,7 @@ class Delta:
         peak = states.abs().amax(-1, keepdim=True)
         for slot in range(self.capacity):
             if slot in touched:
-                off = (values[slot] - states[slot]).abs() - peak[slot] * (0.5 / 127 + 2.0 ** -10)
+                off = (values[slot] - states[slot]).abs() - (peak[slot] * (0.5 / 127) + 2.0 ** -10 * peak[slot].amax(1, keepdim=True))
                 assert off.max() <= 0, (slot, float(off.max()))
                 assert int(self.codes[slot].abs().max()) == 127 or float(peak[slot].max()) == 0.0
             else:
