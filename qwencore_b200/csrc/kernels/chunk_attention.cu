@@ -483,7 +483,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int pair = blockIdx.x >> 1;
     const int pairs = gridDim.x >> 1;
 
-    pdl_launch_dependents();
     if (warp == kMmaWarp) {
         asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
                      "r"(kTmemColumns)
@@ -529,6 +528,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fence_proxy_async();
     __syncthreads();
     pair_sync();  // (the other CTA's shared memory is there)
+    // (Not before this CTA has its tensor memory: a CTA of the next kernel that took some of it first would wait for this
+    // kernel's end, and this CTA for that one's.)
+    pdl_launch_dependents();
     pdl_wait();
     if (rank == 0 && threadIdx.x < 2) {
         // both CTAs of a pair go by what the first one finds in the status word

@@ -20,6 +20,8 @@
 // out only the lower part times the lower part.  The state itself stays in fp32 registers: a thread is a key dim of 32
 // value dims.
 
+#include <cstddef>
+
 #include "chunk.cuh"
 #include "tcgen05.cuh"
 
@@ -34,7 +36,6 @@ constexpr int kQkBytes = 2 * kTileBytes;                 // [half of the dims][q
 constexpr int kWBytes = 2 * kTileBytes;                  // [upper, lower bf16][row][128 bytes]
 constexpr int kSBytes = 2 * kTileBytes;                  // [upper, lower][key dim][128 bytes]
 constexpr int kRBytes = kTileBytes;                      // [upper, lower][token][128 bytes]
-constexpr float kLog2e = 1.4426950408889634f;
 
 // Workspace: images of the operands as shared memory has them.
 struct Images {
@@ -155,32 +156,55 @@ __device__ __forceinline__ void load_columns(uint32_t taddr, float (&x)[32]) {
 }
 
 // ---- W of every block and head ------------------------------------------------------------------------
+//
+// [Q ; K] K^T on the tensor cores gives P and A (a thread has a row), fp32 arithmetic the inverse: columns of the four 16 x 16
+// blocks on the diagonal by substitution, then T_10 = -T_11 A_10 T_00 for blocks of 16 and of 32.  W is a product again,
+// [P ; diag(g_end / g)] times T.
 
 constexpr int kFactorThreads = 128;
-constexpr int kPitch = 68;  // floats of a row of the matrices in shared memory
+constexpr int kPitch = 68;  // floats of a row of the matrices in shared memory: rows begin in different banks
 
 struct FactorSmem {
+    uint8_t operand[kQkBytes];            // q and k, then [P ; diag] in two parts
+    float t[kBlock * kPitch];             // (1 + A)^-1
     union {
-        uint8_t qk[kQkBytes];
-        struct {
-            float a[kBlock * kPitch];  // A, below the diagonal
-            float p[kBlock * kPitch];
-            float t[kBlock * kPitch];  // (1 + A)^-1
-        } m;
+        float a[kBlock * kPitch];         // A, below the diagonal
+        uint8_t product[kRBytes];         // T in two parts
     };
-    float whole[kBlock], part[kBlock];  // log2 of the decay from the start: a whole number and the rest
+    float2 log[kBlock];                   // log2 of the decay from the start: a whole number and the rest
     float beta[kBlock];
     uint64_t done;
     uint32_t tmem_base;
     int failed;
 };
+static_assert(offsetof(FactorSmem, a) % 1024 == 0, "an operand's alignment");
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// x += a * rows[0 .. 3][8 columns] for four steps of the sum.
+__device__ __forceinline__ void multiply4(float (&x)[8], const float4& a, const float* rows) {
+    const float factors[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float4 lo = *reinterpret_cast<const float4*>(rows + k * kPitch);
+        const float4 hi = *reinterpret_cast<const float4*>(rows + k * kPitch + 4);
+        const float row[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            x[c] = fmaf(factors[k], row[c], x[c]);
+        }
+    }
+}
 
 __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
     const __nv_bfloat16* __restrict__ qkv, const float* __restrict__ alpha, const float* __restrict__ beta,
     const uint32_t* __restrict__ begins, const Images images, int tokens, int sequences, int v_heads, int* status) {
     extern __shared__ unsigned char smem_raw[];
     FactorSmem& sm = *reinterpret_cast<FactorSmem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
-    pdl_launch_dependents();
     const int tid = threadIdx.x;
     const int lane = tid & 31;
     const int warp = tid >> 5;
@@ -189,15 +213,6 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
     const int ratio = v_heads / kDeltaKeyHeads;
     const int key_head = head / ratio;
     const int channels = (2 * kDeltaKeyHeads + v_heads) * kDim;
-    pdl_wait();
-    const ChunkTile tile = find_chunk_tile(begins, sequences, tokens, kBlock, block);
-    if (tile.sequence < 0) {
-        return;
-    }
-    const int first = tile.index * kBlock;
-    const int count = min(kBlock, tile.span.length - first);
-    const size_t row0 = static_cast<size_t>(tile.span.begin) + first;
-
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(64)
                      : "memory");
@@ -209,91 +224,260 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
         sm.failed = 0;
         mbar_fence_init();
     }
-    // q and k of the block, zeros behind it: 16 lanes read the 256 bytes of a row
-    for (int i = tid; i < 2 * kBlock * 16; i += kFactorThreads) {
-        const int row = i >> 4, piece = i & 15;
-        const int token = row & (kBlock - 1);
-        uint4 raw = make_uint4(0, 0, 0, 0);
-        if (token < count) {
-            raw = *(reinterpret_cast<const uint4*>(
-                        qkv + (row0 + token) * channels + ((row < kBlock ? 0 : kDeltaKeyHeads) + key_head) * kDim) + piece);
-        }
-        *reinterpret_cast<uint4*>(sm.qk + (piece >> 3) * kTileBytes + swizzled(row, piece & 7)) = raw;
-    }
-    if (warp == 0) {
-        // decay from the start: a scan over the tokens, in whole numbers and rests below one
-        float whole[2], part[2];
+    __syncthreads();
+    // (Not before this CTA has its tensor memory: a CTA of the next kernel that took some of it first would wait for this
+    // kernel's end, and this CTA for that one's.)
+    pdl_launch_dependents();
+    pdl_wait();
+    const ChunkTile tile = find_chunk_tile(begins, sequences, tokens, kBlock, block);
+    const bool here = tile.sequence >= 0;
+    const int first = tile.index * kBlock;
+    const int count = here ? min(kBlock, tile.span.length - first) : 0;
+    const size_t row0 = static_cast<size_t>(tile.span.begin) + first;
+    if (here) {
+        // q and k of the block, zeros behind it: 16 threads fetch the 256 bytes of a row
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const int token = lane + 32 * i;
-            const float log = token < count ? fmaxf(log2f(alpha[(row0 + token) * v_heads + head]), -300.0f) : 0.0f;
-            whole[i] = rintf(log);
-            part[i] = log - whole[i];
-            sm.beta[token] = token < count ? beta[(row0 + token) * v_heads + head] : 0.0f;
+        for (int i = 0; i < 2 * kBlock * 16 / kFactorThreads; ++i) {
+            const int row = (tid >> 4) + i * (kFactorThreads / 16), piece = tid & 15;
+            const int token = row & (kBlock - 1);
+            const __nv_bfloat16* from =
+                qkv + (row0 + (token < count ? token : 0)) * channels + ((row < kBlock ? 0 : kDeltaKeyHeads) + key_head) * kDim + 8 * piece;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                             smem_u32(sm.operand + (piece >> 3) * kTileBytes + swizzled(row, piece & 7))),
+                         "l"(from), "r"(token < count ? 16 : 0)
+                         : "memory");
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+        if (warp == 0) {
+            // decay from the start: a scan over the tokens, in whole numbers and rests below one
+            float whole[2], part[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int token = lane + 32 * i;
+                // (beyond 2^-130 fp32 has nothing, and an alpha of 0 takes everything before it away)
+                const float log = token < count ? fmaxf(log2f(alpha[(row0 + token) * v_heads + head]), -130.0f) : 0.0f;
+                sm.beta[token] = token < count ? beta[(row0 + token) * v_heads + head] : 0.0f;
+                whole[i] = rintf(log);
+                part[i] = log - whole[i];
+            }
 #pragma unroll
             for (int offset = 1; offset < 32; offset <<= 1) {
-                const float w = __shfl_up_sync(0xffffffffu, whole[i], offset);
-                const float p = __shfl_up_sync(0xffffffffu, part[i], offset);
-                if (lane >= offset) {
-                    whole[i] += w;
-                    part[i] += p;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const float w = __shfl_up_sync(0xffffffffu, whole[i], offset);
+                    const float p = __shfl_up_sync(0xffffffffu, part[i], offset);
+                    whole[i] += lane >= offset ? w : 0.0f;
+                    part[i] += lane >= offset ? p : 0.0f;
                 }
             }
-        }
-        whole[1] += __shfl_sync(0xffffffffu, whole[0], 31);
-        part[1] += __shfl_sync(0xffffffffu, part[0], 31);
-        float* decay = images.decay + (static_cast<size_t>(block) * v_heads + head) * kBlock;
+            whole[1] += __shfl_sync(0xffffffffu, whole[0], 31);
+            part[1] += __shfl_sync(0xffffffffu, part[0], 31);
+            float* decay = images.decay + (static_cast<size_t>(block) * v_heads + head) * kBlock;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            sm.whole[lane + 32 * i] = whole[i];
-            sm.part[lane + 32 * i] = part[i];
-            decay[lane + 32 * i] = exp2f(whole[i] + part[i]);
+            for (int i = 0; i < 2; ++i) {
+                sm.log[lane + 32 * i] = make_float2(whole[i], part[i]);
+                decay[lane + 32 * i] = exp2f(whole[i] + part[i]);
+            }
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
     fence_proxy_async();
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sm.tmem_base);
-    // [Q ; K] K^T
-    if (warp == 0) {
-        if (elect_one()) {
-            const uint32_t base = smem_u32(sm.qk);
+    const uint32_t tmem_row = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
+    bool ok = here;
+    if (here) {
+        if (warp == 0) {
+            if (elect_one()) {
+                const uint32_t base = smem_u32(sm.operand);
 #pragma unroll
-            for (int ks = 0; ks < kDim / 16; ++ks) {
-                const uint32_t at = base + (ks >> 2) * kTileBytes + (ks & 3) * 32;
-                mma_bf16(tmem_base, operand(at, 16), operand(at + kBlock * 128, 16), kIdesc, ks > 0 ? 1u : 0u);
+                for (int ks = 0; ks < kDim / 16; ++ks) {
+                    const uint32_t at = base + (ks >> 2) * kTileBytes + (ks & 3) * 32;
+                    mma_bf16(tmem_base, operand(at, 16), operand(at + kBlock * 128, 16), kIdesc, ks > 0 ? 1u : 0u);
+                }
+                umma_commit(&sm.done);
             }
-            umma_commit(&sm.done);
+            __syncwarp();
+        }
+        if (head == key_head * ratio) {
+            // the image of q and k, by the key head's first value head
+            uint4* to = reinterpret_cast<uint4*>(images.qk + (static_cast<size_t>(block) * kDeltaKeyHeads + key_head) * kQkBytes);
+#pragma unroll 4
+            for (int i = tid; i < kQkBytes / 16; i += kFactorThreads) {
+                to[i] = reinterpret_cast<const uint4*>(sm.operand)[i];
+            }
+        }
+        ok = wait(&sm.done, 0, &sm.failed, status);
+    }
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    __syncthreads();  // (the image has been read)
+    const int t = tid & (kBlock - 1);
+    const bool outputs = tid < kBlock;
+    if (ok) {
+        // thread t has row t of Q K^T, thread 64 + t of K K^T: P to its operand, A to shared memory
+        const float2 mine = sm.log[t];
+        const float strength = outputs ? 1.0f : sm.beta[t];
+        const int limit = outputs ? t + 1 : t;
+        const float to_end = exp2_fast((sm.log[kBlock - 1].x - mine.x) + (sm.log[kBlock - 1].y - mine.y));
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+            float x[32];
+            if (32 * c <= (t | 31)) {  // (the same for a warp)
+                load_columns(tmem_row + 32 * c, x);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    const int j = 32 * c + i;
+                    const float2 other = sm.log[j];
+                    const float decay = exp2_fast((mine.x - other.x) + (mine.y - other.y));
+                    x[i] = j < limit ? strength * decay * x[i] : 0.0f;
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    x[i] = 0.0f;
+                }
+            }
+            if (outputs) {
+                store_split(sm.operand, kTileBytes, t, 4 * c, x);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    *reinterpret_cast<float4*>(&sm.a[t * kPitch + 32 * c + 4 * i]) =
+                        make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                }
+#pragma unroll
+                for (int i = 0; i < 32; ++i) {
+                    x[i] = 32 * c + i == t ? to_end : 0.0f;
+                }
+                store_split(sm.operand, kTileBytes, kBlock + t, 4 * c, x);
+            }
+        }
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+    __syncthreads();
+    if (ok) {
+        if (outputs) {
+            // blocks of 16 on the diagonal: a column per thread
+            const int b = tid >> 4, j = tid & 15;
+            float x[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                float sum = 0.0f;
+#pragma unroll
+                for (int k = 0; k < i; k += 4) {
+                    const float4 a = *reinterpret_cast<const float4*>(&sm.a[(16 * b + i) * kPitch + 16 * b + k]);
+                    sum = fmaf(a.x, x[k], sum);
+                    sum = k + 1 < i ? fmaf(a.y, x[k + 1 < i ? k + 1 : 0], sum) : sum;
+                    sum = k + 2 < i ? fmaf(a.z, x[k + 2 < i ? k + 2 : 0], sum) : sum;
+                    sum = k + 3 < i ? fmaf(a.w, x[k + 3 < i ? k + 3 : 0], sum) : sum;
+                }
+                x[i] = i == j ? 1.0f : i < j ? 0.0f : -sum;
+                sm.t[(16 * b + i) * kPitch + 16 * b + j] = x[i];
+            }
+        } else {
+            // zeros above the diagonal, in blocks of 16
+            const int b = t >> 4;
+            for (int j = 16 * (b + 1); j < kBlock; j += 4) {
+                *reinterpret_cast<float4*>(&sm.t[t * kPitch + j]) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+        }
+    }
+    __syncthreads();
+    if (ok) {
+        // blocks of 32: T_10 = -T_11 (A_10 T_00) of 16, eight columns per thread of one row of 32
+        const int pair = tid >> 5;  // two threads' columns of two blocks: pair & 1 the columns' half, pair >> 1 the block
+        const int base = 32 * (pair >> 1), column = base + 8 * (pair & 1);
+        const int r = lane & 15;    // (lanes 16-31 do the same again)
+        float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < 16; k += 4) {
+            multiply4(x, *reinterpret_cast<const float4*>(&sm.a[(base + 16 + r) * kPitch + base + k]), &sm.t[(base + k) * kPitch + column]);
+        }
+        float* at = &sm.t[(base + 16 + r) * kPitch + column];
+        if (lane < 16) {
+            *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
+            *reinterpret_cast<float4*>(at + 4) = make_float4(x[4], x[5], x[6], x[7]);
         }
         __syncwarp();
-    }
-    if (head == key_head * ratio) {
-        // the image of q and k, by the key head's first value head
-        uint4* to = reinterpret_cast<uint4*>(images.qk + (static_cast<size_t>(block) * kDeltaKeyHeads + key_head) * kQkBytes);
-        for (int i = tid; i < kQkBytes / 16; i += kFactorThreads) {
-            to[i] = reinterpret_cast<const uint4*>(sm.qk)[i];
+        float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int k = 0; k < 16; k += 4) {
+            multiply4(y, *reinterpret_cast<const float4*>(&sm.t[(base + 16 + r) * kPitch + base + 16 + k]),
+                      &sm.t[(base + 16 + k) * kPitch + column]);
+        }
+        __syncwarp();
+        if (lane < 16) {
+            *reinterpret_cast<float4*>(at) = make_float4(-y[0], -y[1], -y[2], -y[3]);
+            *reinterpret_cast<float4*>(at + 4) = make_float4(-y[4], -y[5], -y[6], -y[7]);
         }
     }
-    bool ok = wait(&sm.done, 0, &sm.failed, status);
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    __syncthreads();  // the image has been read, too: the matrices go where q and k were
-    const int t = tid & (kBlock - 1);
+    __syncthreads();
     if (ok) {
-        // thread t has row t of Q K^T, thread 64 + t of K K^T
-        const float whole = sm.whole[t], part = sm.part[t];
-        const float mine = tid < kBlock ? 1.0f : sm.beta[t];
-        float* row = (tid < kBlock ? sm.m.p : sm.m.a) + t * kPitch;
-        const int limit = tid < kBlock ? t + 1 : t;
+        // the block of 32 below: a row per lane, eight columns per warp (T_00 is zero above its diagonal)
+        const int column = 8 * warp;
+        float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+        for (int k = column; k < 32; k += 4) {
+            multiply4(x, *reinterpret_cast<const float4*>(&sm.a[(32 + lane) * kPitch + k]), &sm.t[k * kPitch + column]);
+        }
+        float* at = &sm.t[(32 + lane) * kPitch + column];
+        *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
+        *reinterpret_cast<float4*>(at + 4) = make_float4(x[4], x[5], x[6], x[7]);
+        __syncwarp();
+        float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+        for (int k = 0; k < 32; k += 4) {
+            multiply4(y, *reinterpret_cast<const float4*>(&sm.t[(32 + lane) * kPitch + 32 + k]), &sm.t[(32 + k) * kPitch + column]);
+        }
+        __syncwarp();
+        *reinterpret_cast<float4*>(at) = make_float4(-y[0], -y[1], -y[2], -y[3]);
+        *reinterpret_cast<float4*>(at + 4) = make_float4(-y[4], -y[5], -y[6], -y[7]);
+    }
+    __syncthreads();
+    if (ok) {
+        // T diag(beta) as an operand: half a row per thread
+        const int row = tid >> 1, half = tid & 1;
+        float x[32];
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            float g[32];
-            load_columns(tmem_base + (static_cast<uint32_t>(warp * 32) << 16) + 32 * c, g);
+        for (int i = 0; i < 8; ++i) {
+            const float4 value = *reinterpret_cast<const float4*>(&sm.t[row * kPitch + 32 * half + 4 * i]);
+            const float4 strength = *reinterpret_cast<const float4*>(&sm.beta[32 * half + 4 * i]);
+            x[4 * i] = value.x * strength.x;
+            x[4 * i + 1] = value.y * strength.y;
+            x[4 * i + 2] = value.z * strength.z;
+            x[4 * i + 3] = value.w * strength.w;
+        }
+        store_split(sm.product, kRBytes / 2, row, 4 * half, x);
+        fence_proxy_async();
+    }
+    __syncthreads();
+    if (ok) {
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        if (warp == 0) {
+            if (elect_one()) {
+                const uint32_t a = smem_u32(sm.operand), b = smem_u32(sm.product);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                const int j = 32 * c + i;
-                const float ratio_tj = exp2f((whole - sm.whole[j]) + (part - sm.part[j]));
-                row[j] = j < limit ? mine * ratio_tj * g[i] : 0.0f;
+                for (int ks = 0; ks < kBlock / 16; ++ks) {
+                    const uint64_t upper = operand(a + ks * 32, 16), lower = operand(a + kTileBytes + ks * 32, 16);
+                    const uint64_t t_upper = operand(b + ks * 2048, 16), t_lower = operand(b + kRBytes / 2 + ks * 2048, 16);
+                    mma_bf16(tmem_base, upper, t_upper, kIdesc | kTransposeB, ks > 0 ? 1u : 0u);
+                    mma_bf16(tmem_base, upper, t_lower, kIdesc | kTransposeB, 1u);
+                    mma_bf16(tmem_base, lower, t_upper, kIdesc | kTransposeB, 1u);
+                }
+                umma_commit(&sm.done);
             }
+            __syncwarp();
+        }
+        ok = wait(&sm.done, 1, &sm.failed, status);
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    }
+    if (ok) {
+        uint8_t* w = images.w + (static_cast<size_t>(block) * v_heads + head) * kWBytes;
+#pragma unroll 1
+        for (int c = 0; c < 2; ++c) {
+            float x[32];
+            load_columns(tmem_row + 32 * c, x);
+            store_split(w, kTileBytes, tid, 4 * c, x);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -301,115 +485,6 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
     if (warp == 0) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(64) : "memory");
     }
-    if (!ok) {
-        return;  // (the whole CTA: a wait that gave up fails for all, and the MMAs' accumulators are not read)
-    }
-    // (1 + A)^-1: the four blocks of 16 on the diagonal, a column per thread ...
-    if (tid < kBlock) {
-        const int b = tid >> 4, j = tid & 15;
-        float x[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float sum = 0.0f;
-#pragma unroll
-            for (int k = 0; k < i; ++k) {
-                sum = fmaf(sm.m.a[(16 * b + i) * kPitch + 16 * b + k], x[k], sum);
-            }
-            x[i] = i == j ? 1.0f : i < j ? 0.0f : -sum;
-            sm.m.t[(16 * b + i) * kPitch + 16 * b + j] = x[i];
-        }
-    } else {
-        // (above the diagonal: zeros)
-        for (int i = tid - kBlock; i < kBlock * 4; i += kBlock) {
-            const int r = i >> 2, b = i & 3;
-            if (b > (r >> 4)) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    *reinterpret_cast<float4*>(&sm.m.t[r * kPitch + 16 * b + 4 * j]) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                }
-            }
-        }
-    }
-    __syncthreads();
-    // ... then those below, one diagonal of blocks after the other: T_ij = -T_ii sum_k A_ik T_kj
-    const int r = tid >> 3, c2 = (tid & 7) * 2;
-#pragma unroll 1
-    for (int d = 1; d < 4; ++d) {
-        float2 sums[3];
-#pragma unroll
-        for (int i = 1; i < 4; ++i) {
-            if (i >= d) {
-                const int j = i - d;
-                float2 sum = make_float2(0.0f, 0.0f);
-                for (int k = 16 * j; k < 16 * i; ++k) {
-                    const float a = sm.m.a[(16 * i + r) * kPitch + k];
-                    const float2 x = *reinterpret_cast<const float2*>(&sm.m.t[k * kPitch + 16 * j + c2]);
-                    sum.x = fmaf(a, x.x, sum.x);
-                    sum.y = fmaf(a, x.y, sum.y);
-                }
-                sums[i - 1] = sum;
-            }
-        }
-#pragma unroll
-        for (int i = 1; i < 4; ++i) {
-            if (i >= d) {
-                *reinterpret_cast<float2*>(&sm.m.t[(16 * i + r) * kPitch + 16 * (i - d) + c2]) = sums[i - 1];
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 1; i < 4; ++i) {
-            if (i >= d) {
-                float2 sum = make_float2(0.0f, 0.0f);
-                for (int k = 0; k < 16; ++k) {
-                    const float a = sm.m.t[(16 * i + r) * kPitch + 16 * i + k];
-                    const float2 x = *reinterpret_cast<const float2*>(&sm.m.t[(16 * i + k) * kPitch + 16 * (i - d) + c2]);
-                    sum.x = fmaf(a, x.x, sum.x);
-                    sum.y = fmaf(a, x.y, sum.y);
-                }
-                sums[i - 1] = make_float2(-sum.x, -sum.y);
-            }
-        }
-        __syncthreads();
-#pragma unroll
-        for (int i = 1; i < 4; ++i) {
-            if (i >= d) {
-                *reinterpret_cast<float2*>(&sm.m.t[(16 * i + r) * kPitch + 16 * (i - d) + c2]) = sums[i - 1];
-            }
-        }
-        __syncthreads();
-    }
-    // W: a row per thread, half of its columns
-    uint8_t* w = images.w + (static_cast<size_t>(block) * v_heads + head) * kWBytes;
-    const int half = tid >> 6;
-    float x[32];
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        x[i] = 0.0f;
-    }
-    const int last = (t | 31) + 1;  // (the same for a warp)
-    for (int k = 32 * half; k < last; ++k) {
-        const float p = sm.m.p[t * kPitch + k];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float4 row = *reinterpret_cast<const float4*>(&sm.m.t[k * kPitch + 32 * half + 4 * i]);
-            x[4 * i] = fmaf(p, row.x, x[4 * i]);
-            x[4 * i + 1] = fmaf(p, row.y, x[4 * i + 1]);
-            x[4 * i + 2] = fmaf(p, row.z, x[4 * i + 2]);
-            x[4 * i + 3] = fmaf(p, row.w, x[4 * i + 3]);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        x[i] *= sm.beta[32 * half + i];
-    }
-    store_split(w, kTileBytes, t, 4 * half, x);
-    const float to_end = exp2f((sm.whole[kBlock - 1] - sm.whole[t]) + (sm.part[kBlock - 1] - sm.part[t]));
-#pragma unroll
-    for (int i = 0; i < 32; ++i) {
-        x[i] = to_end * sm.m.t[t * kPitch + 32 * half + i] * sm.beta[32 * half + i];
-    }
-    store_split(w, kTileBytes, kBlock + t, 4 * half, x);
 }
 
 // ---- the chain of blocks --------------------------------------------------------------------------------
@@ -441,7 +516,6 @@ __global__ void __launch_bounds__((kChains * (kChainWarps + 1) + 1) * 32, 1) del
     constexpr int kFirstMmaWarp = kChains * kChainWarps;
     constexpr int kLoadWarp = kFirstMmaWarp + kChains;
     constexpr int kTmemColumns = kChains == 1 ? 256 : 512;
-    pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
     const int head = blockIdx.x / (2 / kChains);
@@ -492,6 +566,7 @@ __global__ void __launch_bounds__((kChains * (kChainWarps + 1) + 1) * 32, 1) del
     fence_proxy_async();
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    pdl_launch_dependents();  // (this CTA has its tensor memory)
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sm.tmem_base);
     bool ok = true;
     int n = 0;  // blocks so far
@@ -774,44 +849,63 @@ __global__ void __launch_bounds__((kChains * (kChainWarps + 1) + 1) * 32, 1) del
 }
 
 // RMSNorm over the 128 dims of a value head, times weight, times silu(gate): in place on the bf16 rows of the batch's
-// chunks.  A warp per token and head, four dims per lane; one rounding.
+// chunks, one rounding.  Sixteen lanes to a token and head, eight dims each; a warp has eight rows in flight.
 constexpr int kNormWarps = 8;
+constexpr int kNormRows = 8;  // of a warp
 
 __global__ void __launch_bounds__(kNormWarps * 32) delta_norm_rows_kernel(
     __nv_bfloat16* __restrict__ rows, const __nv_bfloat16* __restrict__ gate, const __nv_bfloat16* __restrict__ weight,
     const uint32_t* __restrict__ begins, int sequences, int tokens, int v_heads, int gate_stride, float epsilon) {
     pdl_launch_dependents();
     const int lane = threadIdx.x & 31;
-    const size_t item = static_cast<size_t>(blockIdx.x) * kNormWarps + (threadIdx.x >> 5);
-    const size_t token = item / v_heads;
-    const int head = static_cast<int>(item % v_heads);
+    const int piece = lane & 15;
+    const uint32_t first = (blockIdx.x * kNormWarps + (threadIdx.x >> 5)) * kNormRows + (lane >> 4);
+    float gain[8];
+    unpack_bf16(*(reinterpret_cast<const uint4*>(weight) + piece), gain);
     pdl_wait();
-    const uint32_t low = __ldcg(begins), high = __ldcg(begins + sequences);
-    if (token < low || token >= high || token >= tokens) {
-        return;
-    }
-    uint2* at = reinterpret_cast<uint2*>(rows + (token * v_heads + head) * kDim) + lane;
-    const uint2 raw = *at;
-    const uint2 gates = *(reinterpret_cast<const uint2*>(gate + token * gate_stride + head * kDim) + lane);
-    const uint2 gains = *(reinterpret_cast<const uint2*>(weight) + lane);
-    const auto unpack = [](const uint2& words, float (&x)[4]) {
-        x[0] = __uint_as_float(words.x << 16);
-        x[1] = __uint_as_float(words.x & 0xffff0000u);
-        x[2] = __uint_as_float(words.y << 16);
-        x[3] = __uint_as_float(words.y & 0xffff0000u);
-    };
-    float x[4], z[4], w[4];
-    unpack(raw, x);
-    unpack(gates, z);
-    unpack(gains, w);
-    const float sum = warp_sum(x[0] * x[0] + x[1] * x[1] + x[2] * x[2] + x[3] * x[3]);
-    const float inverse = rsqrtf(sum / static_cast<float>(kDim) + epsilon);
+    const uint32_t low = __ldcg(begins), high = min(__ldcg(begins + sequences), static_cast<uint32_t>(tokens));
+    uint4 raw[kNormRows / 2], gates[kNormRows / 2];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[i] *= inverse * w[i] * (z[i] / (1.0f + __expf(-z[i])));
+    for (int i = 0; i < kNormRows / 2; ++i) {
+        const uint32_t row = first + 2 * i;
+        const uint32_t token = row / v_heads, head = row % v_heads;
+        raw[i] = gates[i] = make_uint4(0, 0, 0, 0);
+        if (token >= low && token < high) {
+            raw[i] = *(reinterpret_cast<const uint4*>(rows + static_cast<size_t>(row) * kDim) + piece);
+            gates[i] = *(reinterpret_cast<const uint4*>(gate + static_cast<size_t>(token) * gate_stride + head * kDim) + piece);
+        }
     }
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(x[0], x[1]), hi = __floats2bfloat162_rn(x[2], x[3]);
-    *at = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+#pragma unroll
+    for (int i = 0; i < kNormRows / 2; ++i) {
+        const uint32_t row = first + 2 * i;
+        const uint32_t token = row / v_heads;
+        float x[8], z[8];
+        unpack_bf16(raw[i], x);
+        unpack_bf16(gates[i], z);
+        float sum = 0.0f;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            sum = fmaf(x[j], x[j], sum);
+        }
+#pragma unroll
+        for (int offset = 1; offset < 16; offset <<= 1) {
+            sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+        }
+        const float inverse = rsqrtf(sum / static_cast<float>(kDim) + epsilon);
+        uint32_t words[4];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            x[j] *= inverse * gain[j] * __fdividef(z[j], 1.0f + __expf(-z[j]));
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 pair = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+            words[j] = *reinterpret_cast<const uint32_t*>(&pair);
+        }
+        if (token >= low && token < high) {
+            *(reinterpret_cast<uint4*>(rows + static_cast<size_t>(row) * kDim) + piece) = make_uint4(words[0], words[1], words[2], words[3]);
+        }
+    }
 }
 
 }  // namespace
@@ -906,8 +1000,9 @@ extern "C" int qwc_delta_chunk_int8(void* state, float* state_scales, const void
         return launched;
     }
     const int items = tokens * v_heads;  // at most 65536 * 48
-    return launch_chained(delta_norm_rows_kernel, dim3((items + kNormWarps - 1) / kNormWarps), dim3(kNormWarps * 32), 0,
-                          stream, static_cast<__nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(gate),
+    constexpr int kItems = kNormWarps * kNormRows;
+    return launch_chained(delta_norm_rows_kernel, dim3((items + kItems - 1) / kItems), dim3(kNormWarps * 32), 0, stream,
+                           static_cast<__nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(gate),
                           static_cast<const __nv_bfloat16*>(norm_weight), static_cast<const uint32_t*>(chunk_begins),
                           sequences, tokens, v_heads, gate_stride, epsilon);
 }
