@@ -11,14 +11,15 @@
 //   o_t = g_t S0 q_t + sum_{j<=t} (g_t / g_j) (q_t.k_j) u_j,     S1 = g_end S0 + sum_j (g_end / g_j) u_j k_j^T.
 // With T = (1 + A)^-1 diag(beta) and P the matrix of the second sum, W = [P T ; diag(g_end / g) T] (128 x 64) does not
 // depend on the state: the first kernel makes it for all blocks and heads at once.  The second kernel walks through the
-// blocks of a head with three products,
-//   [Q ; K] S0^T  ->  R  ->  W R = [outputs within the block ; updates U']  ->  S1^T = g_end S0^T + K^T U'.
+// blocks of a head, with everything the other way round, a value dim in a row:
+//   X = S0 K^T,  Y = S0 Q^T;     [O | U'] = V^T W^T - (X diag(g)) W^T;     S1 = g_end S0 + U' K;     outputs O + Y diag(g).
 //
-// Bound by the chain of these products: each waits for the one before, block after block, 64 columns of the state (value
-// dims) at a time.  They run on the fifth-generation tensor cores, M = 128 rows, accumulators in tensor memory.  q and k
-// are bf16 as they come; S, R, U' and W are written as the sum of two bf16, which hold 16 bits, and their products leave
-// out only the lower part times the lower part.  The state itself stays in fp32 registers: a thread is a key dim of 32
-// value dims.
+// Bound by the chain S0 -> X -> U' -> S1, block after block.  All products run on the fifth-generation tensor cores, M = 128 value
+// dims.  S (fp32, accumulated in place), X and U' never leave tensor memory: a thread has a row, turns 32 columns of an
+// accumulator into the next product's A operand and puts it where the accumulator was.  The B operands, K, Q, V and W, come
+// as they lie in memory.  What the chain does not wait for, V^T W^T, Y and the outputs, is issued where the tensor cores
+// would wait for such a step.  K, Q and V are bf16 as they come; S, X, U' and W are the sum of two bf16, which hold 16 bits,
+// and their products leave out only the lower part times the lower part.
 
 #include <cstddef>
 
@@ -30,12 +31,11 @@ namespace {
 
 constexpr int kDim = kDeltaHeadDim;
 constexpr int kBlock = 64;                               // tokens
-constexpr int kColumns = 64;                             // value dims of a chain
 constexpr int kTileBytes = 128 * 128;                    // 128 rows of 64 bf16, 128-byte swizzle
 constexpr int kQkBytes = 2 * kTileBytes;                 // [half of the dims][q of the block's tokens, k][128 bytes]
 constexpr int kWBytes = 2 * kTileBytes;                  // [upper, lower bf16][row][128 bytes]
-constexpr int kSBytes = 2 * kTileBytes;                  // [upper, lower][key dim][128 bytes]
-constexpr int kRBytes = kTileBytes;                      // [upper, lower][token][128 bytes]
+constexpr int kVBytes = kTileBytes;                      // [half of the value dims][token][128 bytes]
+constexpr int kProductBytes = kTileBytes;                // T of a block: [upper, lower][row][128 bytes]
 
 // Workspace: images of the operands as shared memory has them.
 struct Images {
@@ -70,7 +70,9 @@ __device__ __forceinline__ void mma_bf16(uint32_t d_tmem, uint64_t a_desc, uint6
         : "memory");
 }
 
-constexpr uint32_t kIdesc = (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(kColumns >> 3) << 17) | (8u << 24);
+constexpr uint32_t idesc_of(int columns) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | (static_cast<uint32_t>(columns >> 3) << 17) | (8u << 24);
+}
 constexpr uint32_t kTransposeA = 1u << 15, kTransposeB = 1u << 16;
 
 // Operand of 128-byte rows with the 128-byte swizzle, eight rows to an atom.  K-major: a row is one of M or N, its bytes 64
@@ -104,15 +106,6 @@ __device__ __forceinline__ void store_split(uint8_t* at, int parts, int row, int
         split2(x[8 * i + 6], x[8 * i + 7], upper.w, lower.w);
         *reinterpret_cast<uint4*>(at + swizzled(row, first_piece + i)) = upper;
         *reinterpret_cast<uint4*>(at + parts + swizzled(row, first_piece + i)) = lower;
-    }
-}
-
-__device__ __forceinline__ void unpack_bf16(const uint4& raw, float* out) {
-    const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        out[2 * i] = __uint_as_float(words[i] << 16);
-        out[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u);
     }
 }
 
@@ -169,7 +162,7 @@ struct FactorSmem {
     float t[kBlock * kPitch];             // (1 + A)^-1
     union {
         float a[kBlock * kPitch];         // A, below the diagonal
-        uint8_t product[kRBytes];         // T in two parts
+        uint8_t product[kProductBytes];   // T in two parts
     };
     float2 log[kBlock];                   // log2 of the decay from the start: a whole number and the rest
     float beta[kBlock];
@@ -294,7 +287,7 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
 #pragma unroll
                 for (int ks = 0; ks < kDim / 16; ++ks) {
                     const uint32_t at = base + (ks >> 2) * kTileBytes + (ks & 3) * 32;
-                    mma_bf16(tmem_base, operand(at, 16), operand(at + kBlock * 128, 16), kIdesc, ks > 0 ? 1u : 0u);
+                    mma_bf16(tmem_base, operand(at, 16), operand(at + kBlock * 128, 16), idesc_of(kBlock), ks > 0 ? 1u : 0u);
                 }
                 umma_commit(&sm.done);
             }
@@ -447,7 +440,7 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
             x[4 * i + 2] = value.z * strength.z;
             x[4 * i + 3] = value.w * strength.w;
         }
-        store_split(sm.product, kRBytes / 2, row, 4 * half, x);
+        store_split(sm.product, kProductBytes / 2, row, 4 * half, x);
         fence_proxy_async();
     }
     __syncthreads();
@@ -459,10 +452,10 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
 #pragma unroll
                 for (int ks = 0; ks < kBlock / 16; ++ks) {
                     const uint64_t upper = operand(a + ks * 32, 16), lower = operand(a + kTileBytes + ks * 32, 16);
-                    const uint64_t t_upper = operand(b + ks * 2048, 16), t_lower = operand(b + kRBytes / 2 + ks * 2048, 16);
-                    mma_bf16(tmem_base, upper, t_upper, kIdesc | kTransposeB, ks > 0 ? 1u : 0u);
-                    mma_bf16(tmem_base, upper, t_lower, kIdesc | kTransposeB, 1u);
-                    mma_bf16(tmem_base, lower, t_upper, kIdesc | kTransposeB, 1u);
+                    const uint64_t t_upper = operand(b + ks * 2048, 16), t_lower = operand(b + kProductBytes / 2 + ks * 2048, 16);
+                    mma_bf16(tmem_base, upper, t_upper, idesc_of(kBlock) | kTransposeB, ks > 0 ? 1u : 0u);
+                    mma_bf16(tmem_base, upper, t_lower, idesc_of(kBlock) | kTransposeB, 1u);
+                    mma_bf16(tmem_base, lower, t_upper, idesc_of(kBlock) | kTransposeB, 1u);
                 }
                 umma_commit(&sm.done);
             }
@@ -488,38 +481,84 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
 }
 
 // ---- the chain of blocks --------------------------------------------------------------------------------
+//
+//   warps 0-7    the chain: four quarters of the 128 rows, two groups of columns
+//   warps 8-15   outputs: the same division, then rows of the batch, norm and gate
+//   warp 16      issues the MMAs
+//   warp 17      fetches K, Q, W and V of the next block
 
-constexpr int kChainWarps = 8;  // of a chain: four quarters of the rows, two halves of its columns
+constexpr int kChainWarps = 8;
+constexpr int kOutputWarps = 8;
+constexpr int kMmaWarp = kChainWarps + kOutputWarps;
+constexpr int kLoadWarp = kMmaWarp + 1;
+constexpr int kChainThreads = (kLoadWarp + 1) * 32;
+// tensor memory
+constexpr int kStateColumn = 0;                          // fp32, 128 key dims
+constexpr int kSplitColumn = 128;                        // upper (64 columns), lower
+constexpr int kKeyColumn = 256;                          // X of 64 tokens; then -g X, 32 tokens upper and lower side by side
+constexpr int kQueryColumn = 320;                        // Y
+constexpr int kResultColumn = 384;                       // O, U'; then U' split as X
+constexpr int kUpdateColumn = kResultColumn + kBlock;
+constexpr int kTmemColumns = 512;
 
-// Two chains (both halves of a head's value dims) to a CTA, or one.
-template <int kChains>
 struct ChainSmem {
     uint8_t qk[2][kQkBytes];
-    uint8_t w[kWBytes];
-    uint8_t s[kChains][kSBytes];
-    uint8_t r[kChains][kRBytes];  // R of a block, then U'
-    uint64_t qk_full[2], qk_empty[2], w_full, w_empty;
-    uint64_t s_ready[kChains], d1_done[kChains], r_ready[kChains], d2_done[kChains], u_ready[kChains], d3_done[kChains];
-    float peak[kChains][4][kColumns];
+    uint8_t w[2][kWBytes];
+    uint8_t v[2][kVBytes];
+    float rows[kBlock * kDim];          // outputs of a block
+    float decay[2][kBlock];
+    float peak[2][kDim];
+    uint64_t qk_full[2], qk_empty[2], w_full[2], w_empty[2], v_full[2], v_empty[2];
+    uint64_t s_ready, x_done, x_ready, u_done, u_ready, o_done, o_free, s_done;
+    uint64_t rows_ready, rows_free;
     uint32_t tmem_base;
     int failed;
 };
+static_assert(sizeof(ChainSmem) + 1024 <= 232448, "shared memory of a CTA");
 
-template <int kChains>
-__global__ void __launch_bounds__((kChains * (kChainWarps + 1) + 1) * 32, 1) delta_chain_kernel(
+// What follows the rule, where it is wanted: RMSNorm over a head's value dims, times weight, times silu(gate).
+struct OutputNorm {
+    const __nv_bfloat16* gate;    // null: not wanted
+    const __nv_bfloat16* weight;
+    int gate_stride;
+    float epsilon;
+};
+
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void tmem_store_columns(uint32_t taddr, const float (&x)[32]) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        uint32_t raw[16];
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+            raw[j] = __float_as_uint(x[16 * i + j]);
+        }
+        tmem_store16(taddr + 16 * i, raw);
+    }
+}
+
+// 32 columns as an A operand in two parts of 16 columns.
+__device__ __forceinline__ void tmem_store_split(uint32_t upper_at, uint32_t lower_at, const float (&x)[32]) {
+    uint32_t upper[16], lower[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        split2(x[2 * i], x[2 * i + 1], upper[i], lower[i]);
+    }
+    tmem_store16(upper_at, upper);
+    tmem_store16(lower_at, lower);
+}
+
+__global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
     int8_t* __restrict__ state, float* __restrict__ state_scales, const uint32_t* __restrict__ state_slots,
     const uint32_t* __restrict__ continues, const uint32_t* __restrict__ begins, const __nv_bfloat16* __restrict__ qkv,
-    const Images images, __nv_bfloat16* __restrict__ out, int tokens, int v_heads, int state_capacity, int* status) {
+    const Images images, __nv_bfloat16* __restrict__ out, int tokens, int v_heads, int state_capacity,
+    const OutputNorm norm, int* status) {
     extern __shared__ unsigned char smem_raw[];
-    using Smem = ChainSmem<kChains>;
-    Smem& sm = *reinterpret_cast<Smem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
-    constexpr int kFirstMmaWarp = kChains * kChainWarps;
-    constexpr int kLoadWarp = kFirstMmaWarp + kChains;
-    constexpr int kTmemColumns = kChains == 1 ? 256 : 512;
+    ChainSmem& sm = *reinterpret_cast<ChainSmem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
-    const int head = blockIdx.x / (2 / kChains);
-    const int first_chain = kChains == 1 ? blockIdx.x & 1 : 0;  // of the head's two
+    const int head = blockIdx.x;
     const int key_head = head / (v_heads / kDeltaKeyHeads);
     const int channels = (2 * kDeltaKeyHeads + v_heads) * kDim;
     const int sequence = blockIdx.y;
@@ -548,18 +587,22 @@ __global__ void __launch_bounds__((kChains * (kChainWarps + 1) + 1) * 32, 1) del
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm.qk_full[i], 1);
-            mbar_init(&sm.qk_empty[i], kChains);
+            mbar_init(&sm.qk_empty[i], 1);
+            mbar_init(&sm.w_full[i], 1);
+            mbar_init(&sm.w_empty[i], 1 + kOutputWarps);  // the MMAs, and who reads the decays
+            mbar_init(&sm.v_full[i], 1);
+            mbar_init(&sm.v_empty[i], 1);
         }
-        mbar_init(&sm.w_full, 1);
-        mbar_init(&sm.w_empty, kChains);
-        for (int i = 0; i < kChains; ++i) {
-            mbar_init(&sm.s_ready[i], kChainWarps);
-            mbar_init(&sm.d1_done[i], 1);
-            mbar_init(&sm.r_ready[i], kChainWarps / 2);
-            mbar_init(&sm.d2_done[i], 1);
-            mbar_init(&sm.u_ready[i], kChainWarps / 2);
-            mbar_init(&sm.d3_done[i], 1);
-        }
+        mbar_init(&sm.s_ready, kChainWarps);
+        mbar_init(&sm.x_done, 1);
+        mbar_init(&sm.x_ready, kChainWarps);
+        mbar_init(&sm.u_done, 1);
+        mbar_init(&sm.u_ready, kChainWarps);
+        mbar_init(&sm.o_done, 1);
+        mbar_init(&sm.o_free, kOutputWarps);
+        mbar_init(&sm.s_done, 1);
+        mbar_init(&sm.rows_ready, kOutputWarps);
+        mbar_init(&sm.rows_free, kOutputWarps);
         sm.failed = 0;
         mbar_fence_init();
     }
@@ -568,9 +611,9 @@ __global__ void __launch_bounds__((kChains * (kChainWarps + 1) + 1) * 32, 1) del
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     pdl_launch_dependents();  // (this CTA has its tensor memory)
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sm.tmem_base);
+    int* const failed = &sm.failed;
     bool ok = true;
     int n = 0;  // blocks so far
-    float s[32];
 
     if (warp == kLoadWarp) {
         // ---------------- operands of the blocks -------------------------------------------------------
@@ -579,46 +622,124 @@ __global__ void __launch_bounds__((kChains * (kChainWarps + 1) + 1) * 32, 1) del
             first_block += (chunk_span(begins, i, tokens).length + kBlock - 1) / kBlock;
         }
         first_block = static_cast<int>(__reduce_add_sync(0xffffffffu, first_block));
+        const __nv_bfloat16* v_rows = qkv + static_cast<size_t>(span.begin) * channels + (2 * kDeltaKeyHeads + head) * kDim;
         for (; n < blocks && ok; ++n) {
+            const int slot_of = n & 1;
+            const uint32_t parity = ((n >> 1) & 1) ^ 1;
             const size_t block = static_cast<size_t>(first_block) + n;
-            ok = wait(&sm.qk_empty[n & 1], ((n >> 1) & 1) ^ 1, &sm.failed, status);
+            ok = wait(&sm.w_empty[slot_of], parity, failed, status);
             if (ok && lane == 0) {
-                mbar_arrive_expect_tx(&sm.qk_full[n & 1], kQkBytes);
-                bulk_g2s(sm.qk[n & 1], images.qk + (block * kDeltaKeyHeads + key_head) * kQkBytes, kQkBytes, &sm.qk_full[n & 1]);
+                mbar_arrive_expect_tx(&sm.w_full[slot_of], kWBytes + kBlock * 4);
+                bulk_g2s(sm.w[slot_of], images.w + (block * v_heads + head) * kWBytes, kWBytes, &sm.w_full[slot_of]);
+                bulk_g2s(sm.decay[slot_of], images.decay + (block * v_heads + head) * kBlock, kBlock * 4, &sm.w_full[slot_of]);
             }
             __syncwarp();
-            ok = ok && wait(&sm.w_empty, (n & 1) ^ 1, &sm.failed, status);
+            ok = ok && wait(&sm.v_empty[slot_of], parity, failed, status);
+            if (ok) {
+                // rows of v, zeros behind the chunk: sixteen lanes to a row
+                const int piece = lane & 15;
+#pragma unroll 8
+                for (int i = 0; i < kBlock / 2; ++i) {
+                    const int t = 2 * i + (lane >> 4);
+                    const int token = n * kBlock + t;
+                    const bool live = token < span.length;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                     smem_u32(sm.v[slot_of] + (piece >> 3) * (kVBytes / 2) + swizzled(t, piece & 7))),
+                                 "l"(v_rows + static_cast<size_t>(live ? token : 0) * channels + 8 * piece), "r"(live ? 16 : 0)
+                                 : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            ok = ok && wait(&sm.qk_empty[slot_of], parity, failed, status);
             if (ok && lane == 0) {
-                mbar_arrive_expect_tx(&sm.w_full, kWBytes);
-                bulk_g2s(sm.w, images.w + (block * v_heads + head) * kWBytes, kWBytes, &sm.w_full);
+                mbar_arrive_expect_tx(&sm.qk_full[slot_of], kQkBytes);
+                bulk_g2s(sm.qk[slot_of], images.qk + (block * kDeltaKeyHeads + key_head) * kQkBytes, kQkBytes, &sm.qk_full[slot_of]);
+            }
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            fence_proxy_async();
+            __syncwarp();
+            if (ok && lane == 0) {
+                mbar_arrive(&sm.v_full[slot_of]);
             }
             __syncwarp();
         }
-    } else if (warp >= kFirstMmaWarp) {
-        // ---------------- tensor-core issue of a chain ---------------------------------------------------
-        const int chain = warp - kFirstMmaWarp;
-        const uint32_t d1 = tmem_base + chain * 256, d2 = d1 + kColumns, d3 = d2 + kColumns;
-        const uint32_t s_base = smem_u32(sm.s[chain]), r_base = smem_u32(sm.r[chain]), w_base = smem_u32(sm.w);
-        for (; n < blocks; ++n) {
+    } else if (warp == kMmaWarp) {
+        // ---------------- tensor-core issue ------------------------------------------------------------
+        constexpr uint32_t kWide = idesc_of(kDim), kNarrow = idesc_of(kBlock);
+        // [O | U'] begins as V^T W^T
+        const auto issue_values = [&](int number) {
+            const int slot_of = number & 1;
+            if (!wait(&sm.w_full[slot_of], (number >> 1) & 1, failed, status) ||
+                !wait(&sm.v_full[slot_of], (number >> 1) & 1, failed, status) ||
+                !wait(&sm.o_free, (number & 1) ^ 1, failed, status)) {
+                return false;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (elect_one()) {
+                const uint32_t v_base = smem_u32(sm.v[slot_of]), w_base = smem_u32(sm.w[slot_of]);
+#pragma unroll
+                for (int ks = 0; ks < kBlock / 16; ++ks) {
+                    const uint64_t a = operand(v_base + ks * 2048, kVBytes / 2);
+                    mma_bf16(tmem_base + kResultColumn, a, operand(w_base + ks * 32, 16), kWide | kTransposeA, ks > 0 ? 1u : 0u);
+                    mma_bf16(tmem_base + kResultColumn, a, operand(w_base + kTileBytes + ks * 32, 16), kWide | kTransposeA, 1u);
+                }
+                umma_commit(&sm.v_empty[slot_of]);
+            }
+            __syncwarp();
+            return true;
+        };
+        ok = issue_values(0);
+        for (; n < blocks && ok; ++n) {
             const uint32_t parity = n & 1;
-            const uint32_t qk_base = smem_u32(sm.qk[n & 1]);
-            ok = wait(&sm.qk_full[n & 1], (n >> 1) & 1, &sm.failed, status) &&
-                 wait(&sm.s_ready[chain], parity, &sm.failed, status);
+            const uint32_t qk_base = smem_u32(sm.qk[n & 1]), w_base = smem_u32(sm.w[n & 1]);
+            ok = wait(&sm.qk_full[n & 1], (n >> 1) & 1, failed, status) && wait(&sm.s_ready, parity, failed, status);
             if (!ok) {
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (elect_one()) {
+                // X, then Y
 #pragma unroll
-                for (int ks = 0; ks < kDim / 16; ++ks) {
-                    const uint64_t a = operand(qk_base + (ks >> 2) * kTileBytes + (ks & 3) * 32, 16);
-                    mma_bf16(d1, a, operand(s_base + ks * 2048, 16), kIdesc | kTransposeB, ks > 0 ? 1u : 0u);
-                    mma_bf16(d1, a, operand(s_base + kTileBytes + ks * 2048, 16), kIdesc | kTransposeB, 1u);
+                for (int part = 0; part < 2; ++part) {
+                    const uint32_t rows = qk_base + (part == 0 ? kBlock * 128 : 0);
+                    const uint32_t d = tmem_base + (part == 0 ? kKeyColumn : kQueryColumn);
+#pragma unroll
+                    for (int ks = 0; ks < kDim / 16; ++ks) {
+                        const uint64_t b = operand(rows + (ks >> 2) * kTileBytes + (ks & 3) * 32, 16);
+                        umma_f16(d, tmem_base + kSplitColumn + ks * 8, b, kNarrow, ks > 0 ? 1u : 0u);
+                        umma_f16(d, tmem_base + kSplitColumn + 64 + ks * 8, b, kNarrow, 1u);
+                    }
+                    if (part == 0) {
+                        umma_commit(&sm.x_done);
+                    }
                 }
-                umma_commit(&sm.d1_done[chain]);
             }
             __syncwarp();
-            ok = wait(&sm.w_full, parity, &sm.failed, status) && wait(&sm.r_ready[chain], parity, &sm.failed, status);
+            ok = wait(&sm.x_ready, parity, failed, status);
+            if (!ok) {
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (elect_one()) {
+                // U', then O
+#pragma unroll
+                for (int part = 0; part < 2; ++part) {
+                    const uint32_t rows = w_base + (part == 0 ? kBlock * 128 : 0);
+                    const uint32_t d = tmem_base + (part == 0 ? kUpdateColumn : kResultColumn);
+#pragma unroll
+                    for (int ks = 0; ks < kBlock / 16; ++ks) {
+                        const uint32_t x = tmem_base + kKeyColumn + (ks >> 1) * 32 + (ks & 1) * 8;
+                        const uint64_t upper = operand(rows + ks * 32, 16), lower = operand(rows + kTileBytes + ks * 32, 16);
+                        umma_f16(d, x, upper, kNarrow, 1u);
+                        umma_f16(d, x + 16, upper, kNarrow, 1u);
+                        umma_f16(d, x, lower, kNarrow, 1u);
+                    }
+                    umma_commit(part == 0 ? &sm.u_done : &sm.o_done);
+                }
+                umma_commit(&sm.w_empty[n & 1]);
+            }
+            __syncwarp();
+            ok = wait(&sm.u_ready, parity, failed, status);
             if (!ok) {
                 break;
             }
@@ -626,187 +747,254 @@ __global__ void __launch_bounds__((kChains * (kChainWarps + 1) + 1) * 32, 1) del
             if (elect_one()) {
 #pragma unroll
                 for (int ks = 0; ks < kBlock / 16; ++ks) {
-                    const uint64_t upper = operand(w_base + ks * 32, 16), lower = operand(w_base + kTileBytes + ks * 32, 16);
-                    const uint64_t r_upper = operand(r_base + ks * 2048, 16), r_lower = operand(r_base + kRBytes / 2 + ks * 2048, 16);
-                    mma_bf16(d2, upper, r_upper, kIdesc | kTransposeB, ks > 0 ? 1u : 0u);
-                    mma_bf16(d2, upper, r_lower, kIdesc | kTransposeB, 1u);
-                    mma_bf16(d2, lower, r_upper, kIdesc | kTransposeB, 1u);
+                    const uint32_t u = tmem_base + kUpdateColumn + (ks >> 1) * 32 + (ks & 1) * 8;
+                    const uint64_t b = operand(qk_base + kBlock * 128 + ks * 2048, kTileBytes);  // k, dims across
+                    umma_f16(tmem_base + kStateColumn, u, b, kWide | kTransposeB, 1u);
+                    umma_f16(tmem_base + kStateColumn, u + 16, b, kWide | kTransposeB, 1u);
                 }
-                umma_commit(&sm.d2_done[chain]);
-                umma_commit(&sm.w_empty);
-            }
-            __syncwarp();
-            ok = wait(&sm.u_ready[chain], parity, &sm.failed, status);
-            if (!ok) {
-                break;
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (elect_one()) {
-#pragma unroll
-                for (int ks = 0; ks < kBlock / 16; ++ks) {
-                    const uint64_t a = operand(qk_base + kBlock * 128 + ks * 2048, kTileBytes);  // k, dims across
-                    mma_bf16(d3, a, operand(r_base + ks * 2048, 16), kIdesc | kTransposeA | kTransposeB, ks > 0 ? 1u : 0u);
-                    mma_bf16(d3, a, operand(r_base + kRBytes / 2 + ks * 2048, 16), kIdesc | kTransposeA | kTransposeB, 1u);
-                }
-                umma_commit(&sm.d3_done[chain]);
+                umma_commit(&sm.s_done);
                 umma_commit(&sm.qk_empty[n & 1]);
             }
             __syncwarp();
+            if (n + 1 < blocks) {
+                ok = issue_values(n + 1);
+            }
         }
-    } else {
-        // ---------------- state, R, U' and the outputs -----------------------------------------------------
-        const int chain = warp / kChainWarps;
+    } else if (warp < kChainWarps) {
+        // ---------------- the chain --------------------------------------------------------------------
         const int quarter = warp & 3;
-        const int group = (warp >> 2) & 1;                       // of 32 columns
-        const int row = quarter * 32 + lane;                     // key dim; or q (0 .. 63) and k (64 ..) of a token
-        const int t = row & (kBlock - 1);
-        const int column = (first_chain + chain) * kColumns + group * 32;  // first value dim
-        const uint32_t lanes = static_cast<uint32_t>(quarter * 32) << 16;
-        const uint32_t d1 = tmem_base + chain * 256 + lanes + group * 32, d2 = d1 + kColumns, d3 = d2 + kColumns;
-        int first_block = 0;
-        for (int i = lane; i < sequence; i += 32) {
-            first_block += (chunk_span(begins, i, tokens).length + kBlock - 1) / kBlock;
-        }
-        first_block = static_cast<int>(__reduce_add_sync(0xffffffffu, first_block));
-        const float* decays = images.decay + (static_cast<size_t>(first_block) * v_heads + head) * kBlock;
-        const size_t state_row = (static_cast<size_t>(slot) * v_heads + head) * kDim + column;
-        if (continues == nullptr || __ldcg(continues + sequence) != 0) {
+        const int group = warp >> 2;
+        const int row = quarter * 32 + lane;
+        const uint32_t tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        const uint32_t held = tmem + kStateColumn + group * 64;                // 64 key dims of the row
+        const uint32_t upper = tmem + kSplitColumn + group * 32, lower = upper + 64;
+        const uint32_t x_at = tmem + kKeyColumn + group * 32, u_at = tmem + kUpdateColumn + group * 32;
+        const size_t state_row = (static_cast<size_t>(slot) * v_heads + head) * kDim + row;
+        {
+            const bool holds = continues == nullptr || __ldcg(continues + sequence) != 0;
+            const float scale = holds ? state_scales[state_row] : 0.0f;
+            const uint4* codes = reinterpret_cast<const uint4*>(state + state_row * kDim + group * 64);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                s[i] = state[(state_row + i) * kDim + row] * state_scales[state_row + i];
-            }
-        } else {
+            for (int c = 0; c < 2; ++c) {
+                float s[32];
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                s[i] = 0.0f;
-            }
-        }
-        const __nv_bfloat16* v_rows = qkv + static_cast<size_t>(span.begin) * channels + (2 * kDeltaKeyHeads + head) * kDim + column;
-        uint4 v_next[4] = {};
-        if (quarter >= 2 && t < span.length) {
+                for (int i = 0; i < 2; ++i) {
+                    const uint4 raw = codes[2 * c + i];
+                    const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                v_next[i] = *(reinterpret_cast<const uint4*>(v_rows + static_cast<size_t>(t) * channels) + i);
+                    for (int j = 0; j < 16; ++j) {
+                        s[16 * i + j] = holds ? static_cast<float>(static_cast<int8_t>(words[j >> 2] >> (8 * (j & 3)))) * scale : 0.0f;
+                    }
+                }
+                tmem_store_columns(held + 32 * c, s);
+                tmem_store_split(upper + 16 * c, lower + 16 * c, s);
             }
         }
-        float decay_next = decays[t], end_next = decays[kBlock - 1];
-        store_split(sm.s[chain], kTileBytes, row, 4 * group, s);
-        fence_proxy_async();
+        tmem_store_wait();
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
         __syncwarp();
         if (lane == 0) {
-            mbar_arrive(&sm.s_ready[chain]);
+            mbar_arrive(&sm.s_ready);
         }
         for (; n < blocks; ++n) {
             const uint32_t parity = n & 1;
-            const int token = n * kBlock + t;
-            const bool live = token < span.length;
-            const float decay = decay_next, end = end_next;
-            if (n + 1 < blocks) {
-                decays += static_cast<size_t>(v_heads) * kBlock;
-                decay_next = decays[t];
-                end_next = decays[kBlock - 1];
+            const float* decay = sm.decay[n & 1];
+            float x[32];
+            ok = wait(&sm.w_full[n & 1], (n >> 1) & 1, failed, status) && wait(&sm.x_done, parity, failed, status);
+            if (!ok) {
+                break;
             }
-            if (quarter >= 2) {
-                float v[32], x[32];
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            load_columns(x_at, x);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    unpack_bf16(v_next[i], v + 8 * i);
-                }
-                if (token + kBlock < span.length) {
+            for (int i = 0; i < 8; ++i) {
+                const float4 g = *reinterpret_cast<const float4*>(decay + group * 32 + 4 * i);
+                x[4 * i] *= -g.x;
+                x[4 * i + 1] *= -g.y;
+                x[4 * i + 2] *= -g.z;
+                x[4 * i + 3] *= -g.w;
+            }
+            tmem_store_split(x_at, x_at + 16, x);
+            tmem_store_wait();
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.x_ready);
+            }
+            // the state decays while U' is made
+            const float end = decay[kBlock - 1];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        v_next[i] = *(reinterpret_cast<const uint4*>(v_rows + static_cast<size_t>(token + kBlock) * channels) + i);
-                    }
-                }
-                ok = wait(&sm.d1_done[chain], parity, &sm.failed, status);
-                if (!ok) {
-                    break;
-                }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                load_columns(d1, x);
+            for (int c = 0; c < 2; ++c) {
+                load_columns(held + 32 * c, x);
 #pragma unroll
                 for (int i = 0; i < 32; ++i) {
-                    x[i] = live ? fmaf(-decay, x[i], v[i]) : 0.0f;
+                    x[i] *= end;
                 }
-                store_split(sm.r[chain], kRBytes / 2, t, 4 * group, x);
-                fence_proxy_async();
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&sm.r_ready[chain]);
-                }
-                ok = wait(&sm.d2_done[chain], parity, &sm.failed, status);
-                if (!ok) {
-                    break;
-                }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                load_columns(d2, x);
-                store_split(sm.r[chain], kRBytes / 2, t, 4 * group, x);
-                fence_proxy_async();
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&sm.u_ready[chain]);
-                }
-            } else {
-                ok = wait(&sm.d2_done[chain], parity, &sm.failed, status);
-                if (!ok) {
-                    break;
-                }
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                float x[32], y[32];
-                load_columns(d1, x);
-                load_columns(d2, y);
-                if (live) {
-                    uint4* to = reinterpret_cast<uint4*>(out + ((static_cast<size_t>(span.begin) + token) * v_heads + head) * kDim + column);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t words[4];
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) {
-                            const int e = 8 * i + 2 * j;
-                            const __nv_bfloat162 pair = __floats2bfloat162_rn(fmaf(decay, x[e], y[e]), fmaf(decay, x[e + 1], y[e + 1]));
-                            words[j] = *reinterpret_cast<const uint32_t*>(&pair);
-                        }
-                        to[i] = make_uint4(words[0], words[1], words[2], words[3]);
-                    }
-                }
-                __syncwarp();
+                tmem_store_columns(held + 32 * c, x);
             }
-            ok = wait(&sm.d3_done[chain], parity, &sm.failed, status);
+            ok = wait(&sm.u_done, parity, failed, status);
+            if (!ok) {
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            load_columns(u_at, x);
+            tmem_store_split(u_at, u_at + 16, x);
+            tmem_store_wait();
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.u_ready);
+            }
+            ok = wait(&sm.s_done, parity, failed, status);
+            if (!ok) {
+                break;
+            }
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (n + 1 < blocks) {
+#pragma unroll
+                for (int c = 0; c < 2; ++c) {
+                    load_columns(held + 32 * c, x);
+                    tmem_store_split(upper + 16 * c, lower + 16 * c, x);
+                }
+                tmem_store_wait();
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&sm.s_ready);
+                }
+            }
+        }
+        float peak = 0.0f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+            float s[32];
+            load_columns(held + 32 * c, s);
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                peak = fmaxf(peak, fabsf(s[i]));
+            }
+        }
+        sm.peak[group][row] = peak;
+    } else {
+        // ---------------- outputs ----------------------------------------------------------------------
+        const int quarter = warp & 3;
+        const int group = (warp - kChainWarps) >> 2;
+        const int row = quarter * 32 + lane;     // value dim
+        const uint32_t tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + group * 32;
+        const int piece = lane & 15;             // later: value dims 4 piece .. + 3 and 64 + 4 piece .. + 3 of a token
+        float gain[8] = {};
+        if (norm.gate != nullptr) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const uint2 raw = *reinterpret_cast<const uint2*>(norm.weight + 64 * i + 4 * piece);
+                gain[4 * i] = __uint_as_float(raw.x << 16);
+                gain[4 * i + 1] = __uint_as_float(raw.x & 0xffff0000u);
+                gain[4 * i + 2] = __uint_as_float(raw.y << 16);
+                gain[4 * i + 3] = __uint_as_float(raw.y & 0xffff0000u);
+            }
+        }
+        for (; n < blocks; ++n) {
+            const uint32_t parity = n & 1;
+            // the gates of this block's rows, ahead
+            uint2 gates[4][2] = {};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int token = n * kBlock + (warp - kChainWarps) * 8 + 2 * i + (lane >> 4);
+                if (norm.gate != nullptr && token < span.length) {
+                    const __nv_bfloat16* from =
+                        norm.gate + (static_cast<size_t>(span.begin) + token) * norm.gate_stride + head * kDim + 4 * piece;
+                    gates[i][0] = *reinterpret_cast<const uint2*>(from);
+                    gates[i][1] = *reinterpret_cast<const uint2*>(from + 64);
+                }
+            }
+            ok = wait(&sm.w_full[n & 1], (n >> 1) & 1, failed, status) && wait(&sm.o_done, parity, failed, status);
             if (!ok) {
                 break;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             float x[32];
-            load_columns(d3, x);
+            {
+                float y[32];
+                load_columns(tmem + kResultColumn, x);
+                load_columns(tmem + kQueryColumn, y);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                s[i] = fmaf(end, s[i], x[i]);
-            }
-            if (n + 1 < blocks) {
-                store_split(sm.s[chain], kTileBytes, row, 4 * group, s);
-                fence_proxy_async();
-                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&sm.s_ready[chain]);
+                for (int i = 0; i < 8; ++i) {
+                    const float4 g = *reinterpret_cast<const float4*>(&sm.decay[n & 1][group * 32 + 4 * i]);
+                    x[4 * i] = fmaf(g.x, y[4 * i], x[4 * i]);
+                    x[4 * i + 1] = fmaf(g.y, y[4 * i + 1], x[4 * i + 1]);
+                    x[4 * i + 2] = fmaf(g.z, y[4 * i + 2], x[4 * i + 2]);
+                    x[4 * i + 3] = fmaf(g.w, y[4 * i + 3], x[4 * i + 3]);
                 }
             }
-        }
-        // the largest of a row of the state: over the warp's key dims, then over the quarters
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.o_free);
+                mbar_arrive(&sm.w_empty[n & 1]);
+            }
+            ok = wait(&sm.rows_free, parity ^ 1, failed, status);
+            if (!ok) {
+                break;
+            }
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            float highest;
-            asm volatile("redux.sync.max.abs.f32 %0, %1, 0xffffffff;" : "=f"(highest) : "f"(s[i]));
-            if (lane == i) {
-                sm.peak[chain][quarter][group * 32 + i] = highest;
+            for (int i = 0; i < 32; ++i) {
+                sm.rows[(group * 32 + i) * kDim + row] = x[i];
+            }
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.rows_ready);
+            }
+            ok = wait(&sm.rows_ready, parity, failed, status);
+            if (!ok) {
+                break;
+            }
+            // rows of the batch: eight tokens of this warp, two at a time
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = (warp - kChainWarps) * 8 + 2 * i + (lane >> 4);
+                const int token = n * kBlock + t;
+                const float4 lo = *reinterpret_cast<const float4*>(&sm.rows[t * kDim + 4 * piece]);
+                const float4 hi = *reinterpret_cast<const float4*>(&sm.rows[t * kDim + 64 + 4 * piece]);
+                float o[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+                if (norm.gate != nullptr) {
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        sum = fmaf(o[j], o[j], sum);
+                    }
+#pragma unroll
+                    for (int offset = 1; offset < 16; offset <<= 1) {
+                        sum += __shfl_xor_sync(0xffffffffu, sum, offset);
+                    }
+                    const float inverse = rsqrtf(sum / static_cast<float>(kDim) + norm.epsilon);
+                    const uint32_t words[4] = {gates[i][0].x, gates[i][0].y, gates[i][1].x, gates[i][1].y};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        const float z = __uint_as_float((j & 1) != 0 ? words[j >> 1] & 0xffff0000u : words[j >> 1] << 16);
+                        o[j] *= inverse * gain[j] * __fdividef(z, 1.0f + __expf(-z));
+                    }
+                }
+                uint32_t words[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const __nv_bfloat162 pair = __floats2bfloat162_rn(o[2 * j], o[2 * j + 1]);
+                    words[j] = *reinterpret_cast<const uint32_t*>(&pair);
+                }
+                if (token < span.length) {
+                    __nv_bfloat16* to = out + ((static_cast<size_t>(span.begin) + token) * v_heads + head) * kDim + 4 * piece;
+                    *reinterpret_cast<uint2*>(to) = make_uint2(words[0], words[1]);
+                    *reinterpret_cast<uint2*>(to + 64) = make_uint2(words[2], words[3]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.rows_free);
             }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
-    if (*reinterpret_cast<volatile int*>(&sm.failed) != 0) {
+    if (*reinterpret_cast<volatile int*>(failed) != 0) {
         // A wait gave up somewhere.  What was asked for and arrives by itself is waited for, 0.2 ms at most for each.
         const auto arrived = [](uint64_t* bar, uint32_t parity) {
             const long long start = clock64();
@@ -814,97 +1002,46 @@ __global__ void __launch_bounds__((kChains * (kChainWarps + 1) + 1) * 32, 1) del
             }
         };
         if (warp == kLoadWarp) {
-            for (int i = n > 2 ? n - 2 : 0; i < n; ++i) {
+            for (int i = n > 2 ? n - 2 : 0; i <= n && i < blocks; ++i) {
                 arrived(&sm.qk_full[i & 1], (i >> 1) & 1);
+                arrived(&sm.w_full[i & 1], (i >> 1) & 1);
             }
-            if (n > 0) {
-                arrived(&sm.w_full, (n - 1) & 1);
-            }
-        } else if (warp >= kFirstMmaWarp) {
-            const int chain = warp - kFirstMmaWarp;
-            arrived(&sm.d1_done[chain], n & 1);
-            arrived(&sm.d2_done[chain], n & 1);
-            arrived(&sm.d3_done[chain], n & 1);
+        } else if (warp == kMmaWarp) {
+            arrived(&sm.v_empty[n & 1], (n >> 1) & 1);
+            arrived(&sm.o_done, n & 1);
+            arrived(&sm.s_done, n & 1);
         }
-        __syncthreads();
-    } else if (warp < kFirstMmaWarp) {
-        const int chain = warp / kChainWarps;
-        const int quarter = warp & 3, group = (warp >> 2) & 1;
+    } else if (warp < kChainWarps) {
+        // the state's eight bits: 64 of a row
+        const int quarter = warp & 3, group = warp >> 2;
         const int row = quarter * 32 + lane;
-        const size_t state_row = (static_cast<size_t>(slot) * v_heads + head) * kDim + (first_chain + chain) * kColumns + group * 32;
+        const uint32_t held = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kStateColumn + group * 64;
+        const size_t state_row = (static_cast<size_t>(slot) * v_heads + head) * kDim + row;
+        const float peak = fmaxf(sm.peak[0][row], sm.peak[1][row]);
+        const float inverse = peak == 0.0f ? 0.0f : __fdiv_rn(127.0f, peak);
+        uint4* codes = reinterpret_cast<uint4*>(state + state_row * kDim + group * 64);
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            const float* peaks = &sm.peak[chain][0][group * 32 + i];
-            const float peak = fmaxf(fmaxf(peaks[0], peaks[kColumns]), fmaxf(peaks[2 * kColumns], peaks[3 * kColumns]));
-            const float inverse = peak == 0.0f ? 0.0f : __fdiv_rn(127.0f, peak);
-            state[(state_row + i) * kDim + row] = static_cast<int8_t>(__float2int_rn(s[i] * inverse));
-            if (quarter == 0 && lane == i) {
-                state_scales[state_row + i] = __fmul_rn(peak, 1.0f / 127.0f);
+        for (int c = 0; c < 2; ++c) {
+            float s[32];
+            load_columns(held + 32 * c, s);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t words[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    words[j >> 2] |= (static_cast<uint32_t>(__float2int_rn(s[16 * i + j] * inverse)) & 0xffu) << (8 * (j & 3));
+                }
+                codes[2 * c + i] = make_uint4(words[0], words[1], words[2], words[3]);
             }
+        }
+        if (group == 0) {
+            state_scales[state_row] = __fmul_rn(peak, 1.0f / 127.0f);
         }
     }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
     if (warp == kLoadWarp) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemColumns) : "memory");
-    }
-}
-
-// RMSNorm over the 128 dims of a value head, times weight, times silu(gate): in place on the bf16 rows of the batch's
-// chunks, one rounding.  Sixteen lanes to a token and head, eight dims each; a warp has eight rows in flight.
-constexpr int kNormWarps = 8;
-constexpr int kNormRows = 8;  // of a warp
-
-__global__ void __launch_bounds__(kNormWarps * 32) delta_norm_rows_kernel(
-    __nv_bfloat16* __restrict__ rows, const __nv_bfloat16* __restrict__ gate, const __nv_bfloat16* __restrict__ weight,
-    const uint32_t* __restrict__ begins, int sequences, int tokens, int v_heads, int gate_stride, float epsilon) {
-    pdl_launch_dependents();
-    const int lane = threadIdx.x & 31;
-    const int piece = lane & 15;
-    const uint32_t first = (blockIdx.x * kNormWarps + (threadIdx.x >> 5)) * kNormRows + (lane >> 4);
-    float gain[8];
-    unpack_bf16(*(reinterpret_cast<const uint4*>(weight) + piece), gain);
-    pdl_wait();
-    const uint32_t low = __ldcg(begins), high = min(__ldcg(begins + sequences), static_cast<uint32_t>(tokens));
-    uint4 raw[kNormRows / 2], gates[kNormRows / 2];
-#pragma unroll
-    for (int i = 0; i < kNormRows / 2; ++i) {
-        const uint32_t row = first + 2 * i;
-        const uint32_t token = row / v_heads, head = row % v_heads;
-        raw[i] = gates[i] = make_uint4(0, 0, 0, 0);
-        if (token >= low && token < high) {
-            raw[i] = *(reinterpret_cast<const uint4*>(rows + static_cast<size_t>(row) * kDim) + piece);
-            gates[i] = *(reinterpret_cast<const uint4*>(gate + static_cast<size_t>(token) * gate_stride + head * kDim) + piece);
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < kNormRows / 2; ++i) {
-        const uint32_t row = first + 2 * i;
-        const uint32_t token = row / v_heads;
-        float x[8], z[8];
-        unpack_bf16(raw[i], x);
-        unpack_bf16(gates[i], z);
-        float sum = 0.0f;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            sum = fmaf(x[j], x[j], sum);
-        }
-#pragma unroll
-        for (int offset = 1; offset < 16; offset <<= 1) {
-            sum += __shfl_xor_sync(0xffffffffu, sum, offset);
-        }
-        const float inverse = rsqrtf(sum / static_cast<float>(kDim) + epsilon);
-        uint32_t words[4];
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            x[j] *= inverse * gain[j] * __fdividef(z[j], 1.0f + __expf(-z[j]));
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const __nv_bfloat162 pair = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-            words[j] = *reinterpret_cast<const uint32_t*>(&pair);
-        }
-        if (token >= low && token < high) {
-            *(reinterpret_cast<uint4*>(rows + static_cast<size_t>(row) * kDim) + piece) = make_uint4(words[0], words[1], words[2], words[3]);
-        }
     }
 }
 
@@ -946,63 +1083,36 @@ extern "C" int qwc_delta_chunk_int8(void* state, float* state_scales, const void
     if (status == nullptr) {
         return cudaErrorInvalidValue;
     }
-    struct Setup {
-        cudaError_t error;
-        int sms;
-    };
-    static PerDevice<Setup> per_device;
-    const Setup* setup = per_device.get([]() {
-        Setup found = {cudaSuccess, 0};
-        int device = 0;
-        found.error = cudaFuncSetAttribute(delta_factor_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                           static_cast<int>(sizeof(FactorSmem)) + 1024);
-        if (found.error == cudaSuccess) {
-            found.error = cudaFuncSetAttribute(delta_chain_kernel<1>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(sizeof(ChainSmem<1>)) + 1024);
+    static PerDevice<cudaError_t> per_device;
+    const cudaError_t* setup = per_device.get([]() {
+        cudaError_t error = cudaFuncSetAttribute(delta_factor_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                                 static_cast<int>(sizeof(FactorSmem)) + 1024);
+        if (error == cudaSuccess) {
+            error = cudaFuncSetAttribute(delta_chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                         static_cast<int>(sizeof(ChainSmem)) + 1024);
         }
-        if (found.error == cudaSuccess) {
-            found.error = cudaFuncSetAttribute(delta_chain_kernel<2>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               static_cast<int>(sizeof(ChainSmem<2>)) + 1024);
-        }
-        if (found.error == cudaSuccess) {
-            found.error = cudaGetDevice(&device);
-        }
-        if (found.error == cudaSuccess) {
-            found.error = cudaDeviceGetAttribute(&found.sms, cudaDevAttrMultiProcessorCount, device);
-        }
-        return found;
+        return error;
     });
     if (setup == nullptr) {
         return cudaErrorInvalidDevice;
     }
-    if (setup->error != cudaSuccess) {
-        return setup->error;
+    if (*setup != cudaSuccess) {
+        return *setup;
     }
     const int blocks = most_chunk_tiles(tokens, sequences, kBlock);
     const Images images = images_at(workspace, blocks, v_heads);
-    cudaError_t launched = launch_chained(
+    const cudaError_t launched = launch_chained(
         delta_factor_kernel, dim3(v_heads, blocks), dim3(kFactorThreads), sizeof(FactorSmem) + 1024, stream,
         static_cast<const __nv_bfloat16*>(qkv), static_cast<const float*>(alpha), static_cast<const float*>(beta),
         static_cast<const uint32_t*>(chunk_begins), images, tokens, sequences, v_heads, status);
     if (launched != cudaSuccess) {
         return launched;
     }
-    // A head's two chains on an SM each as long as there are SMs for all of them.
-    const bool apart = 2 * v_heads * sequences <= setup->sms;
-    launched = launch_chained(
-        apart ? delta_chain_kernel<1> : delta_chain_kernel<2>, dim3(apart ? 2 * v_heads : v_heads, sequences),
-        dim3((apart ? kChainWarps + 2 : 2 * kChainWarps + 3) * 32),
-        (apart ? sizeof(ChainSmem<1>) : sizeof(ChainSmem<2>)) + 1024, stream, static_cast<int8_t*>(state), state_scales,
-        static_cast<const uint32_t*>(state_slots), static_cast<const uint32_t*>(continues),
-        static_cast<const uint32_t*>(chunk_begins), static_cast<const __nv_bfloat16*>(qkv), images,
-        static_cast<__nv_bfloat16*>(out), tokens, v_heads, state_capacity, status);
-    if (launched != cudaSuccess || gate == nullptr) {
-        return launched;
-    }
-    const int items = tokens * v_heads;  // at most 65536 * 48
-    constexpr int kItems = kNormWarps * kNormRows;
-    return launch_chained(delta_norm_rows_kernel, dim3((items + kItems - 1) / kItems), dim3(kNormWarps * 32), 0, stream,
-                           static_cast<__nv_bfloat16*>(out), static_cast<const __nv_bfloat16*>(gate),
-                          static_cast<const __nv_bfloat16*>(norm_weight), static_cast<const uint32_t*>(chunk_begins),
-                          sequences, tokens, v_heads, gate_stride, epsilon);
+    const OutputNorm norm = {static_cast<const __nv_bfloat16*>(gate), static_cast<const __nv_bfloat16*>(norm_weight),
+                             gate_stride, epsilon};
+    return launch_chained(delta_chain_kernel, dim3(v_heads, sequences), dim3(kChainThreads), sizeof(ChainSmem) + 1024, stream,
+                          static_cast<int8_t*>(state), state_scales, static_cast<const uint32_t*>(state_slots),
+                          static_cast<const uint32_t*>(continues), static_cast<const uint32_t*>(chunk_begins),
+                          static_cast<const __nv_bfloat16*>(qkv), images, static_cast<__nv_bfloat16*>(out), tokens, v_heads,
+                          state_capacity, norm, status);
 }
