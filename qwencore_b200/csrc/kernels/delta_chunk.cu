@@ -77,10 +77,15 @@ constexpr uint32_t kTransposeA = 1u << 15, kTransposeB = 1u << 16;
 
 // Operand of 128-byte rows with the 128-byte swizzle, eight rows to an atom.  K-major: a row is one of M or N, its bytes 64
 // of the contracted elements.  MN-major: a row is one of the contracted, its bytes 64 of M or N, the next 64 `block` bytes on.
-__device__ __forceinline__ uint64_t operand(uint32_t address, uint32_t block) {
-    const uint64_t lo = ((address >> 4) & 0x3FFFu) | (static_cast<uint64_t>((block >> 4) & 0x3FFFu) << 16);
-    const uint64_t hi = (1024u >> 4) | (1u << 14) | (2u << 29);
-    return lo | (hi << 32);
+// Made in two steps, the lower word of its beginning once and then the part of it that an MMA reads: the thread that issues
+// needs an operand in uniform registers, and one addition is all that is left there (it is what the issue then takes).
+__device__ __forceinline__ uint32_t operand_base(uint32_t address, uint32_t block) {
+    return ((address >> 4) & 0x3FFFu) | ((block >> 4) & 0x3FFFu) << 16;
+}
+
+__device__ __forceinline__ uint64_t operand_at(uint32_t base, uint32_t bytes) {
+    constexpr uint32_t kUpper = (1024u >> 4) | (1u << 14) | (2u << 29);
+    return static_cast<uint64_t>(kUpper) << 32 | (base + (bytes >> 4));
 }
 
 // Where 16 bytes of a row lie.
@@ -283,11 +288,11 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
     if (here) {
         if (warp == 0) {
             if (elect_one()) {
-                const uint32_t base = smem_u32(sm.operand);
+                const uint32_t base = operand_base(smem_u32(sm.operand), 16);
 #pragma unroll
                 for (int ks = 0; ks < kDim / 16; ++ks) {
-                    const uint32_t at = base + (ks >> 2) * kTileBytes + (ks & 3) * 32;
-                    mma_bf16(tmem_base, operand(at, 16), operand(at + kBlock * 128, 16), idesc_of(kBlock), ks > 0 ? 1u : 0u);
+                    const uint32_t at = (ks >> 2) * kTileBytes + (ks & 3) * 32;
+                    mma_bf16(tmem_base, operand_at(base, at), operand_at(base, at + kBlock * 128), idesc_of(kBlock), ks > 0 ? 1u : 0u);
                 }
                 umma_commit(&sm.done);
             }
@@ -448,11 +453,11 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (warp == 0) {
             if (elect_one()) {
-                const uint32_t a = smem_u32(sm.operand), b = smem_u32(sm.product);
+                const uint32_t a = operand_base(smem_u32(sm.operand), 16), b = operand_base(smem_u32(sm.product), 16);
 #pragma unroll
                 for (int ks = 0; ks < kBlock / 16; ++ks) {
-                    const uint64_t upper = operand(a + ks * 32, 16), lower = operand(a + kTileBytes + ks * 32, 16);
-                    const uint64_t t_upper = operand(b + ks * 2048, 16), t_lower = operand(b + kProductBytes / 2 + ks * 2048, 16);
+                    const uint64_t upper = operand_at(a, ks * 32), lower = operand_at(a, kTileBytes + ks * 32);
+                    const uint64_t t_upper = operand_at(b, ks * 2048), t_lower = operand_at(b, kProductBytes / 2 + ks * 2048);
                     mma_bf16(tmem_base, upper, t_upper, idesc_of(kBlock) | kTransposeB, ks > 0 ? 1u : 0u);
                     mma_bf16(tmem_base, upper, t_lower, idesc_of(kBlock) | kTransposeB, 1u);
                     mma_bf16(tmem_base, lower, t_upper, idesc_of(kBlock) | kTransposeB, 1u);
@@ -485,13 +490,14 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
 //   warps 0-7    the chain: four quarters of the 128 rows, two groups of columns
 //   warps 8-15   outputs: the same division, then rows of the batch, norm and gate
 //   warp 16      issues the MMAs
-//   warp 17      fetches K, Q, W and V of the next block
+//   warp 17      fetches K, Q, W and V of the next block, warp 18 the gates of the next outputs
 
 constexpr int kChainWarps = 8;
 constexpr int kOutputWarps = 8;
 constexpr int kMmaWarp = kChainWarps + kOutputWarps;
 constexpr int kLoadWarp = kMmaWarp + 1;
-constexpr int kChainThreads = (kLoadWarp + 1) * 32;
+constexpr int kGateWarp = kLoadWarp + 1;
+constexpr int kChainThreads = (kGateWarp + 1) * 32;
 // tensor memory
 constexpr int kStateColumn = 0;                          // fp32, 128 key dims
 constexpr int kSplitColumn = 128;                        // upper (64 columns), lower
@@ -499,18 +505,19 @@ constexpr int kKeyColumn = 256;                          // X of 64 tokens; then
 constexpr int kQueryColumn = 320;                        // Y
 constexpr int kResultColumn = 384;                       // O, U'; then U' split as X
 constexpr int kUpdateColumn = kResultColumn + kBlock;
-constexpr int kTmemColumns = 512;
+constexpr int kTmemColumns = 512;                        // all of it: the address that the allocation returns is 0
 
 struct ChainSmem {
     uint8_t qk[2][kQkBytes];
     uint8_t w[2][kWBytes];
-    uint8_t v[2][kVBytes];
+    uint8_t v[kVBytes];
     float rows[kBlock * kDim];          // outputs of a block
+    uint8_t gate[2][kBlock * kDim * 2]; // [token][256 bytes]
     float decay[2][kBlock];
     float peak[2][kDim];
-    uint64_t qk_full[2], qk_empty[2], w_full[2], w_empty[2], v_full[2], v_empty[2];
+    uint64_t qk_full[2], qk_empty[2], w_full[2], w_empty[2], v_full, v_empty;
     uint64_t s_ready, x_done, x_ready, u_done, u_ready, o_done, o_free, s_done;
-    uint64_t rows_ready, rows_free;
+    uint64_t rows_ready, rows_free, gate_full[2], gate_empty[2];
     uint32_t tmem_base;
     int failed;
 };
@@ -590,8 +597,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             mbar_init(&sm.qk_empty[i], 1);
             mbar_init(&sm.w_full[i], 1);
             mbar_init(&sm.w_empty[i], 1 + kOutputWarps);  // the MMAs, and who reads the decays
-            mbar_init(&sm.v_full[i], 1);
-            mbar_init(&sm.v_empty[i], 1);
+            mbar_init(&sm.gate_full[i], 1);
+            mbar_init(&sm.gate_empty[i], kOutputWarps);
         }
         mbar_init(&sm.s_ready, kChainWarps);
         mbar_init(&sm.x_done, 1);
@@ -603,6 +610,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
         mbar_init(&sm.s_done, 1);
         mbar_init(&sm.rows_ready, kOutputWarps);
         mbar_init(&sm.rows_free, kOutputWarps);
+        mbar_init(&sm.v_full, 1);
+        mbar_init(&sm.v_empty, 1);
         sm.failed = 0;
         mbar_fence_init();
     }
@@ -610,7 +619,6 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
     __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     pdl_launch_dependents();  // (this CTA has its tensor memory)
-    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sm.tmem_base);
     int* const failed = &sm.failed;
     bool ok = true;
     int n = 0;  // blocks so far
@@ -634,7 +642,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 bulk_g2s(sm.decay[slot_of], images.decay + (block * v_heads + head) * kBlock, kBlock * 4, &sm.w_full[slot_of]);
             }
             __syncwarp();
-            ok = ok && wait(&sm.v_empty[slot_of], parity, failed, status);
+            ok = ok && wait(&sm.v_empty, (n & 1) ^ 1, failed, status);
             if (ok) {
                 // rows of v, zeros behind the chunk: sixteen lanes to a row
                 const int piece = lane & 15;
@@ -644,7 +652,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                     const int token = n * kBlock + t;
                     const bool live = token < span.length;
                     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                     smem_u32(sm.v[slot_of] + (piece >> 3) * (kVBytes / 2) + swizzled(t, piece & 7))),
+                                     smem_u32(sm.v + (piece >> 3) * (kVBytes / 2) + swizzled(t, piece & 7))),
                                  "l"(v_rows + static_cast<size_t>(live ? token : 0) * channels + 8 * piece), "r"(live ? 16 : 0)
                                  : "memory");
                 }
@@ -659,31 +667,59 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             fence_proxy_async();
             __syncwarp();
             if (ok && lane == 0) {
-                mbar_arrive(&sm.v_full[slot_of]);
+                mbar_arrive(&sm.v_full);
+            }
+            __syncwarp();
+        }
+    } else if (warp == kGateWarp) {
+        // ---------------- gates of the blocks' rows ---------------------------------------------------------
+        const int piece = lane & 15;
+        const __nv_bfloat16* rows = norm.gate + static_cast<size_t>(span.begin) * norm.gate_stride + head * kDim + 8 * piece;
+        for (; norm.gate != nullptr && n < blocks && ok; ++n) {
+            ok = wait(&sm.gate_empty[n & 1], ((n >> 1) & 1) ^ 1, failed, status);
+            if (ok) {
+#pragma unroll 4
+                for (int i = 0; i < kBlock / 2; ++i) {
+                    const int t = 2 * i + (lane >> 4);
+                    const int token = n * kBlock + t;
+                    const bool live = token < span.length;
+                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(sm.gate[n & 1] + t * (kDim * 2) + 16 * piece)),
+                                 "l"(rows + static_cast<size_t>(live ? token : 0) * norm.gate_stride), "r"(live ? 16 : 0)
+                                 : "memory");
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            __syncwarp();
+            if (ok && lane == 0) {
+                mbar_arrive(&sm.gate_full[n & 1]);
             }
             __syncwarp();
         }
     } else if (warp == kMmaWarp) {
         // ---------------- tensor-core issue ------------------------------------------------------------
         constexpr uint32_t kWide = idesc_of(kDim), kNarrow = idesc_of(kBlock);
+        const uint32_t qk_operand = operand_base(smem_u32(sm.qk[0]), 16), w_operand = operand_base(smem_u32(sm.w[0]), 16);
+        const uint32_t k_across = operand_base(smem_u32(sm.qk[0]) + kBlock * 128, kTileBytes);  // k, dims across
+        const uint32_t v_operand = operand_base(smem_u32(sm.v), kVBytes / 2);
         // [O | U'] begins as V^T W^T
         const auto issue_values = [&](int number) {
             const int slot_of = number & 1;
             if (!wait(&sm.w_full[slot_of], (number >> 1) & 1, failed, status) ||
-                !wait(&sm.v_full[slot_of], (number >> 1) & 1, failed, status) ||
+                !wait(&sm.v_full, number & 1, failed, status) ||
                 !wait(&sm.o_free, (number & 1) ^ 1, failed, status)) {
                 return false;
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (elect_one()) {
-                const uint32_t v_base = smem_u32(sm.v[slot_of]), w_base = smem_u32(sm.w[slot_of]);
+                const uint32_t w_base = w_operand + slot_of * (kWBytes >> 4);
 #pragma unroll
                 for (int ks = 0; ks < kBlock / 16; ++ks) {
-                    const uint64_t a = operand(v_base + ks * 2048, kVBytes / 2);
-                    mma_bf16(tmem_base + kResultColumn, a, operand(w_base + ks * 32, 16), kWide | kTransposeA, ks > 0 ? 1u : 0u);
-                    mma_bf16(tmem_base + kResultColumn, a, operand(w_base + kTileBytes + ks * 32, 16), kWide | kTransposeA, 1u);
+                    const uint64_t a = operand_at(v_operand, ks * 2048);
+                    mma_bf16(kResultColumn, a, operand_at(w_base, ks * 32), kWide | kTransposeA, ks > 0 ? 1u : 0u);
+                    mma_bf16(kResultColumn, a, operand_at(w_base, kTileBytes + ks * 32), kWide | kTransposeA, 1u);
                 }
-                umma_commit(&sm.v_empty[slot_of]);
+                umma_commit(&sm.v_empty);
             }
             __syncwarp();
             return true;
@@ -691,7 +727,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
         ok = issue_values(0);
         for (; n < blocks && ok; ++n) {
             const uint32_t parity = n & 1;
-            const uint32_t qk_base = smem_u32(sm.qk[n & 1]), w_base = smem_u32(sm.w[n & 1]);
+            const uint32_t qk_offset = (n & 1) * (kQkBytes >> 4);
+            const uint32_t qk_base = qk_operand + qk_offset, w_base = w_operand + (n & 1) * (kWBytes >> 4);
             ok = wait(&sm.qk_full[n & 1], (n >> 1) & 1, failed, status) && wait(&sm.s_ready, parity, failed, status);
             if (!ok) {
                 break;
@@ -701,13 +738,13 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 // X, then Y
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {
-                    const uint32_t rows = qk_base + (part == 0 ? kBlock * 128 : 0);
-                    const uint32_t d = tmem_base + (part == 0 ? kKeyColumn : kQueryColumn);
+                    const uint32_t rows = part == 0 ? kBlock * 128 : 0;
+                    const uint32_t d = part == 0 ? kKeyColumn : kQueryColumn;
 #pragma unroll
                     for (int ks = 0; ks < kDim / 16; ++ks) {
-                        const uint64_t b = operand(rows + (ks >> 2) * kTileBytes + (ks & 3) * 32, 16);
-                        umma_f16(d, tmem_base + kSplitColumn + ks * 8, b, kNarrow, ks > 0 ? 1u : 0u);
-                        umma_f16(d, tmem_base + kSplitColumn + 64 + ks * 8, b, kNarrow, 1u);
+                        const uint64_t b = operand_at(qk_base, rows + (ks >> 2) * kTileBytes + (ks & 3) * 32);
+                        umma_f16(d, kSplitColumn + ks * 8, b, kNarrow, ks > 0 ? 1u : 0u);
+                        umma_f16(d, kSplitColumn + 64 + ks * 8, b, kNarrow, 1u);
                     }
                     if (part == 0) {
                         umma_commit(&sm.x_done);
@@ -724,12 +761,12 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 // U', then O
 #pragma unroll
                 for (int part = 0; part < 2; ++part) {
-                    const uint32_t rows = w_base + (part == 0 ? kBlock * 128 : 0);
-                    const uint32_t d = tmem_base + (part == 0 ? kUpdateColumn : kResultColumn);
+                    const uint32_t rows = part == 0 ? kBlock * 128 : 0;
+                    const uint32_t d = part == 0 ? kUpdateColumn : kResultColumn;
 #pragma unroll
                     for (int ks = 0; ks < kBlock / 16; ++ks) {
-                        const uint32_t x = tmem_base + kKeyColumn + (ks >> 1) * 32 + (ks & 1) * 8;
-                        const uint64_t upper = operand(rows + ks * 32, 16), lower = operand(rows + kTileBytes + ks * 32, 16);
+                        const uint32_t x = kKeyColumn + (ks >> 1) * 32 + (ks & 1) * 8;
+                        const uint64_t upper = operand_at(w_base, rows + ks * 32), lower = operand_at(w_base, rows + kTileBytes + ks * 32);
                         umma_f16(d, x, upper, kNarrow, 1u);
                         umma_f16(d, x + 16, upper, kNarrow, 1u);
                         umma_f16(d, x, lower, kNarrow, 1u);
@@ -747,10 +784,10 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             if (elect_one()) {
 #pragma unroll
                 for (int ks = 0; ks < kBlock / 16; ++ks) {
-                    const uint32_t u = tmem_base + kUpdateColumn + (ks >> 1) * 32 + (ks & 1) * 8;
-                    const uint64_t b = operand(qk_base + kBlock * 128 + ks * 2048, kTileBytes);  // k, dims across
-                    umma_f16(tmem_base + kStateColumn, u, b, kWide | kTransposeB, 1u);
-                    umma_f16(tmem_base + kStateColumn, u + 16, b, kWide | kTransposeB, 1u);
+                    const uint32_t u = kUpdateColumn + (ks >> 1) * 32 + (ks & 1) * 8;
+                    const uint64_t b = operand_at(k_across + qk_offset, ks * 2048);
+                    umma_f16(kStateColumn, u, b, kWide | kTransposeB, 1u);
+                    umma_f16(kStateColumn, u + 16, b, kWide | kTransposeB, 1u);
                 }
                 umma_commit(&sm.s_done);
                 umma_commit(&sm.qk_empty[n & 1]);
@@ -765,7 +802,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
         const int quarter = warp & 3;
         const int group = warp >> 2;
         const int row = quarter * 32 + lane;
-        const uint32_t tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16);
+        const uint32_t tmem = static_cast<uint32_t>(quarter * 32) << 16;
         const uint32_t held = tmem + kStateColumn + group * 64;                // 64 key dims of the row
         const uint32_t upper = tmem + kSplitColumn + group * 32, lower = upper + 64;
         const uint32_t x_at = tmem + kKeyColumn + group * 32, u_at = tmem + kUpdateColumn + group * 32;
@@ -823,7 +860,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             }
             // the state decays while U' is made
             const float end = decay[kBlock - 1];
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < 2; ++c) {
                 load_columns(held + 32 * c, x);
 #pragma unroll
@@ -851,7 +888,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             }
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             if (n + 1 < blocks) {
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < 2; ++c) {
                     load_columns(held + 32 * c, x);
                     tmem_store_split(upper + 16 * c, lower + 16 * c, x);
@@ -880,7 +917,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
         const int quarter = warp & 3;
         const int group = (warp - kChainWarps) >> 2;
         const int row = quarter * 32 + lane;     // value dim
-        const uint32_t tmem = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + group * 32;
+        const uint32_t tmem = (static_cast<uint32_t>(quarter * 32) << 16) + group * 32;
         const int piece = lane & 15;             // later: value dims 4 piece .. + 3 and 64 + 4 piece .. + 3 of a token
         float gain[8] = {};
         if (norm.gate != nullptr) {
@@ -895,18 +932,6 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
         }
         for (; n < blocks; ++n) {
             const uint32_t parity = n & 1;
-            // the gates of this block's rows, ahead
-            uint2 gates[4][2] = {};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int token = n * kBlock + (warp - kChainWarps) * 8 + 2 * i + (lane >> 4);
-                if (norm.gate != nullptr && token < span.length) {
-                    const __nv_bfloat16* from =
-                        norm.gate + (static_cast<size_t>(span.begin) + token) * norm.gate_stride + head * kDim + 4 * piece;
-                    gates[i][0] = *reinterpret_cast<const uint2*>(from);
-                    gates[i][1] = *reinterpret_cast<const uint2*>(from + 64);
-                }
-            }
             ok = wait(&sm.w_full[n & 1], (n >> 1) & 1, failed, status) && wait(&sm.o_done, parity, failed, status);
             if (!ok) {
                 break;
@@ -944,12 +969,14 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             if (lane == 0) {
                 mbar_arrive(&sm.rows_ready);
             }
-            ok = wait(&sm.rows_ready, parity, failed, status);
+            ok = wait(&sm.rows_ready, parity, failed, status) &&
+                 (norm.gate == nullptr || wait(&sm.gate_full[n & 1], (n >> 1) & 1, failed, status));
             if (!ok) {
                 break;
             }
-            // rows of the batch: eight tokens of this warp, two at a time
-#pragma unroll
+            // rows of the batch: eight tokens of this warp, two at a time (not all unrolled: the warps' code has to fit
+            // the instruction cache together)
+#pragma unroll 2
             for (int i = 0; i < 4; ++i) {
                 const int t = (warp - kChainWarps) * 8 + 2 * i + (lane >> 4);
                 const int token = n * kBlock + t;
@@ -967,7 +994,9 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                         sum += __shfl_xor_sync(0xffffffffu, sum, offset);
                     }
                     const float inverse = rsqrtf(sum / static_cast<float>(kDim) + norm.epsilon);
-                    const uint32_t words[4] = {gates[i][0].x, gates[i][0].y, gates[i][1].x, gates[i][1].y};
+                    const uint2 gate_lo = *reinterpret_cast<const uint2*>(sm.gate[n & 1] + t * (kDim * 2) + 8 * piece);
+                    const uint2 gate_hi = *reinterpret_cast<const uint2*>(sm.gate[n & 1] + t * (kDim * 2) + kDim + 8 * piece);
+                    const uint32_t words[4] = {gate_lo.x, gate_lo.y, gate_hi.x, gate_hi.y};
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float z = __uint_as_float((j & 1) != 0 ? words[j >> 1] & 0xffff0000u : words[j >> 1] << 16);
@@ -989,6 +1018,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             __syncwarp();
             if (lane == 0) {
                 mbar_arrive(&sm.rows_free);
+                mbar_arrive(&sm.gate_empty[n & 1]);
             }
         }
     }
@@ -1007,7 +1037,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 arrived(&sm.w_full[i & 1], (i >> 1) & 1);
             }
         } else if (warp == kMmaWarp) {
-            arrived(&sm.v_empty[n & 1], (n >> 1) & 1);
+            arrived(&sm.v_empty, n & 1);
             arrived(&sm.o_done, n & 1);
             arrived(&sm.s_done, n & 1);
         }
@@ -1015,7 +1045,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
         // the state's eight bits: 64 of a row
         const int quarter = warp & 3, group = warp >> 2;
         const int row = quarter * 32 + lane;
-        const uint32_t held = tmem_base + (static_cast<uint32_t>(quarter * 32) << 16) + kStateColumn + group * 64;
+        const uint32_t held = (static_cast<uint32_t>(quarter * 32) << 16) + kStateColumn + group * 64;
         const size_t state_row = (static_cast<size_t>(slot) * v_heads + head) * kDim + row;
         const float peak = fmaxf(sm.peak[0][row], sm.peak[1][row]);
         const float inverse = peak == 0.0f ? 0.0f : __fdiv_rn(127.0f, peak);
@@ -1041,7 +1071,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == kLoadWarp) {
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemColumns) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(0), "r"(kTmemColumns) : "memory");
     }
 }
 
