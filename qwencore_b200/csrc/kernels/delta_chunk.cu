@@ -976,7 +976,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             }
             // rows of the batch: eight tokens of this warp, two at a time (not all unrolled: the warps' code has to fit
             // the instruction cache together)
-#pragma unroll 2
+#pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int t = (warp - kChainWarps) * 8 + 2 * i + (lane >> 4);
                 const int token = n * kBlock + t;
