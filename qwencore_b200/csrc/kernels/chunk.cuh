@@ -21,6 +21,22 @@ __device__ __forceinline__ ChunkSpan chunk_span(const uint32_t* begins, int sequ
     return {static_cast<int>(first), end > first ? static_cast<int>(end - first) : 0};
 }
 
+// 2^x and 1 / x of the unit for special functions, to 2^-22 of themselves, without the instructions that would save results
+// below 2^-126.
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float reciprocal_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ float sigmoid_fast(float x) { return reciprocal_fast(1.0f + exp2_fast(x * -1.4426950408889634f)); }
+
 // Every chunk is cut into tiles of `tile_tokens` from its own first row; tile numbers run through the chunks in order.
 // For a converged warp: which chunk tile `tile` lies in (-1: there is no such tile), and its number inside it.
 struct ChunkTile {

@@ -264,12 +264,6 @@ __device__ __forceinline__ void tmem_store32(uint32_t taddr, const uint32_t (&r)
 
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Largest of three; a NaN counts as nothing.
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float d;
@@ -1141,8 +1135,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         for (int j = 0; j < 4; ++j) {
                             float lo = value[8 * i + 2 * j] * v_scale, hi = value[8 * i + 2 * j + 1] * v_scale;
                             if (gated) {
-                                lo = __fdividef(lo, 1.0f + exp2_fast(__uint_as_float(gate_words[j] << 16) * -kLog2e));
-                                hi = __fdividef(hi, 1.0f + exp2_fast(__uint_as_float(gate_words[j] & 0xffff0000u) * -kLog2e));
+                                lo *= sigmoid_fast(__uint_as_float(gate_words[j] << 16));
+                                hi *= sigmoid_fast(__uint_as_float(gate_words[j] & 0xffff0000u));
                             }
                             const __nv_bfloat162 both = __floats2bfloat162_rn(lo, hi);
                             words[j] = *reinterpret_cast<const uint32_t*>(&both);
@@ -1285,8 +1279,8 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const __g
     for (int j = 0; j < 4; ++j) {
         float lo = acc[2 * j] * inverse, hi = acc[2 * j + 1] * inverse;
         if (p.gate != nullptr) {
-            lo *= 1.0f / (1.0f + __expf(-__uint_as_float(gate_words[j] << 16)));
-            hi *= 1.0f / (1.0f + __expf(-__uint_as_float(gate_words[j] & 0xffff0000u)));
+            lo *= sigmoid_fast(__uint_as_float(gate_words[j] << 16));
+            hi *= sigmoid_fast(__uint_as_float(gate_words[j] & 0xffff0000u));
         }
         const __nv_bfloat162 both = __floats2bfloat162_rn(lo, hi);
         words[j] = *reinterpret_cast<const uint32_t*>(&both);

@@ -177,12 +177,6 @@ struct FactorSmem {
 };
 static_assert(offsetof(FactorSmem, a) % 1024 == 0, "an operand's alignment");
 
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // x += a * rows[0 .. 3][8 columns] for four steps of the sum.
 __device__ __forceinline__ void multiply4(float (&x)[8], const float4& a, const float* rows) {
     const float factors[4] = {a.x, a.y, a.z, a.w};
@@ -1000,7 +994,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float z = __uint_as_float((j & 1) != 0 ? words[j >> 1] & 0xffff0000u : words[j >> 1] << 16);
-                        o[j] *= inverse * gain[j] * __fdividef(z, 1.0f + __expf(-z));
+                        o[j] *= inverse * gain[j] * (z * sigmoid_fast(z));
                     }
                 }
                 uint32_t words[4];

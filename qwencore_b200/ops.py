@@ -310,7 +310,7 @@ def _check_here(*tensors) -> None:
     """The launch goes to the current device: every tensor has to be there."""
     device = torch.cuda.current_device()
     for tensor in tensors:
-        assert tensor is None or (tensor.is_cuda and tensor.device.index == device and tensor.is_contiguous())
+        assert tensor is None or (tensor.get_device() == device and tensor.is_contiguous())
 
 
 def copy_table(tensors, units: int) -> np.ndarray:
