@@ -156,26 +156,32 @@ __device__ __forceinline__ void load_columns(uint32_t taddr, float (&x)[32]) {
 // ---- W of every block and head ------------------------------------------------------------------------
 //
 // [Q ; K] K^T on the tensor cores gives P and A (a thread has a row), fp32 arithmetic the inverse: columns of the four 16 x 16
-// blocks on the diagonal by substitution, then T_10 = -T_11 A_10 T_00 for blocks of 16 and of 32.  W is a product again,
-// [P ; diag(g_end / g)] times T.
+// blocks on the diagonal by substitution, then T_10 = -T_11 A_10 T_00 for blocks of 16 and of 32.  P T is a product on the tensor
+// cores again.  Bound by the latencies of these steps: what counts is how many CTAs an SM holds.
 
 constexpr int kFactorThreads = 128;
 constexpr int kPitch = 68;  // floats of a row of the matrices in shared memory: rows begin in different banks
 
 struct FactorSmem {
-    uint8_t operand[kQkBytes];            // q and k, then [P ; diag] in two parts
-    float t[kBlock * kPitch];             // (1 + A)^-1
     union {
-        float a[kBlock * kPitch];         // A, below the diagonal
-        uint8_t product[kProductBytes];   // T in two parts
+        uint8_t qk[kQkBytes];
+        struct {
+            uint8_t p[kProductBytes];             // [upper, lower][row][128 bytes]
+            union {
+                float a[kBlock * kPitch];         // A, below the diagonal
+                uint8_t product[kProductBytes];   // T diag(beta) in two parts
+            };
+        } m;
     };
-    float2 log[kBlock];                   // log2 of the decay from the start: a whole number and the rest
+    float t[kBlock * kPitch];                     // (1 + A)^-1
+    float2 log[kBlock];                           // log2 of the decay from the start: a whole number and the rest
     float beta[kBlock];
     uint64_t done;
     uint32_t tmem_base;
     int failed;
 };
-static_assert(offsetof(FactorSmem, a) % 1024 == 0, "an operand's alignment");
+static_assert(offsetof(FactorSmem, m.product) % 1024 == 0, "an operand's alignment");
+static_assert(4 * (sizeof(FactorSmem) + 2048) <= 233472, "four CTAs per SM");
 
 // x += a * rows[0 .. 3][8 columns] for four steps of the sum.
 __device__ __forceinline__ void multiply4(float (&x)[8], const float4& a, const float* rows) {
@@ -235,7 +241,7 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
             const __nv_bfloat16* from =
                 qkv + (row0 + (token < count ? token : 0)) * channels + ((row < kBlock ? 0 : kDeltaKeyHeads) + key_head) * kDim + 8 * piece;
             asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                             smem_u32(sm.operand + (piece >> 3) * kTileBytes + swizzled(row, piece & 7))),
+                             smem_u32(sm.qk + (piece >> 3) * kTileBytes + swizzled(row, piece & 7))),
                          "l"(from), "r"(token < count ? 16 : 0)
                          : "memory");
         }
@@ -282,7 +288,7 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
     if (here) {
         if (warp == 0) {
             if (elect_one()) {
-                const uint32_t base = operand_base(smem_u32(sm.operand), 16);
+                const uint32_t base = operand_base(smem_u32(sm.qk), 16);
 #pragma unroll
                 for (int ks = 0; ks < kDim / 16; ++ks) {
                     const uint32_t at = (ks >> 2) * kTileBytes + (ks & 3) * 32;
@@ -297,7 +303,7 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
             uint4* to = reinterpret_cast<uint4*>(images.qk + (static_cast<size_t>(block) * kDeltaKeyHeads + key_head) * kQkBytes);
 #pragma unroll 4
             for (int i = tid; i < kQkBytes / 16; i += kFactorThreads) {
-                to[i] = reinterpret_cast<const uint4*>(sm.operand)[i];
+                to[i] = reinterpret_cast<const uint4*>(sm.qk)[i];
             }
         }
         ok = wait(&sm.done, 0, &sm.failed, status);
@@ -306,12 +312,12 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
     __syncthreads();  // (the image has been read)
     const int t = tid & (kBlock - 1);
     const bool outputs = tid < kBlock;
+    uint8_t* w = images.w + (static_cast<size_t>(block) * v_heads + head) * kWBytes;
     if (ok) {
         // thread t has row t of Q K^T, thread 64 + t of K K^T: P to its operand, A to shared memory
         const float2 mine = sm.log[t];
         const float strength = outputs ? 1.0f : sm.beta[t];
         const int limit = outputs ? t + 1 : t;
-        const float to_end = exp2_fast((sm.log[kBlock - 1].x - mine.x) + (sm.log[kBlock - 1].y - mine.y));
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
             float x[32];
@@ -331,18 +337,13 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
                 }
             }
             if (outputs) {
-                store_split(sm.operand, kTileBytes, t, 4 * c, x);
+                store_split(sm.m.p, kProductBytes / 2, t, 4 * c, x);
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    *reinterpret_cast<float4*>(&sm.a[t * kPitch + 32 * c + 4 * i]) =
+                    *reinterpret_cast<float4*>(&sm.m.a[t * kPitch + 32 * c + 4 * i]) =
                         make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
                 }
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    x[i] = 32 * c + i == t ? to_end : 0.0f;
-                }
-                store_split(sm.operand, kTileBytes, kBlock + t, 4 * c, x);
             }
         }
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -358,7 +359,7 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
                 float sum = 0.0f;
 #pragma unroll
                 for (int k = 0; k < i; k += 4) {
-                    const float4 a = *reinterpret_cast<const float4*>(&sm.a[(16 * b + i) * kPitch + 16 * b + k]);
+                    const float4 a = *reinterpret_cast<const float4*>(&sm.m.a[(16 * b + i) * kPitch + 16 * b + k]);
                     sum = fmaf(a.x, x[k], sum);
                     sum = k + 1 < i ? fmaf(a.y, x[k + 1 < i ? k + 1 : 0], sum) : sum;
                     sum = k + 2 < i ? fmaf(a.z, x[k + 2 < i ? k + 2 : 0], sum) : sum;
@@ -384,7 +385,7 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
         float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int k = 0; k < 16; k += 4) {
-            multiply4(x, *reinterpret_cast<const float4*>(&sm.a[(base + 16 + r) * kPitch + base + k]), &sm.t[(base + k) * kPitch + column]);
+            multiply4(x, *reinterpret_cast<const float4*>(&sm.m.a[(base + 16 + r) * kPitch + base + k]), &sm.t[(base + k) * kPitch + column]);
         }
         float* at = &sm.t[(base + 16 + r) * kPitch + column];
         if (lane < 16) {
@@ -410,7 +411,7 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
         const int column = 8 * warp;
         float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
         for (int k = column; k < 32; k += 4) {
-            multiply4(x, *reinterpret_cast<const float4*>(&sm.a[(32 + lane) * kPitch + k]), &sm.t[k * kPitch + column]);
+            multiply4(x, *reinterpret_cast<const float4*>(&sm.m.a[(32 + lane) * kPitch + k]), &sm.t[k * kPitch + column]);
         }
         float* at = &sm.t[(32 + lane) * kPitch + column];
         *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
@@ -427,7 +428,7 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
     }
     __syncthreads();
     if (ok) {
-        // T diag(beta) as an operand: half a row per thread
+        // T diag(beta) as an operand, and the lower half of W: half a row per thread
         const int row = tid >> 1, half = tid & 1;
         float x[32];
 #pragma unroll
@@ -439,18 +440,26 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
             x[4 * i + 2] = value.z * strength.z;
             x[4 * i + 3] = value.w * strength.w;
         }
-        store_split(sm.product, kProductBytes / 2, row, 4 * half, x);
+        store_split(sm.m.product, kProductBytes / 2, row, 4 * half, x);
         fence_proxy_async();
+        const float2 mine = sm.log[row], end = sm.log[kBlock - 1];
+        const float to_end = exp2_fast((end.x - mine.x) + (end.y - mine.y));
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+            x[i] *= to_end;
+        }
+        store_split(w, kTileBytes, kBlock + row, 4 * half, x);
     }
     __syncthreads();
     if (ok) {
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
         if (warp == 0) {
             if (elect_one()) {
-                const uint32_t a = operand_base(smem_u32(sm.operand), 16), b = operand_base(smem_u32(sm.product), 16);
+                // (rows 64 .. of this operand are whatever lies behind P: their results are not read)
+                const uint32_t a = operand_base(smem_u32(sm.m.p), 16), b = operand_base(smem_u32(sm.m.product), 16);
 #pragma unroll
                 for (int ks = 0; ks < kBlock / 16; ++ks) {
-                    const uint64_t upper = operand_at(a, ks * 32), lower = operand_at(a, kTileBytes + ks * 32);
+                    const uint64_t upper = operand_at(a, ks * 32), lower = operand_at(a, kProductBytes / 2 + ks * 32);
                     const uint64_t t_upper = operand_at(b, ks * 2048), t_lower = operand_at(b, kProductBytes / 2 + ks * 2048);
                     mma_bf16(tmem_base, upper, t_upper, idesc_of(kBlock) | kTransposeB, ks > 0 ? 1u : 0u);
                     mma_bf16(tmem_base, upper, t_lower, idesc_of(kBlock) | kTransposeB, 1u);
@@ -463,13 +472,12 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
         ok = wait(&sm.done, 1, &sm.failed, status);
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     }
-    if (ok) {
-        uint8_t* w = images.w + (static_cast<size_t>(block) * v_heads + head) * kWBytes;
+    if (ok && outputs) {
 #pragma unroll 1
         for (int c = 0; c < 2; ++c) {
             float x[32];
             load_columns(tmem_row + 32 * c, x);
-            store_split(w, kTileBytes, tid, 4 * c, x);
+            store_split(w, kTileBytes, t, 4 * c, x);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");

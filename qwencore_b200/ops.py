@@ -29,7 +29,7 @@ PACKED_PARTIAL_BYTES = 520  # crates/qwc-cuda/src/paged_attention.rs (max, sum f
 
 
 def _stream() -> int:
-    return torch.cuda.current_stream().cuda_stream
+    return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
 
 
 def _p(tensor) -> int:
