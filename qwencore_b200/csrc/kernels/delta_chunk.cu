@@ -114,6 +114,9 @@ __device__ __forceinline__ void store_split(uint8_t* at, int parts, int row, int
     }
 }
 
+// Until the copies out of shared memory have been written.
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
+
 // Bounded as in the other kernels: 20 ms, then the status word is set and the CTA's waits fail.
 __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* failed, int* status) {
     const long long start = clock64();
@@ -162,26 +165,27 @@ __device__ __forceinline__ void load_columns(uint32_t taddr, float (&x)[32]) {
 constexpr int kFactorThreads = 128;
 constexpr int kPitch = 68;  // floats of a row of the matrices in shared memory: rows begin in different banks
 
+constexpr int kMaxRatio = 3;  // value heads of a key head
+constexpr int kFewBlocks = 12;
+
 struct FactorSmem {
     union {
         uint8_t qk[kQkBytes];
         struct {
             uint8_t p[kProductBytes];             // [upper, lower][row][128 bytes]
             union {
-                float a[kBlock * kPitch];         // A, below the diagonal
+                float t[kBlock * kPitch];         // A below the diagonal; it becomes (1 + A)^-1 where it is
                 uint8_t product[kProductBytes];   // T diag(beta) in two parts
             };
         } m;
     };
-    float t[kBlock * kPitch];                     // (1 + A)^-1
-    float2 log[kBlock];                           // log2 of the decay from the start: a whole number and the rest
-    float beta[kBlock];
+    float2 log[kMaxRatio][kBlock];                // log2 of the decay from the start: a whole number and the rest
+    float beta[kMaxRatio][kBlock];
     uint64_t done;
     uint32_t tmem_base;
     int failed;
 };
 static_assert(offsetof(FactorSmem, m.product) % 1024 == 0, "an operand's alignment");
-static_assert(4 * (sizeof(FactorSmem) + 2048) <= 233472, "four CTAs per SM");
 
 // x += a * rows[0 .. 3][8 columns] for four steps of the sum.
 __device__ __forceinline__ void multiply4(float (&x)[8], const float4& a, const float* rows) {
@@ -198,21 +202,25 @@ __device__ __forceinline__ void multiply4(float (&x)[8], const float4& a, const 
     }
 }
 
-__global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
+// A CTA has a block with `per_cta` value heads of one key head: all of them, or one where CTAs are few (see the launch).
+__global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
     const __nv_bfloat16* __restrict__ qkv, const float* __restrict__ alpha, const float* __restrict__ beta,
-    const uint32_t* __restrict__ begins, const Images images, int tokens, int sequences, int v_heads, int* status) {
+    const uint32_t* __restrict__ begins, const Images images, int tokens, int sequences, int v_heads, int per_cta,
+    int* status) {
     extern __shared__ unsigned char smem_raw[];
     FactorSmem& sm = *reinterpret_cast<FactorSmem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
+    constexpr int kTmemFactor = 2 * kBlock;  // [Q ; K] K^T, P T
     const int tid = threadIdx.x;
     const int lane = tid & 31;
     const int warp = tid >> 5;
-    const int head = blockIdx.x;
-    const int block = blockIdx.y;
     const int ratio = v_heads / kDeltaKeyHeads;
-    const int key_head = head / ratio;
+    const int first_head = blockIdx.x * per_cta;
+    const int key_head = first_head / ratio;
+    const int block = blockIdx.y;
     const int channels = (2 * kDeltaKeyHeads + v_heads) * kDim;
     if (warp == 0) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)), "r"(64)
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
+                     "r"(kTmemFactor)
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -246,15 +254,16 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
                          : "memory");
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
-        if (warp == 0) {
-            // decay from the start: a scan over the tokens, in whole numbers and rests below one
+        if (warp < per_cta) {
+            // decay from the start, a warp for a head: a scan over the tokens, in whole numbers and rests below one
+            const int head = first_head + warp;
             float whole[2], part[2];
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int token = lane + 32 * i;
                 // (beyond 2^-130 fp32 has nothing, and an alpha of 0 takes everything before it away)
                 const float log = token < count ? fmaxf(log2f(alpha[(row0 + token) * v_heads + head]), -130.0f) : 0.0f;
-                sm.beta[token] = token < count ? beta[(row0 + token) * v_heads + head] : 0.0f;
+                sm.beta[warp][token] = token < count ? beta[(row0 + token) * v_heads + head] : 0.0f;
                 whole[i] = rintf(log);
                 part[i] = log - whole[i];
             }
@@ -273,7 +282,7 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
             float* decay = images.decay + (static_cast<size_t>(block) * v_heads + head) * kBlock;
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                sm.log[lane + 32 * i] = make_float2(whole[i], part[i]);
+                sm.log[warp][lane + 32 * i] = make_float2(whole[i], part[i]);
                 decay[lane + 32 * i] = exp2f(whole[i] + part[i]);
             }
         }
@@ -298,59 +307,59 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
             }
             __syncwarp();
         }
-        if (head == key_head * ratio) {
-            // the image of q and k, by the key head's first value head
-            uint4* to = reinterpret_cast<uint4*>(images.qk + (static_cast<size_t>(block) * kDeltaKeyHeads + key_head) * kQkBytes);
-#pragma unroll 4
-            for (int i = tid; i < kQkBytes / 16; i += kFactorThreads) {
-                to[i] = reinterpret_cast<const uint4*>(sm.qk)[i];
-            }
+        if (tid == 0 && first_head == key_head * ratio) {
+            // the image of q and k, once for the key head
+            bulk_s2g(images.qk + (static_cast<size_t>(block) * kDeltaKeyHeads + key_head) * kQkBytes, sm.qk, kQkBytes);
+            bulk_commit();
         }
         ok = wait(&sm.done, 0, &sm.failed, status);
     }
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    __syncthreads();  // (the image has been read)
     const int t = tid & (kBlock - 1);
     const bool outputs = tid < kBlock;
-    uint8_t* w = images.w + (static_cast<size_t>(block) * v_heads + head) * kWBytes;
-    if (ok) {
-        // thread t has row t of Q K^T, thread 64 + t of K K^T: P to its operand, A to shared memory
-        const float2 mine = sm.log[t];
-        const float strength = outputs ? 1.0f : sm.beta[t];
-        const int limit = outputs ? t + 1 : t;
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-            float x[32];
-            if (32 * c <= (t | 31)) {  // (the same for a warp)
-                load_columns(tmem_row + 32 * c, x);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    const int j = 32 * c + i;
-                    const float2 other = sm.log[j];
-                    const float decay = exp2_fast((mine.x - other.x) + (mine.y - other.y));
-                    x[i] = j < limit ? strength * decay * x[i] : 0.0f;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    x[i] = 0.0f;
-                }
-            }
-            if (outputs) {
-                store_split(sm.m.p, kProductBytes / 2, t, 4 * c, x);
-            } else {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    *reinterpret_cast<float4*>(&sm.m.a[t * kPitch + 32 * c + 4 * i]) =
-                        make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
-                }
-            }
+    for (int h = 0; h < per_cta; ++h) {
+        if (tid == 0) {
+            bulk_wait_all_read();  // (what has been copied from shared memory)
         }
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    }
-    __syncthreads();
-    if (ok) {
-        if (outputs) {
+        __syncthreads();
+        if (ok) {
+            // thread t has row t of Q K^T, thread 64 + t of K K^T: P to its operand, A to shared memory
+            const float2 mine = sm.log[h][t];
+            const float strength = outputs ? 1.0f : sm.beta[h][t];
+            const int limit = outputs ? t + 1 : t;
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+                float x[32];
+                if (32 * c <= (t | 31)) {  // (the same for a warp)
+                    load_columns(tmem_row + 32 * c, x);
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        const int j = 32 * c + i;
+                        const float2 other = sm.log[h][j];
+                        const float decay = exp2_fast((mine.x - other.x) + (mine.y - other.y));
+                        x[i] = j < limit ? strength * decay * x[i] : 0.0f;
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) {
+                        x[i] = 0.0f;
+                    }
+                }
+                if (outputs) {
+                    store_split(sm.m.p, kProductBytes / 2, t, 4 * c, x);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        *reinterpret_cast<float4*>(&sm.m.t[t * kPitch + 32 * c + 4 * i]) =
+                            make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]);
+                    }
+                }
+            }
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+        }
+        __syncthreads();
+        if (ok && outputs) {
             // blocks of 16 on the diagonal: a column per thread
             const int b = tid >> 4, j = tid & 15;
             float x[16];
@@ -359,131 +368,160 @@ __global__ void __launch_bounds__(kFactorThreads) delta_factor_kernel(
                 float sum = 0.0f;
 #pragma unroll
                 for (int k = 0; k < i; k += 4) {
-                    const float4 a = *reinterpret_cast<const float4*>(&sm.m.a[(16 * b + i) * kPitch + 16 * b + k]);
+                    const float4 a = *reinterpret_cast<const float4*>(&sm.m.t[(16 * b + i) * kPitch + 16 * b + k]);
                     sum = fmaf(a.x, x[k], sum);
                     sum = k + 1 < i ? fmaf(a.y, x[k + 1 < i ? k + 1 : 0], sum) : sum;
                     sum = k + 2 < i ? fmaf(a.z, x[k + 2 < i ? k + 2 : 0], sum) : sum;
                     sum = k + 3 < i ? fmaf(a.w, x[k + 3 < i ? k + 3 : 0], sum) : sum;
                 }
                 x[i] = i == j ? 1.0f : i < j ? 0.0f : -sum;
-                sm.t[(16 * b + i) * kPitch + 16 * b + j] = x[i];
-            }
-        } else {
-            // zeros above the diagonal, in blocks of 16
-            const int b = t >> 4;
-            for (int j = 16 * (b + 1); j < kBlock; j += 4) {
-                *reinterpret_cast<float4*>(&sm.t[t * kPitch + j]) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            }
-        }
-    }
-    __syncthreads();
-    if (ok) {
-        // blocks of 32: T_10 = -T_11 (A_10 T_00) of 16, eight columns per thread of one row of 32
-        const int pair = tid >> 5;  // two threads' columns of two blocks: pair & 1 the columns' half, pair >> 1 the block
-        const int base = 32 * (pair >> 1), column = base + 8 * (pair & 1);
-        const int r = lane & 15;    // (lanes 16-31 do the same again)
-        float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int k = 0; k < 16; k += 4) {
-            multiply4(x, *reinterpret_cast<const float4*>(&sm.m.a[(base + 16 + r) * kPitch + base + k]), &sm.t[(base + k) * kPitch + column]);
-        }
-        float* at = &sm.t[(base + 16 + r) * kPitch + column];
-        if (lane < 16) {
-            *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
-            *reinterpret_cast<float4*>(at + 4) = make_float4(x[4], x[5], x[6], x[7]);
-        }
-        __syncwarp();
-        float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int k = 0; k < 16; k += 4) {
-            multiply4(y, *reinterpret_cast<const float4*>(&sm.t[(base + 16 + r) * kPitch + base + 16 + k]),
-                      &sm.t[(base + 16 + k) * kPitch + column]);
-        }
-        __syncwarp();
-        if (lane < 16) {
-            *reinterpret_cast<float4*>(at) = make_float4(-y[0], -y[1], -y[2], -y[3]);
-            *reinterpret_cast<float4*>(at + 4) = make_float4(-y[4], -y[5], -y[6], -y[7]);
-        }
-    }
-    __syncthreads();
-    if (ok) {
-        // the block of 32 below: a row per lane, eight columns per warp (T_00 is zero above its diagonal)
-        const int column = 8 * warp;
-        float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-        for (int k = column; k < 32; k += 4) {
-            multiply4(x, *reinterpret_cast<const float4*>(&sm.m.a[(32 + lane) * kPitch + k]), &sm.t[k * kPitch + column]);
-        }
-        float* at = &sm.t[(32 + lane) * kPitch + column];
-        *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
-        *reinterpret_cast<float4*>(at + 4) = make_float4(x[4], x[5], x[6], x[7]);
-        __syncwarp();
-        float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 2
-        for (int k = 0; k < 32; k += 4) {
-            multiply4(y, *reinterpret_cast<const float4*>(&sm.t[(32 + lane) * kPitch + 32 + k]), &sm.t[(32 + k) * kPitch + column]);
-        }
-        __syncwarp();
-        *reinterpret_cast<float4*>(at) = make_float4(-y[0], -y[1], -y[2], -y[3]);
-        *reinterpret_cast<float4*>(at + 4) = make_float4(-y[4], -y[5], -y[6], -y[7]);
-    }
-    __syncthreads();
-    if (ok) {
-        // T diag(beta) as an operand, and the lower half of W: half a row per thread
-        const int row = tid >> 1, half = tid & 1;
-        float x[32];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float4 value = *reinterpret_cast<const float4*>(&sm.t[row * kPitch + 32 * half + 4 * i]);
-            const float4 strength = *reinterpret_cast<const float4*>(&sm.beta[32 * half + 4 * i]);
-            x[4 * i] = value.x * strength.x;
-            x[4 * i + 1] = value.y * strength.y;
-            x[4 * i + 2] = value.z * strength.z;
-            x[4 * i + 3] = value.w * strength.w;
-        }
-        store_split(sm.m.product, kProductBytes / 2, row, 4 * half, x);
-        fence_proxy_async();
-        const float2 mine = sm.log[row], end = sm.log[kBlock - 1];
-        const float to_end = exp2_fast((end.x - mine.x) + (end.y - mine.y));
-#pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            x[i] *= to_end;
-        }
-        store_split(w, kTileBytes, kBlock + row, 4 * half, x);
-    }
-    __syncthreads();
-    if (ok) {
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        if (warp == 0) {
-            if (elect_one()) {
-                // (rows 64 .. of this operand are whatever lies behind P: their results are not read)
-                const uint32_t a = operand_base(smem_u32(sm.m.p), 16), b = operand_base(smem_u32(sm.m.product), 16);
-#pragma unroll
-                for (int ks = 0; ks < kBlock / 16; ++ks) {
-                    const uint64_t upper = operand_at(a, ks * 32), lower = operand_at(a, kProductBytes / 2 + ks * 32);
-                    const uint64_t t_upper = operand_at(b, ks * 2048), t_lower = operand_at(b, kProductBytes / 2 + ks * 2048);
-                    mma_bf16(tmem_base, upper, t_upper, idesc_of(kBlock) | kTransposeB, ks > 0 ? 1u : 0u);
-                    mma_bf16(tmem_base, upper, t_lower, idesc_of(kBlock) | kTransposeB, 1u);
-                    mma_bf16(tmem_base, lower, t_upper, idesc_of(kBlock) | kTransposeB, 1u);
-                }
-                umma_commit(&sm.done);
             }
             __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                sm.m.t[(16 * b + i) * kPitch + 16 * b + j] = x[i];
+            }
         }
-        ok = wait(&sm.done, 1, &sm.failed, status);
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    }
-    if (ok && outputs) {
+        __syncthreads();
+        // blocks of 32: T_10 = -T_11 (A_10 T_00) of 16, eight columns per warp, a row per lane (lanes 16-31 do the same again)
+        {
+            const int base = 32 * (warp >> 1), column = base + 8 * (warp & 1);
+            const int r = lane & 15;
+            float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            if (ok) {
+#pragma unroll
+                for (int k = 0; k < 16; k += 4) {
+                    multiply4(x, *reinterpret_cast<const float4*>(&sm.m.t[(base + 16 + r) * kPitch + base + k]),
+                              &sm.m.t[(base + k) * kPitch + column]);
+                }
+            }
+            __syncthreads();  // (A_10 has been read)
+            if (ok) {
+                float* at = &sm.m.t[(base + 16 + r) * kPitch + column];
+                if (lane < 16) {
+                    *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
+                    *reinterpret_cast<float4*>(at + 4) = make_float4(x[4], x[5], x[6], x[7]);
+                }
+                __syncwarp();
+                float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int k = 0; k < 16; k += 4) {
+                    multiply4(y, *reinterpret_cast<const float4*>(&sm.m.t[(base + 16 + r) * kPitch + base + 16 + k]),
+                              &sm.m.t[(base + 16 + k) * kPitch + column]);
+                }
+                __syncwarp();
+                if (lane < 16) {
+                    *reinterpret_cast<float4*>(at) = make_float4(-y[0], -y[1], -y[2], -y[3]);
+                    *reinterpret_cast<float4*>(at + 4) = make_float4(-y[4], -y[5], -y[6], -y[7]);
+                }
+            }
+        }
+        __syncthreads();
+        // the block of 32 below: a row per lane, eight columns per warp (T_00 is zero above its diagonal)
+        {
+            const int column = 8 * warp;
+            float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            if (ok) {
+                for (int k = column; k < 32; k += 4) {
+                    multiply4(x, *reinterpret_cast<const float4*>(&sm.m.t[(32 + lane) * kPitch + k]), &sm.m.t[k * kPitch + column]);
+                }
+            }
+            __syncthreads();  // (A_10 has been read)
+            if (ok) {
+                float* at = &sm.m.t[(32 + lane) * kPitch + column];
+                *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
+                *reinterpret_cast<float4*>(at + 4) = make_float4(x[4], x[5], x[6], x[7]);
+                __syncwarp();
+                float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+                for (int k = 0; k < 32; k += 4) {
+                    multiply4(y, *reinterpret_cast<const float4*>(&sm.m.t[(32 + lane) * kPitch + 32 + k]),
+                              &sm.m.t[(32 + k) * kPitch + column]);
+                }
+                __syncwarp();
+                *reinterpret_cast<float4*>(at) = make_float4(-y[0], -y[1], -y[2], -y[3]);
+                *reinterpret_cast<float4*>(at + 4) = make_float4(-y[4], -y[5], -y[6], -y[7]);
+            }
+        }
+        __syncthreads();
+        // T diag(beta) as an operand: half a row per thread
+        const int row = tid >> 1, half = tid & 1;
+        float x[32];
+        if (ok) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float4 value = *reinterpret_cast<const float4*>(&sm.m.t[row * kPitch + 32 * half + 4 * i]);
+                const float4 strength = *reinterpret_cast<const float4*>(&sm.beta[h][32 * half + 4 * i]);
+                x[4 * i] = value.x * strength.x;
+                x[4 * i + 1] = value.y * strength.y;
+                x[4 * i + 2] = value.z * strength.z;
+                x[4 * i + 3] = value.w * strength.w;
+            }
+        }
+        __syncthreads();  // (T has been read)
+        if (ok) {
+            store_split(sm.m.product, kProductBytes / 2, row, 4 * half, x);
+            fence_proxy_async();
+        }
+        __syncthreads();
+        if (ok) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (warp == 0) {
+                if (elect_one()) {
+                    // (rows 64 .. of this operand are whatever lies behind P: their results are not read)
+                    const uint32_t a = operand_base(smem_u32(sm.m.p), 16), b = operand_base(smem_u32(sm.m.product), 16);
+#pragma unroll
+                    for (int ks = 0; ks < kBlock / 16; ++ks) {
+                        const uint64_t upper = operand_at(a, ks * 32), lower = operand_at(a, kProductBytes / 2 + ks * 32);
+                        const uint64_t t_upper = operand_at(b, ks * 2048), t_lower = operand_at(b, kProductBytes / 2 + ks * 2048);
+                        mma_bf16(tmem_base + kBlock, upper, t_upper, idesc_of(kBlock) | kTransposeB, ks > 0 ? 1u : 0u);
+                        mma_bf16(tmem_base + kBlock, upper, t_lower, idesc_of(kBlock) | kTransposeB, 1u);
+                        mma_bf16(tmem_base + kBlock, lower, t_upper, idesc_of(kBlock) | kTransposeB, 1u);
+                    }
+                    umma_commit(&sm.done);
+                }
+                __syncwarp();
+            }
+            const float2 mine = sm.log[h][row], end = sm.log[h][kBlock - 1];
+            const float to_end = exp2_fast((end.x - mine.x) + (end.y - mine.y));
+#pragma unroll
+            for (int i = 0; i < 32; ++i) {
+                x[i] *= to_end;
+            }
+            ok = wait(&sm.done, (h + 1) & 1, &sm.failed, status);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        }
+        if (ok) {
+            // W's halves where the operands were, and from there to memory in one piece each
+            store_split(sm.m.product, kProductBytes / 2, row, 4 * half, x);
+            if (outputs) {
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
-            float x[32];
-            load_columns(tmem_row + 32 * c, x);
-            store_split(w, kTileBytes, t, 4 * c, x);
+                for (int c = 0; c < 2; ++c) {
+                    load_columns(tmem_row + kBlock + 32 * c, x);
+                    store_split(sm.m.p, kProductBytes / 2, t, 4 * c, x);
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            }
+            fence_proxy_async();
         }
+        __syncthreads();
+        if (ok && tid == 0) {
+            uint8_t* w = images.w + (static_cast<size_t>(block) * v_heads + first_head + h) * kWBytes;
+#pragma unroll
+            for (int part = 0; part < 2; ++part) {
+                bulk_s2g(w + part * kTileBytes, sm.m.p + part * (kProductBytes / 2), kProductBytes / 2);
+                bulk_s2g(w + part * kTileBytes + kTileBytes / 2, sm.m.product + part * (kProductBytes / 2), kProductBytes / 2);
+            }
+            bulk_commit();
+        }
+    }
+    if (tid == 0) {
+        bulk_wait_all();
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if (warp == 0) {
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(64) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(kTmemFactor) : "memory");
     }
 }
 
@@ -1133,10 +1171,11 @@ extern "C" int qwc_delta_chunk_int8(void* state, float* state_scales, const void
     }
     const int blocks = most_chunk_tiles(tokens, sequences, kBlock);
     const Images images = images_at(workspace, blocks, v_heads);
+    const int per_cta = blocks < kFewBlocks ? 1 : v_heads / kDeltaKeyHeads;
     const cudaError_t launched = launch_chained(
-        delta_factor_kernel, dim3(v_heads, blocks), dim3(kFactorThreads), sizeof(FactorSmem) + 1024, stream,
+        delta_factor_kernel, dim3(v_heads / per_cta, blocks), dim3(kFactorThreads), sizeof(FactorSmem) + 1024, stream,
         static_cast<const __nv_bfloat16*>(qkv), static_cast<const float*>(alpha), static_cast<const float*>(beta),
-        static_cast<const uint32_t*>(chunk_begins), images, tokens, sequences, v_heads, status);
+        static_cast<const uint32_t*>(chunk_begins), images, tokens, sequences, v_heads, per_cta, status);
     if (launched != cudaSuccess) {
         return launched;
     }
