@@ -477,13 +477,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     const int pair = blockIdx.x >> 1;
     const int pairs = gridDim.x >> 1;
 
-    if (warp == kMmaWarp) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
-                     "r"(kTmemColumns)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    }
     if (threadIdx.x == kFetchWarp * 32) {
         for (int i = 0; i < kKeyStages; ++i) {
             mbar_init(&sm.raw_k_full[i], 1);
@@ -522,10 +515,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     fence_proxy_async();
     __syncthreads();
     pair_sync();  // (the other CTA's shared memory is there)
-    // (Not before this CTA has its tensor memory: a CTA of the next kernel that took some of it first would wait for this
-    // kernel's end, and this CTA for that one's.)
-    pdl_launch_dependents();
     pdl_wait();
+    // Tensor memory is asked for when the kernels before this one have given theirs back, and the next kernel may start
+    // when this CTA has its own: CTAs of two kernels that each held some and asked for the rest would wait for each other.
+    if (warp == kMmaWarp) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
+                     "r"(kTmemColumns)
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
     if (rank == 0 && threadIdx.x < 2) {
         // both CTAs of a pair go by what the first one finds in the status word
         const uint32_t stop = status_is_set(p.status) ? 1u : 0u;
@@ -540,6 +539,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     find_start(p, sm, pair, pairs);
     __syncthreads();
+    pdl_launch_dependents();
     pair_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sm.tmem_base);

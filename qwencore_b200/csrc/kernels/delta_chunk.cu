@@ -218,6 +218,14 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
     const int key_head = first_head / ratio;
     const int block = blockIdx.y;
     const int channels = (2 * kDeltaKeyHeads + v_heads) * kDim;
+    if (tid == 0) {
+        mbar_init(&sm.done, 1);
+        sm.failed = 0;
+        mbar_fence_init();
+    }
+    pdl_wait();
+    // Tensor memory is asked for when the kernels before this one have given theirs back, and the next kernel may start
+    // when this CTA has its own: CTAs of two kernels that each held some and asked for the rest would wait for each other.
     if (warp == 0) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
                      "r"(kTmemFactor)
@@ -225,16 +233,6 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     }
-    if (tid == 0) {
-        mbar_init(&sm.done, 1);
-        sm.failed = 0;
-        mbar_fence_init();
-    }
-    __syncthreads();
-    // (Not before this CTA has its tensor memory: a CTA of the next kernel that took some of it first would wait for this
-    // kernel's end, and this CTA for that one's.)
-    pdl_launch_dependents();
-    pdl_wait();
     const ChunkTile tile = find_chunk_tile(begins, sequences, tokens, kBlock, block);
     const bool here = tile.sequence >= 0;
     const int first = tile.index * kBlock;
@@ -290,6 +288,7 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
     }
     fence_proxy_async();
     __syncthreads();
+    pdl_launch_dependents();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sm.tmem_base);
     const uint32_t tmem_row = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
