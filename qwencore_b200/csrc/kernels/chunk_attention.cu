@@ -886,36 +886,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (lane == 0) {
                 mbar_arrive(&sm.scales_ready);
             }
-            // Into L2: the gates that this item ends with, 512 bytes of a row ...
-            if (p.gate != nullptr) {
-                const int r = me * kWarpRows + lane;
-                const int token = first_token + r / kGqaGroup;
-                if (r < kRowTokens * kGqaGroup && token < walk.info.length) {
-                    bulk_prefetch_l2(p.gate + (static_cast<size_t>(walk.info.begin) + token) * p.gate_stride +
-                                         (walk.head * kGqaGroup + r % kGqaGroup) * (2 * kHeadDim) + kHeadDim,
-                                     kHeadDim * 2);
-                }
-                __syncwarp();
-            }
-            {
-                // ... and the next item's queries, 6 heads of a token together
-                ChunkWalk ahead = walk;
-                ChunkPiece next;
-                if (me == 0 && next_piece(ahead, false, p.sequences, info, next)) {
-                    const int token = ahead.tile * kItemTokens + rank * kRowTokens + lane;
-                    if (lane < kRowTokens && token < ahead.info.length) {
-                        bulk_prefetch_l2(p.query + ((static_cast<size_t>(ahead.info.begin) + token) * kQueryHeads +
-                                                    ahead.head * kGqaGroup) * kHeadDim, kGqaGroup * kHeadDim * 2);
-                    }
-                    __syncwarp();
-                }
-            }
             ok = !widened || widen_keys(g);
             for (int unit = piece.unit_begin; ok && unit < piece.unit_end; ++unit, ++g) {
                 if (widened && unit + 1 < piece.unit_end) {
                     ok = widen_keys(g + 1);
                 }
                 ok = ok && widen_values(g);
+                if (unit > piece.unit_begin) {
+                    continue;
+                }
+                // Into L2: the gates that this item ends with, 512 bytes of a row ...
+                if (p.gate != nullptr) {
+                    const int r = me * kWarpRows + lane;
+                    const int token = first_token + r / kGqaGroup;
+                    if (r < kRowTokens * kGqaGroup && token < walk.info.length) {
+                        bulk_prefetch_l2(p.gate + (static_cast<size_t>(walk.info.begin) + token) * p.gate_stride +
+                                             (walk.head * kGqaGroup + r % kGqaGroup) * (2 * kHeadDim) + kHeadDim,
+                                         kHeadDim * 2);
+                    }
+                    __syncwarp();
+                }
+                {
+                    // ... and the next item's queries, 6 heads of a token together
+                    ChunkWalk ahead = walk;
+                    ChunkPiece next;
+                    if (me == 0 && next_piece(ahead, false, p.sequences, info, next)) {
+                        const int token = ahead.tile * kItemTokens + rank * kRowTokens + lane;
+                        if (lane < kRowTokens && token < ahead.info.length) {
+                            bulk_prefetch_l2(p.query + ((static_cast<size_t>(ahead.info.begin) + token) * kQueryHeads +
+                                                        ahead.head * kGqaGroup) * kHeadDim, kGqaGroup * kHeadDim * 2);
+                        }
+                        __syncwarp();
+                    }
+                }
             }
             ++item;
         }
