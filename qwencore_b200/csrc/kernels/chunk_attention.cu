@@ -84,7 +84,8 @@ struct Smem {
     float row_scale[kRows];                   // what the row's query times key has been divided by
     uint32_t inexact[2 * kWidenWarps];        // rows whose digits leave too much, by warp of the pair (first CTA)
     uint32_t mode;                            // what follows from that: queries and keys are widened
-    long long sequence_line[kMaxChunkSequences];
+    ChunkSequence sequence[kMaxChunkSequences];
+    long long sequence_line[kMaxChunkSequences];  // a head's length of line
     ChunkWalk start;
     long long total;
     uint32_t tmem_base;
@@ -378,7 +379,6 @@ __device__ __forceinline__ ChunkSequence sequence_info(const Params& p, int sequ
 __device__ __forceinline__ void find_start(const Params& p, Smem& sm, int pair, int pairs) {
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
-    // a head's length of line for every sequence
     for (int s = warp; s < p.sequences; s += kThreads / 32) {
         const ChunkSequence info = sequence_info(p, s);
         const int tiles = item_tiles(info);
@@ -391,6 +391,7 @@ __device__ __forceinline__ void find_start(const Params& p, Smem& sm, int pair, 
             sum += __shfl_xor_sync(0xffffffffu, sum, offset);
         }
         if (lane == 0) {
+            sm.sequence[s] = info;
             sm.sequence_line[s] = sum;
         }
     }
@@ -432,10 +433,11 @@ __device__ __forceinline__ void find_start(const Params& p, Smem& sm, int pair, 
         carry += __shfl_sync(0xffffffffu, inclusive, 31);
     }
     if (walk.left > 0) {
-        walk.info = sequence_info(p, walk.sequence);
+        walk.info = sm.sequence[walk.sequence];
         const long long head_line = sm.sequence_line[walk.sequence];
-        walk.head = static_cast<int>((begin - carry) / head_line);
-        carry += walk.head * head_line;
+        for (; walk.head < kPlanHeads - 1 && begin >= carry + head_line; ++walk.head) {
+            carry += head_line;
+        }
         // ... and the tile
         const int tiles = item_tiles(walk.info);
         for (int base = 0; base < tiles; base += 32) {
@@ -543,7 +545,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     pair_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sm.tmem_base);
-    const auto info = [&](int sequence) { return sequence_info(p, sequence); };
+    const auto info = [&](int sequence) { return sm.sequence[sequence]; };
     ChunkWalk walk = sm.start;
     if (*reinterpret_cast<volatile int*>(&sm.stop) != 0) {
         walk.left = 0;

@@ -47,22 +47,22 @@ QWC_CHUNK_PLAN_FUNCTION int plan_workers(long long total, int workers) {
     return most >= workers ? workers : most < 1 ? 1 : static_cast<int>(most);
 }
 
-QWC_CHUNK_PLAN_FUNCTION long long share_begin(long long total, int worker, int workers) {
-    return total / workers * worker + total % workers * worker / workers;
+// a / b; of 32 bits where they do (a division of 64 is a few hundred cycles).
+QWC_CHUNK_PLAN_FUNCTION long long plan_divide(long long a, long long b) {
+    if (a <= 0xffffffffll && b <= 0xffffffffll) {
+        return static_cast<uint32_t>(a) / static_cast<uint32_t>(b);
+    }
+    return a / b;
 }
 
-// The worker whose share holds `position` (below total).
+// (A line is below 2^37: 1689 tiles at most of 2^16 tokens, 4 heads, 2^24 units.)
+QWC_CHUNK_PLAN_FUNCTION long long share_begin(long long total, int worker, int workers) {
+    return plan_divide(total * worker, workers);
+}
+
+// The worker whose share holds `position` (below total): the last one with total * worker / workers < position + 1.
 QWC_CHUNK_PLAN_FUNCTION int worker_of(long long total, long long position, int workers) {
-    int low = 0, high = workers - 1;  // the last one that begins at or before it
-    while (low < high) {
-        const int middle = (low + high + 1) >> 1;
-        if (share_begin(total, middle, workers) <= position) {
-            low = middle;
-        } else {
-            high = middle - 1;
-        }
-    }
-    return low;
+    return static_cast<int>(plan_divide((position + 1) * workers - 1, total));
 }
 
 struct ChunkPiece {
