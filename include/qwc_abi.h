@@ -564,7 +564,7 @@ int qwc_delta_prepare_chunk(const void* mixed_qkv, const void* a_projection, con
  * The gated delta rule over chunks, on the slots' int8 state (layout of qwc_delta_decode_int8): per token
  *   S <- alpha S;  u = beta (v - S k);  S <- S + u k^T;  o = S q
  * The state is read from its eight bits at the start of a chunk, carried in fp32, and written back at its end.
- * qkv, alpha, beta: what qwc_delta_prepare_chunk wrote.  out bf16[tokens, heads, 128].  With norm_weight
+ * qkv, alpha (none negative), beta: what qwc_delta_prepare_chunk wrote.  out bf16[tokens, heads, 128].  With norm_weight
  * bf16[128] and gate bf16 rows of gate_stride elements (0 = heads * 128; both or neither NULL), out is
  * rmsnorm(o) * norm_weight * silu(gate) instead.  workspace: qwc_delta_chunk_workspace_bytes(tokens, sequences) bytes;
  * calls that overlap on the device must not share one.  Row pointers, state and workspace 16-byte aligned.

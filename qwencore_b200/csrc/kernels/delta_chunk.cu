@@ -259,8 +259,9 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const int token = lane + 32 * i;
-                // (beyond 2^-130 fp32 has nothing, and an alpha of 0 takes everything before it away)
-                const float log = token < count ? fmaxf(log2f(alpha[(row0 + token) * v_heads + head]), -130.0f) : 0.0f;
+                // (beyond 2^-130 fp32 has nothing, and an alpha of 0 takes everything before it away; a NaN stays one)
+                float log = token < count ? log2f(alpha[(row0 + token) * v_heads + head]) : 0.0f;
+                log = log < -130.0f ? -130.0f : log;
                 sm.beta[warp][token] = token < count ? beta[(row0 + token) * v_heads + head] : 0.0f;
                 whole[i] = rintf(log);
                 part[i] = log - whole[i];

@@ -343,12 +343,15 @@ def paged_attention_chunk(query, query_gate_projection, key_cache, value_cache, 
     assert query.numel() >= tokens * NUM_ATTN_HEADS * ATTN_HEAD_DIM and query.dtype == torch.bfloat16
     assert output.numel() >= tokens * NUM_ATTN_HEADS * ATTN_HEAD_DIM and output.dtype == torch.bfloat16
     assert context_lengths.numel() >= sequences and chunk_begins.numel() > sequences
+    for scales in (key_scales, value_scales):
+        assert scales is None or (scales.numel() >= NUM_KV_HEADS and scales.dtype == torch.float32)
     assert block_tables.numel() >= sequences * max_blocks_per_sequence
     for cache in (key_cache, value_cache):
         assert cache.numel() * cache.element_size() >= num_blocks * NUM_KV_HEADS * page_size * ATTN_HEAD_DIM
     if query_gate_projection is not None:
         stride = gate_stride or NUM_ATTN_HEADS * 2 * ATTN_HEAD_DIM
         assert query_gate_projection.numel() >= (tokens - 1) * stride + NUM_ATTN_HEADS * 2 * ATTN_HEAD_DIM
+        assert query_gate_projection.dtype == torch.bfloat16
     _check_here(query, query_gate_projection, key_cache, value_cache, block_tables, context_lengths, chunk_begins, output,
                 workspace, key_scales, value_scales)
     workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
@@ -373,6 +376,7 @@ def delta_prepare_chunk(mixed, a_offset: int, b_offset: int, conv_weight, a_log,
     assert qkv.numel() >= tokens * channels and alpha.numel() >= tokens * heads and beta.numel() >= tokens * heads
     assert conv_state.numel() >= state_capacity * channels * 3 and conv_weight.numel() >= channels * 4
     assert mixed.dtype == torch.bfloat16 and qkv.dtype == torch.bfloat16 and conv_state.dtype == torch.float32
+    assert alpha.dtype == torch.float32 and beta.dtype == torch.float32 and conv_weight.dtype == torch.bfloat16
     assert state_slots.numel() >= sequences and chunk_begins.numel() > sequences
     assert continues is None or continues.numel() >= sequences
     _check_here(mixed, conv_weight, a_log, dt_bias, conv_state, state_slots, continues, chunk_begins, qkv, alpha, beta)

@@ -79,3 +79,70 @@ def test_cache_copy(abi):
     assert call([good], count=-1) == abi.CUDA_ERROR_INVALID_VALUE
     assert abi.lib.qwc_cache_copy(0, 1, ONE, 1, 0) == abi.CUDA_ERROR_INVALID_VALUE
     assert call([good], count=0) == 0 and call([good], pairs=0, count=0) == 0
+
+
+def test_wrappers_refuse_what_does_not_fit(abi):
+    """Types and sizes are looked at before anything that needs a GPU."""
+    import torch
+
+    from qwencore_b200 import ops
+
+    bf16, f32, i32 = torch.bfloat16, torch.float32, torch.int32
+    zeros = lambda n, dtype: torch.zeros(n, dtype=dtype)  # noqa: E731
+
+    def attention(**other):
+        given = dict(query=zeros(2 * 6144, bf16), query_gate_projection=zeros(2 * 12288, bf16), key_cache=zeros(3 * 16384, torch.uint8),
+                     value_cache=zeros(3 * 16384, torch.uint8), block_tables=zeros(4, i32), context_lengths=zeros(1, i32),
+                     chunk_begins=zeros(2, i32), max_blocks_per_sequence=4, output=zeros(2 * 6144, bf16), tokens=2, sequences=1,
+                     workspace=zeros(16, torch.uint8), page_size=16, num_blocks=3)
+        ops.paged_attention_chunk(**{**given, **other})
+
+    for other in (dict(query=zeros(2 * 6144 - 1, bf16)), dict(query=zeros(2 * 6144, torch.float16)), dict(output=zeros(2 * 6144, f32)),
+                  dict(context_lengths=zeros(0, i32)), dict(chunk_begins=zeros(1, i32)), dict(block_tables=zeros(3, i32)),
+                  dict(num_blocks=4), dict(query_gate_projection=zeros(2 * 12288 - 1, bf16)), dict(gate_stride=20000),
+                  dict(query_gate_projection=zeros(2 * 12288, f32)), dict(key_scales=zeros(3, f32)), dict(value_scales=zeros(4, bf16))):
+        with pytest.raises(AssertionError):
+            attention(**other)
+
+    before = abi.get_shape()
+    abi.configure(32, 64)
+    channels, width = 8192, 8192 + 4096 + 64
+
+    def prepare(**other):
+        given = dict(mixed=zeros(2 * width, bf16), a_offset=width - 64, b_offset=width - 32, conv_weight=zeros(channels * 4, bf16),
+                     a_log=zeros(32, bf16), dt_bias=zeros(32, bf16), conv_state=zeros(2 * channels * 3, f32), state_slots=zeros(1, i32),
+                     continues=None, chunk_begins=zeros(2, i32), qkv=zeros(2 * channels, bf16), alpha=zeros(64, f32),
+                     beta=zeros(64, f32), state_capacity=2, tokens=2, sequences=1, mixed_stride=width)
+        ops.delta_prepare_chunk(**{**given, **other})
+
+    def delta(**other):
+        given = dict(state=zeros(2 * 32 * 16384, torch.int8), state_scales=zeros(2 * 32 * 128, f32), state_slots=zeros(1, i32),
+                     continues=zeros(1, i32), chunk_begins=zeros(2, i32), qkv=zeros(2 * channels, bf16), alpha=zeros(64, f32),
+                     beta=zeros(64, f32), out=zeros(2 * 4096, bf16), state_capacity=2, tokens=2, sequences=1,
+                     workspace=zeros(16, torch.uint8), gate=zeros(2 * 4096, bf16), norm_weight=zeros(128, bf16))
+        ops.delta_chunk(**{**given, **other})
+
+    try:
+        for other in (dict(mixed=zeros(2 * width - 1, bf16)), dict(mixed=zeros(2 * width, f32)), dict(qkv=zeros(2 * channels - 1, bf16)),
+                      dict(alpha=zeros(63, f32)), dict(beta=zeros(64, bf16)), dict(conv_state=zeros(2 * channels * 3, bf16)),
+                      dict(state_capacity=3), dict(chunk_begins=zeros(1, i32)), dict(conv_weight=zeros(channels * 4, f32)),
+                      dict(continues=zeros(0, i32))):
+            with pytest.raises(AssertionError):
+                prepare(**other)
+        for other in (dict(state=zeros(2 * 32 * 16384, torch.uint8)), dict(state_capacity=3), dict(state_scales=zeros(8192, bf16)),
+                      dict(qkv=zeros(2 * channels, f32)), dict(alpha=zeros(63, f32)), dict(out=zeros(2 * 4096, f32)),
+                      dict(out=zeros(4096, bf16)), dict(gate=zeros(2 * 4096, f32)), dict(gate_offset=8), dict(gate_stride=4104),
+                      dict(norm_weight=zeros(127, bf16)), dict(sequences=2)):
+            with pytest.raises(AssertionError):
+                delta(**other)
+    finally:
+        abi.configure(*before)
+
+    with pytest.raises(AssertionError):
+        ops.copy_table([zeros(7, f32)], 2)
+    with pytest.raises(AssertionError):
+        ops.copy_table([zeros((4, 4), f32).T], 2)
+    with pytest.raises(AssertionError):
+        ops.cache_copy(np.zeros((1, 3), dtype=np.int64), zeros(2, i32), 1)
+    with pytest.raises(AssertionError):
+        ops.cache_copy(np.zeros((1, 3), dtype=np.uint64), zeros(2, i32), 2)

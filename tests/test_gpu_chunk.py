@@ -532,3 +532,336 @@ def test_cache_copy_beyond_the_array(cuda, ops):
     abi.check(abi.lib.qwc_device_status_reset(), "reset")
     ops.cache_copy(ops.copy_table([array], 5), i32(cuda, [0, 1]), 0)
     assert cuda.equal(array, want)
+
+
+# ---- as they are used -----------------------------------------------------------------------------
+
+class Layers:
+    """A DeltaNet and an attention layer that take a ragged batch of prompts, share a prefix and go on token by token."""
+
+    def __init__(self, torch, ops, seed, lengths, past, heads, page=16):
+        from qwencore_b200 import abi
+        abi.configure(heads, 64)
+        g = generator(torch, seed)
+        self.torch, self.ops, self.heads, self.page, self.lengths = torch, ops, heads, page, lengths
+        self.sequences = count = len(lengths)
+        self.first, self.tokens = begins_of(lengths), sum(lengths)
+        self.channels = (2 * KEY_HEADS + heads) * DIM
+        self.z = self.channels
+        self.a = self.z + heads * DIM
+        self.b = self.a + heads
+        self.width = self.b + heads + (-(self.b + heads)) % 8
+        randn = lambda *shape: torch.randn(shape, device="cuda", generator=g)  # noqa: E731
+        # rows of the prompts, and of the next token of every sequence and of a copy of the first
+        self.mixed, self.next_mixed = randn(self.tokens, self.width).bfloat16(), randn(count + 1, self.width).bfloat16()
+        self.next_mixed[count] = self.next_mixed[0]
+        self.taps = (randn(self.channels, 4) * 0.5).bfloat16()
+        self.a_log, self.dt_bias = (randn(heads) * 0.5).bfloat16(), (randn(heads) * 0.5).bfloat16()
+        self.weight = (1 + 0.1 * randn(DIM)).bfloat16()
+        self.slots = list(range(count, 0, -1)) + [0]  # the copy's is the last
+        self.capacity = count + 1
+        held = randn(self.capacity, heads, DIM, DIM) * 0.1
+        peak = held.abs().amax(-1)
+        self.codes, self.scales = (held * (127.0 / peak)[..., None]).round().to(torch.int8), peak / 127.0
+        self.history = randn(self.capacity, self.channels, 3).bfloat16().float()
+        self.continues = [int(p > 0) for p in past]
+        # attention: the sequences' pages, with room for a token more, and as many for the copy
+        self.contexts = [n + p for n, p in zip(lengths, past)]
+        blocks = [c // page + 1 for c in self.contexts]
+        self.widest, self.pool = max(blocks), sum(blocks) + blocks[0]
+        order = np.random.default_rng(seed).permutation(self.pool)
+        table = np.zeros((count + 1, self.widest), dtype=np.int32)
+        at = 0
+        for row, blocks_of in enumerate(blocks + [blocks[0]]):
+            table[row, :blocks_of] = order[at:at + blocks_of]
+            at += blocks_of
+        self.table = torch.from_numpy(table).cuda()
+        self.state_pairs = i32(torch, [self.slots[0], 0])
+        self.page_pairs = i32(torch, np.stack([table[0, :blocks[0]], table[count, :blocks[0]]], 1).flatten())
+        self.copied = blocks[0]
+        self.kv_scale = (0.5 + torch.rand(KV, device="cuda", generator=g)) / 32.0
+        self.caches = [(randn(self.pool, KV, page, WIDE) / self.kv_scale[None, :, None, None]).clamp(-448, 448)
+                       .to(torch.float8_e4m3fn).view(torch.uint8) for _ in range(2)]
+        self.row = 2 * HEADS * WIDE + 2 * KV * WIDE  # [q | gate per head][k][v]
+        self.projected, self.next_projected = (randn(n, self.row).bfloat16() for n in (self.tokens, count + 1))
+        self.next_projected[count] = self.next_projected[0]
+        self.q_weight, self.k_weight = (randn(WIDE) * 0.1).bfloat16(), (randn(WIDE) * 0.1).bfloat16()
+        positions = [p + i for n, p in zip(lengths, past) for i in range(n)]
+        self.places = self.place(positions, [s for s, n in enumerate(lengths) for _ in range(n)])
+        self.next_places = self.place(self.contexts + [self.contexts[0]], list(range(count + 1)))
+        # what the calls write
+        bf16 = lambda *shape: torch.zeros(shape, dtype=torch.bfloat16, device="cuda")  # noqa: E731
+        f32 = lambda *shape: torch.zeros(shape, device="cuda")  # noqa: E731
+        self.qkv, self.alpha, self.beta = bf16(self.tokens, self.channels), f32(self.tokens, heads), f32(self.tokens, heads)
+        self.out, self.attended, self.query = bf16(self.tokens, heads, DIM), bf16(self.tokens, HEADS, WIDE), bf16(self.tokens, HEADS, WIDE)
+        n = count + 1
+        self.q, self.k, self.v = f32(n, KEY_HEADS, DIM), f32(n, KEY_HEADS, DIM), f32(n, heads, DIM)
+        self.next_alpha, self.next_beta, self.kq = f32(n, heads), f32(n, heads), f32(n, KEY_HEADS)
+        self.next_values, self.next_out = f32(n, heads, DIM), bf16(n, heads, DIM)
+        self.next_query, self.next_attended = bf16(n, HEADS, WIDE), bf16(n, HEADS, WIDE)
+        self.lists = [i32(torch, x) for x in (self.slots, self.continues, self.first, self.contexts,
+                                              [c + 1 for c in self.contexts] + [self.contexts[0] + 1])]
+        size = lambda n: torch.zeros(max(16, n), dtype=torch.uint8, device="cuda")  # noqa: E731
+        self.workspaces = [size(ops.delta_chunk_workspace_bytes(self.tokens, count)), size(ops.attention_chunk_workspace_bytes()),
+                           size(ops.packed_workspace_bytes(n, 8))]
+        self.tables = [ops.copy_table([self.codes, self.scales, self.history], self.capacity), ops.copy_table(self.caches, self.pool)]
+        self.state = [self.codes, self.scales, self.history, *self.caches]
+        self.before = [x.clone() for x in self.state]
+        self.between = [torch.empty_like(x) for x in self.state]  # behind the prompts and the copies
+        self.results = [self.qkv, self.alpha, self.beta, self.out, self.query, self.attended, self.next_values, self.next_out,
+                        self.next_query, self.next_attended, *self.state]
+
+    def place(self, positions, rows):
+        """cos, sin, page and offset of every row's token."""
+        torch = self.torch
+        at = torch.tensor(positions, dtype=torch.float64, device="cuda")
+        angle = at[:, None] * 10.0 ** (-(torch.arange(64, dtype=torch.float64, device="cuda") % 32) / 8)[None]
+        pages = self.table[torch.tensor(rows, device="cuda"), torch.tensor([p // self.page for p in positions], device="cuda")]
+        return angle.cos().bfloat16(), angle.sin().bfloat16(), pages.contiguous(), i32(torch, [p % self.page for p in positions])
+
+    def restore(self):
+        for held, before in zip(self.state, self.before):
+            held.copy_(before)
+
+    def prompts(self):
+        ops, (slots, continues, first, contexts, _) = self.ops, self.lists
+        ops.delta_prepare_chunk(self.mixed, self.a, self.b, self.taps, self.a_log, self.dt_bias, self.history, slots, continues,
+                                first, self.qkv, self.alpha, self.beta, self.capacity, self.tokens, self.sequences, self.width)
+        ops.delta_chunk(self.codes, self.scales, slots, continues, first, self.qkv, self.alpha, self.beta, self.out, self.capacity,
+                        self.tokens, self.sequences, self.workspaces[0], gate=self.mixed, gate_offset=self.z,
+                        gate_stride=self.width, norm_weight=self.weight, epsilon=EPS)
+        self.attention_rows(self.projected, self.places, self.query, self.tokens)
+        ops.paged_attention_chunk(self.query, self.projected, *self.caches, self.table, contexts, first, self.widest,
+                                  self.attended, self.tokens, self.sequences, self.workspaces[1], self.page, self.pool,
+                                  key_scales=self.kv_scale, value_scales=self.kv_scale, gate_stride=self.row)
+        ops.cache_copy(self.tables[0], self.state_pairs, 1)
+        ops.cache_copy(self.tables[1], self.page_pairs, self.copied)
+
+    def attention_rows(self, projected, places, query, rows):
+        k, v = projected[0, 2 * HEADS * WIDE:], projected[0, (2 * HEADS + KV) * WIDE:]
+        self.ops.prepare_attention_decode(projected, k, v, self.q_weight, self.k_weight, *places, query, *self.caches, rows,
+                                          self.page, self.row, self.row, self.row, self.kv_scale, self.kv_scale)
+
+    def next_token(self):
+        ops, (slots, _, _, _, contexts), n = self.ops, self.lists, self.sequences + 1
+        ops.delta_prepare_decode(self.next_mixed, self.a, self.b, self.taps, self.a_log, self.dt_bias, self.history, slots, self.q,
+                                 self.k, self.v, self.next_alpha, self.next_beta, self.kq, self.capacity, n, self.width)
+        ops.delta_decode_slots_packed(self.codes, self.scales, slots, self.q, self.k, self.v, self.next_alpha, self.next_beta,
+                                      self.kq, self.next_values, self.capacity, n)
+        ops.delta_gated_rmsnorm(self.next_values, self.next_mixed, self.z, self.weight, self.next_out, n, self.width)
+        self.attention_rows(self.next_projected, self.next_places, self.next_query, n)
+        ops.gated_packed(self.next_query, self.next_projected, *self.caches, self.table, contexts, self.widest,
+                         self.next_attended, n, 0, 8, self.workspaces[2], self.page, self.kv_scale, self.kv_scale, self.row)
+
+    def run(self):
+        self.prompts()
+        for held, state in zip(self.between, self.state):
+            held.copy_(state)
+        self.next_token()
+
+
+def layers_as_cases(torch, layers):
+    """The chunk operators' cases on what the layers' calls have read and written."""
+    delta = Delta(torch, 0, layers.lengths, layers.heads, continues=layers.continues, normed=True, gate_offset=layers.z)
+    delta.slots, delta.capacity = layers.slots[:-1], layers.capacity
+    delta.qkv, delta.alpha, delta.beta = layers.qkv, layers.alpha, layers.beta
+    delta.codes, delta.scales = layers.before[0].clone(), layers.before[1].clone()
+    delta.gate, delta.gate_stride, delta.weight = layers.mixed[:, :layers.a].contiguous(), 0, layers.weight
+    delta.gate_stride = layers.a
+    attention = Attention(torch, 0, layers.lengths, [c - n for c, n in zip(layers.contexts, layers.lengths)], layers.page)
+    attention.table, attention.widest, attention.pool = layers.table[:-1].contiguous(), layers.widest, layers.pool
+    attention.query, attention.gate, attention.gate_stride = layers.query, layers.projected, layers.row
+    attention.caches, attention.scale = layers.between[3:], layers.kv_scale
+    return delta, attention
+
+
+@pytest.mark.parametrize("heads,page,lengths,past", [(32, 16, [70, 1, 33], [0, 40, 95]), (48, 64, [130, 64], [0, 0]),
+                                                    (32, 64, [5], [1000])])
+def test_prompts_a_shared_prefix_and_the_next_token(cuda, ops, heads, page, lengths, past):
+    torch = cuda
+    layers = Layers(torch, ops, 41, lengths, past, heads, page)
+    layers.run()
+    count = layers.sequences
+    # the chunk operators, on what they were given (the same calls again: the same bits), against their plain forms
+    delta, attention = layers_as_cases(torch, layers)
+    delta.check(ops)
+    attention.check(ops)
+    assert torch.equal(delta.out, layers.out) and torch.equal(attention.output, layers.attended)
+    for s in range(count):
+        assert torch.equal(delta.codes[layers.slots[s]], layers.between[0][layers.slots[s]])
+    # the decode step begins where the chunk ended: the convolution's history ...
+    for s in range(count):
+        rows = layers.mixed[layers.first[s]:layers.first[s + 1], :layers.channels].float().T
+        before = layers.before[2][layers.slots[s]] * layers.continues[s]
+        assert torch.equal(layers.between[2][layers.slots[s]], torch.cat([before, rows], 1)[:, -3:])
+    # ... the state (fp32 sums of 128 products of either sign: 2^-17 of their magnitudes) ...
+    held = layers.between[0].double() * layers.between[1].double()[..., None]
+    state = held[layers.slots]
+    ratio = heads // KEY_HEADS
+    q, k = (x.double().repeat_interleave(ratio, 1) for x in (layers.q, layers.k))
+    state = state * layers.next_alpha.double()[..., None, None]
+    u = (layers.v.double() - torch.einsum("shij,shj->shi", state, k)) * layers.next_beta.double()[..., None]
+    want = torch.einsum("shij,shj->shi", state, q) + u * (k * q).sum(-1, keepdim=True)
+    terms = torch.einsum("shij,shj->shi", state.abs(), q.abs() + k.abs()) + layers.v.abs().double()
+    assert ((layers.next_values.double() - want).abs() <= 2.0 ** -17 * terms + 1e-6 * want.abs().amax()).all()
+    # ... and the cache
+    tail = Attention(torch, 0, [1] * (count + 1), layers.contexts + [layers.contexts[0]], page)
+    tail.table, tail.widest, tail.pool = layers.table, layers.widest, layers.pool
+    tail.query, tail.gate, tail.gate_stride = layers.next_query, layers.next_projected, layers.row
+    tail.caches, tail.scale = layers.caches, layers.kv_scale
+    tail.check(ops)
+    want, spread = tail.want()
+    # (the decode attention's own rounding: see its tests)
+    assert ((layers.next_attended.double() - want).abs() <= 2.0 ** -7 * want.abs() + 2.0 ** -6 * spread).all()
+    # the copy of the first sequence says what that one says (the decode attention cuts rows where its shares end, so that
+    # row is above, within its rounding)
+    for x in (layers.next_values, layers.next_out, layers.next_query):
+        assert torch.equal(x[0], x[count])
+    for x in layers.state[:3]:
+        assert torch.equal(x[layers.slots[0]], x[0])
+
+
+def test_captured_and_replayed(cuda, ops):
+    torch = cuda
+    layers = Layers(torch, ops, 42, [100, 1, 60], [0, 500, 30], 32)
+    layers.run()
+    want = [x.clone() for x in layers.results]
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    layers.restore()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side), torch.cuda.graph(graph, stream=side):
+        layers.run()
+    for _ in range(3):
+        layers.restore()
+        for x in layers.results[:-5]:
+            x.fill_(3.0)
+        graph.replay()
+        assert all(torch.equal(x, y) for x, y in zip(layers.results, want))
+
+
+def test_two_at_once_on_streams_of_their_own(cuda, ops):
+    torch = cuda
+    both = [Layers(torch, ops, 43, [300, 1, 60], [0, 900, 30], 48), Layers(torch, ops, 44, [65, 129], [3000, 0], 48)]
+    wants = []
+    for layers in both:
+        layers.run()
+        wants.append([x.clone() for x in layers.results])
+    streams = [torch.cuda.Stream() for _ in both]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for layers in both:
+            layers.restore()
+        for stream in streams:
+            stream.wait_stream(torch.cuda.current_stream())
+        for layers, stream in zip(both, streams):
+            with torch.cuda.stream(stream):
+                layers.run()
+        torch.cuda.synchronize()
+        for layers, want in zip(both, wants):
+            assert all(torch.equal(x, y) for x, y in zip(layers.results, want))
+
+
+# ---- ranges ---------------------------------------------------------------------------------------
+
+def off_by_16(torch, tensor):
+    """The same numbers at an address that is a multiple of 16 and not of 32."""
+    room = torch.empty(tensor.numel() + 32, dtype=tensor.dtype, device="cuda")
+    skip = 16 // tensor.element_size()
+    if room.data_ptr() % 32:
+        skip = 0
+    moved = room[skip:skip + tensor.numel()].view(tensor.shape)
+    moved.copy_(tensor)
+    assert moved.data_ptr() % 32 == 16
+    return moved
+
+
+@pytest.mark.parametrize("part", ["query", "gate", "output", "workspace"])
+def test_attention_chunk_rows_at_16_byte_boundaries(cuda, ops, part):
+    case = Attention(cuda, 51, [100, 1, 30], [2000, 40, 0], 16, gate_stride=HEADS * 2 * WIDE + (8 if part == "gate" else 0))
+    workspace = cuda.zeros(ops.attention_chunk_workspace_bytes(), dtype=cuda.uint8, device="cuda")
+    if part == "workspace":
+        workspace = off_by_16(cuda, workspace)
+    else:
+        setattr(case, part, off_by_16(cuda, getattr(case, part)))
+    case.check(ops, workspace=workspace)
+
+
+def test_delta_chunk_rows_at_16_byte_boundaries(cuda, ops):
+    case = Delta(cuda, 52, [100, 1, 30], 32, normed=True, gate_offset=8)
+    for name in ("qkv", "gate", "out", "codes", "weight"):
+        setattr(case, name, off_by_16(cuda, getattr(case, name)))
+    case.check(ops, workspace=off_by_16(cuda, cuda.zeros(ops.delta_chunk_workspace_bytes(131, 3), dtype=cuda.uint8, device="cuda")))
+
+
+def test_128_sequences(cuda, ops):
+    lengths = [(7 * i) % 13 for i in range(128)]
+    Attention(cuda, 53, lengths, [(31 * i) % 200 for i in range(128)], 16).check(ops)
+    Delta(cuda, 54, lengths, 32, continues=[i % 3 % 2 for i in range(128)], normed=True).check(ops)
+    Prepare(cuda, 55, lengths, 32, continues=[i % 3 % 2 for i in range(128)]).check(ops)
+
+
+def test_attention_chunk_pages_beyond_four_gigabytes(cuda, ops):
+    torch = cuda
+    case = Attention(cuda, 56, [50, 3], [300, 700], 16)
+    small, pool = case.caches, 266000  # pages of 16 KiB
+    first = pool - case.pool
+    assert first * KV * 16 * WIDE > 1 << 32
+    big = [torch.full((pool, KV, 16, WIDE), 0x7f, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    want, spread = case.want()
+    for to, rows in zip(big, small):
+        to[first:] = rows
+    case.table[case.table < case.pool] += first
+    case.caches, case.pool = big, pool
+    got = case.run(ops).double()
+    assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * spread).all()
+
+
+def test_cache_copy_beyond_four_gigabytes(cuda, ops):
+    torch = cuda
+    array = torch.zeros((70000, 65536), dtype=torch.uint8, device="cuda")
+    array[3] = torch.arange(65536, device="cuda") % 251
+    ops.cache_copy(ops.copy_table([array], 70000), i32(torch, [3, 69999]), 1)
+    assert torch.equal(array[69999], array[3]) and not array[69998].any()
+
+
+def test_longest_chunk(cuda, ops):
+    """65536 tokens: rows of the beginning, and of the end, where nothing of the beginning is left."""
+    torch, n, warm, rows = cuda, 65536, 400, 100
+    case = Delta(cuda, 57, [n], 32, rate=(0.8, 2.0))  # (alpha^400 is below e^-150)
+    case.run(ops)
+    start = Delta(cuda, 57, [rows], 32)
+    start.qkv, start.alpha, start.beta = (x[:rows].contiguous() for x in (case.qkv, case.alpha, case.beta))
+    fresh = Delta(cuda, 57, [n], 32, rate=(0.8, 2.0))
+    start.slots, start.codes, start.scales = fresh.slots, fresh.codes, fresh.scales
+    want, largest, _ = start.want()
+    assert ((case.out[:rows].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * largest).all()
+    end = Delta(cuda, 57, [warm + rows], 32, continues=[0])
+    end.qkv, end.alpha, end.beta = (x[-warm - rows:].contiguous() for x in (case.qkv, case.alpha, case.beta))
+    want, largest, _ = end.want()
+    got = case.out[-rows:].double()
+    assert ((got - want[-rows:]).abs() <= 2.0 ** -8 * want[-rows:].abs() + 2.0 ** -10 * largest[-rows:]).all()
+    attention = Attention(cuda, 58, [n], [0], 64, gated=False)
+    got = attention.run(ops)
+    picked = torch.tensor([0, 1, 41, 42, 127, 128, 4095, 32767, 50000, 65535], device="cuda")
+    k, v = (c[attention.table[0].long()].view(torch.float8_e4m3fn).double().transpose(0, 1).reshape(KV, -1, WIDE) *
+            attention.scale.double()[:, None, None] for c in attention.caches)
+    for row in picked.tolist():
+        q = attention.query[row].double().reshape(KV, GROUP, WIDE)
+        weights = torch.softmax(q @ k[:, :row + 1].transpose(1, 2) / 16.0, -1)
+        want, spread = ((weights @ x[:, :row + 1]).reshape(HEADS, WIDE) for x in (v, v.abs()))
+        assert ((got[row].double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * spread).all(), row
+
+
+def test_delta_chunk_a_gate_that_is_no_number(cuda, ops):
+    # it reaches its head's rows from there on, and nothing else
+    case = Delta(cuda, 59, [100, 30], 32)
+    want, largest, _ = case.want()
+    case.alpha[40, 5] = float("nan")
+    case.run(ops)
+    got = case.out.double()
+    reached = cuda.zeros((130, 32), dtype=cuda.bool, device="cuda")
+    reached[64:100, 5] = True   # (of the block that holds it, rows in front may be reached too)
+    inside = cuda.zeros_like(reached)
+    inside[:64, 5] = True
+    close = ((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * largest).all(-1)
+    assert close[~(reached | inside)].all() and got[64:100, 5].isnan().all() and got[40:64, 5].isnan().all()
