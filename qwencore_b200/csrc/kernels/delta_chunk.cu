@@ -904,8 +904,10 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             for (int c = 0; c < 2; ++c) {
                 load_columns(held + 32 * c, x);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    x[i] *= end;
+                for (int i = 0; i < 32; i += 2) {
+                    const float2 both = mul_pair({x[i], x[i + 1]}, {end, end});
+                    x[i] = both.x;
+                    x[i + 1] = both.y;
                 }
                 tmem_store_columns(held + 32 * c, x);
             }
@@ -959,15 +961,13 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
         const int row = quarter * 32 + lane;     // value dim
         const uint32_t tmem = (static_cast<uint32_t>(quarter * 32) << 16) + group * 32;
         const int piece = lane & 15;             // later: value dims 4 piece .. + 3 and 64 + 4 piece .. + 3 of a token
-        float gain[8] = {};
+        float2 gain[4] = {};
         if (norm.gate != nullptr) {
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const uint2 raw = *reinterpret_cast<const uint2*>(norm.weight + 64 * i + 4 * piece);
-                gain[4 * i] = __uint_as_float(raw.x << 16);
-                gain[4 * i + 1] = __uint_as_float(raw.x & 0xffff0000u);
-                gain[4 * i + 2] = __uint_as_float(raw.y << 16);
-                gain[4 * i + 3] = __uint_as_float(raw.y & 0xffff0000u);
+                gain[2 * i] = {__uint_as_float(raw.x << 16), __uint_as_float(raw.x & 0xffff0000u)};
+                gain[2 * i + 1] = {__uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
             }
         }
         for (; n < blocks; ++n) {
@@ -985,10 +985,12 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float4 g = *reinterpret_cast<const float4*>(&sm.decay[n & 1][group * 32 + 4 * i]);
-                    x[4 * i] = fmaf(g.x, y[4 * i], x[4 * i]);
-                    x[4 * i + 1] = fmaf(g.y, y[4 * i + 1], x[4 * i + 1]);
-                    x[4 * i + 2] = fmaf(g.z, y[4 * i + 2], x[4 * i + 2]);
-                    x[4 * i + 3] = fmaf(g.w, y[4 * i + 3], x[4 * i + 3]);
+                    const float2 lo = fma_pair({g.x, g.y}, {y[4 * i], y[4 * i + 1]}, {x[4 * i], x[4 * i + 1]});
+                    const float2 hi = fma_pair({g.z, g.w}, {y[4 * i + 2], y[4 * i + 3]}, {x[4 * i + 2], x[4 * i + 3]});
+                    x[4 * i] = lo.x;
+                    x[4 * i + 1] = lo.y;
+                    x[4 * i + 2] = hi.x;
+                    x[4 * i + 3] = hi.y;
                 }
             }
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1014,45 +1016,66 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             if (!ok) {
                 break;
             }
-            // rows of the batch: eight tokens of this warp, two at a time (not all unrolled: the warps' code has to fit
-            // the instruction cache together)
+            // rows of the batch: eight tokens of this warp, two at a time
+            const int first = (warp - kChainWarps) * 8 + (lane >> 4);
+            float2 o[4][4];
+            float inverse[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int t = (warp - kChainWarps) * 8 + 2 * i + (lane >> 4);
+                const float4 lo = *reinterpret_cast<const float4*>(&sm.rows[(first + 2 * i) * kDim + 4 * piece]);
+                const float4 hi = *reinterpret_cast<const float4*>(&sm.rows[(first + 2 * i) * kDim + 64 + 4 * piece]);
+                o[i][0] = {lo.x, lo.y};
+                o[i][1] = {lo.z, lo.w};
+                o[i][2] = {hi.x, hi.y};
+                o[i][3] = {hi.z, hi.w};
+            }
+            if (norm.gate != nullptr) {
+                // (the four sums go through the warp side by side)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float2 sums = mul_pair(o[i][0], o[i][0]);
+#pragma unroll
+                    for (int j = 1; j < 4; ++j) {
+                        sums = fma_pair(o[i][j], o[i][j], sums);
+                    }
+                    inverse[i] = sums.x + sums.y;
+                }
+#pragma unroll
+                for (int offset = 1; offset < 16; offset <<= 1) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        inverse[i] += __shfl_xor_sync(0xffffffffu, inverse[i], offset);
+                    }
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    inverse[i] = rsqrtf(inverse[i] / static_cast<float>(kDim) + norm.epsilon);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int t = first + 2 * i;
                 const int token = n * kBlock + t;
-                const float4 lo = *reinterpret_cast<const float4*>(&sm.rows[t * kDim + 4 * piece]);
-                const float4 hi = *reinterpret_cast<const float4*>(&sm.rows[t * kDim + 64 + 4 * piece]);
-                float o[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
                 if (norm.gate != nullptr) {
-                    float sum = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        sum = fmaf(o[j], o[j], sum);
-                    }
-#pragma unroll
-                    for (int offset = 1; offset < 16; offset <<= 1) {
-                        sum += __shfl_xor_sync(0xffffffffu, sum, offset);
-                    }
-                    const float inverse = rsqrtf(sum / static_cast<float>(kDim) + norm.epsilon);
                     const uint2 gate_lo = *reinterpret_cast<const uint2*>(sm.gate[n & 1] + t * (kDim * 2) + 8 * piece);
                     const uint2 gate_hi = *reinterpret_cast<const uint2*>(sm.gate[n & 1] + t * (kDim * 2) + kDim + 8 * piece);
                     const uint32_t words[4] = {gate_lo.x, gate_lo.y, gate_hi.x, gate_hi.y};
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const float z = __uint_as_float((j & 1) != 0 ? words[j >> 1] & 0xffff0000u : words[j >> 1] << 16);
-                        o[j] *= inverse * gain[j] * (z * sigmoid_fast(z));
+                    for (int j = 0; j < 4; ++j) {
+                        const float2 z = {__uint_as_float(words[j] << 16), __uint_as_float(words[j] & 0xffff0000u)};
+                        const float2 silu = mul_pair(z, sigmoid_pair(z));
+                        o[i][j] = mul_pair(mul_pair(o[i][j], {inverse[i], inverse[i]}), mul_pair(gain[j], silu));
                     }
-                }
-                uint32_t words[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const __nv_bfloat162 pair = __floats2bfloat162_rn(o[2 * j], o[2 * j + 1]);
-                    words[j] = *reinterpret_cast<const uint32_t*>(&pair);
                 }
                 if (token < span.length) {
                     __nv_bfloat16* to = out + ((static_cast<size_t>(span.begin) + token) * v_heads + head) * kDim + 4 * piece;
-                    *reinterpret_cast<uint2*>(to) = make_uint2(words[0], words[1]);
-                    *reinterpret_cast<uint2*>(to + 64) = make_uint2(words[2], words[3]);
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        const __nv_bfloat162 lo = __floats2bfloat162_rn(o[i][2 * j].x, o[i][2 * j].y);
+                        const __nv_bfloat162 hi = __floats2bfloat162_rn(o[i][2 * j + 1].x, o[i][2 * j + 1].y);
+                        *reinterpret_cast<uint2*>(to + 64 * j) =
+                            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+                    }
                 }
             }
             __syncwarp();
