@@ -77,8 +77,7 @@ constexpr uint32_t kTransposeA = 1u << 15, kTransposeB = 1u << 16;
 
 // Operand of 128-byte rows with the 128-byte swizzle, eight rows to an atom.  K-major: a row is one of M or N, its bytes 64
 // of the contracted elements.  MN-major: a row is one of the contracted, its bytes 64 of M or N, the next 64 `block` bytes on.
-// Made in two steps, the lower word of its beginning once and then the part of it that an MMA reads: the thread that issues
-// needs an operand in uniform registers, and one addition is all that is left there (it is what the issue then takes).
+// Made in two steps, the lower word of its beginning once and then the part of it that an MMA reads, one addition.
 __device__ __forceinline__ uint32_t operand_base(uint32_t address, uint32_t block) {
     return ((address >> 4) & 0x3FFFu) | ((block >> 4) & 0x3FFFu) << 16;
 }
@@ -166,7 +165,10 @@ constexpr int kFactorThreads = 128;
 constexpr int kPitch = 68;  // floats of a row of the matrices in shared memory: rows begin in different banks
 
 constexpr int kMaxRatio = 3;  // value heads of a key head
-constexpr int kFewBlocks = 12;
+// Below this many blocks of a call a CTA takes one value head, from there on all of a key head, which share [Q ; K] K^T:
+// 48 heads, 64 tokens 31.1 us with one head and 40.5 with three, 512 tokens 55 and 60, 1280 tokens 102 and 106, 1600
+// tokens 123 and 121, 4 x 2048 tokens 352 and 335; 32 heads, 704 tokens 58.8 and 62.1, 1600 tokens 108.4 and 107.7.
+constexpr int kFewBlocks = 24;
 
 struct FactorSmem {
     union {
