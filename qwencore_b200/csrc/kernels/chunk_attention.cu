@@ -1218,6 +1218,24 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const __g
         return (2 * static_cast<size_t>(pair + piece) + (piece == 0 ? 1 : 0)) * kSlotRows + r;
     };
     const int pieces = item.last_pair - pair + 1;
+    const size_t row = static_cast<size_t>(item.first_row) + token;
+    const int head = item.head * kGqaGroup + index % kGqaGroup;
+    // everything that does not wait for something else is asked for at once: gates, the first pieces, the statistics
+    uint4 gates = make_uint4(0, 0, 0, 0);
+    if (p.gate != nullptr) {
+        gates = __ldg(reinterpret_cast<const uint4*>(p.gate + row * p.gate_stride + head * (2 * kHeadDim) + kHeadDim) + lane);
+    }
+    uint4 raw[kMergeDepth];
+    const auto fetch = [&](int first) {
+#pragma unroll
+        for (int j = 0; j < kMergeDepth; ++j) {
+            raw[j] = make_uint4(0, 0, 0, 0);
+            if (first + j < pieces) {
+                raw[j] = reinterpret_cast<const uint4*>(p.partial_out + slot(first + j) * kHeadDim)[lane];
+            }
+        }
+    };
+    fetch(0);
     // a piece per lane: its weight (at most 96 pieces)
     float maximum = -INFINITY;
     PartialStats stats[(kMaxPairs + 31) / 32];
@@ -1240,21 +1258,12 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const __g
 #pragma unroll
     for (int i = 0; i < (kMaxPairs + 31) / 32; ++i) {
         const float mine = !(stats[i].sum <= 0.0f) ? stats[i].sum * exp2f(stats[i].maximum - maximum) : 0.0f;
-        const int count = min(32, pieces - 32 * i);
 #pragma unroll 1
-        for (int first = 0; first < count; first += kMergeDepth) {
-            uint4 raw[kMergeDepth];
-#pragma unroll
-            for (int j = 0; j < kMergeDepth; ++j) {
-                raw[j] = make_uint4(0, 0, 0, 0);
-                if (first + j < count) {
-                    raw[j] = reinterpret_cast<const uint4*>(p.partial_out + slot(32 * i + first + j) * kHeadDim)[lane];
-                }
-            }
+        for (int first = 32 * i; first < min(32 * i + 32, pieces); first += kMergeDepth) {
 #pragma unroll
             for (int j = 0; j < kMergeDepth; ++j) {
                 const float weight = __shfl_sync(0xffffffffu, mine, (first + j) & 31);
-                if (first + j < count) {
+                if (first + j < pieces) {
                     denominator += weight;
                     const uint32_t words[4] = {raw[j].x, raw[j].y, raw[j].z, raw[j].w};
 #pragma unroll
@@ -1265,20 +1274,14 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const __g
                     }
                 }
             }
+            if (first + kMergeDepth < pieces) {
+                fetch(first + kMergeDepth);
+            }
         }
     }
     const float v_scale = p.value_scales ? p.value_scales[item.head] : 1.0f;
     const float inverse = denominator > 0.0f || isnan(denominator) ? v_scale / denominator : 0.0f;
-    const size_t row = static_cast<size_t>(item.first_row) + token;
-    const int head = item.head * kGqaGroup + index % kGqaGroup;
-    uint32_t gate_words[4] = {0, 0, 0, 0};
-    if (p.gate != nullptr) {
-        const uint4 raw = __ldg(reinterpret_cast<const uint4*>(p.gate + row * p.gate_stride + head * (2 * kHeadDim) + kHeadDim) + lane);
-        gate_words[0] = raw.x;
-        gate_words[1] = raw.y;
-        gate_words[2] = raw.z;
-        gate_words[3] = raw.w;
-    }
+    const uint32_t gate_words[4] = {gates.x, gates.y, gates.z, gates.w};
     uint32_t words[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
