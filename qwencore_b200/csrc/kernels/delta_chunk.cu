@@ -419,8 +419,9 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
             }
         }
         __syncthreads();
-        // the block of 32 below: a row per lane, eight columns per warp (T_00 is zero above its diagonal)
-        {
+        // the block of 32 below: a row per lane, eight columns per warp (T_00 is zero above its diagonal); in blocks of 32
+        // tokens or fewer it is zero, as A is there
+        if (count > 32) {
             const int column = 8 * warp;
             float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
             if (ok) {
@@ -444,8 +445,8 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
                 *reinterpret_cast<float4*>(at) = make_float4(-y[0], -y[1], -y[2], -y[3]);
                 *reinterpret_cast<float4*>(at + 4) = make_float4(-y[4], -y[5], -y[6], -y[7]);
             }
+            __syncthreads();
         }
-        __syncthreads();
         // T diag(beta) as an operand: half a row per thread
         const int row = tid >> 1, half = tid & 1;
         float x[32];
