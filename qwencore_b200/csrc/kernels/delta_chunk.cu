@@ -189,17 +189,17 @@ struct FactorSmem {
 };
 static_assert(offsetof(FactorSmem, m.product) % 1024 == 0, "an operand's alignment");
 
-// x += a * rows[0 .. 3][8 columns] for four steps of the sum.
-__device__ __forceinline__ void multiply4(float (&x)[8], const float4& a, const float* rows) {
-    const float factors[4] = {a.x, a.y, a.z, a.w};
+// x += a * rows[0 .. 3][4 columns] for four steps of the sum, for kRows rows of a.
+template <int kRows>
+__device__ __forceinline__ void multiply4(float2 (&x)[kRows][2], const float4 (&a)[kRows], const float* rows) {
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-        const float4 lo = *reinterpret_cast<const float4*>(rows + k * kPitch);
-        const float4 hi = *reinterpret_cast<const float4*>(rows + k * kPitch + 4);
-        const float row[8] = {lo.x, lo.y, lo.z, lo.w, hi.x, hi.y, hi.z, hi.w};
+        const float4 row = *reinterpret_cast<const float4*>(rows + k * kPitch);
 #pragma unroll
-        for (int c = 0; c < 8; ++c) {
-            x[c] = fmaf(factors[k], row[c], x[c]);
+        for (int r = 0; r < kRows; ++r) {
+            const float factor = k == 0 ? a[r].x : k == 1 ? a[r].y : k == 2 ? a[r].z : a[r].w;
+            x[r][0] = fma_pair({factor, factor}, {row.x, row.y}, x[r][0]);
+            x[r][1] = fma_pair({factor, factor}, {row.z, row.w}, x[r][1]);
         }
     }
 }
@@ -385,65 +385,67 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
             }
         }
         __syncthreads();
-        // blocks of 32: T_10 = -T_11 (A_10 T_00) of 16, eight columns per warp, a row per lane (lanes 16-31 do the same again)
+        // blocks of 32: T_10 = -T_11 (A_10 T_00) of 16, eight columns per warp, four columns of a row per lane
         {
-            const int base = 32 * (warp >> 1), column = base + 8 * (warp & 1);
-            const int r = lane & 15;
-            float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            const int base = 32 * (warp >> 1), column = base + 8 * (warp & 1) + 4 * (lane >> 4);
+            const int r = base + 16 + (lane & 15);
+            float* at = &sm.m.t[r * kPitch + column];
+            float2 x[1][2] = {};
             if (ok) {
 #pragma unroll
                 for (int k = 0; k < 16; k += 4) {
-                    multiply4(x, *reinterpret_cast<const float4*>(&sm.m.t[(base + 16 + r) * kPitch + base + k]),
-                              &sm.m.t[(base + k) * kPitch + column]);
+                    const float4 left[1] = {*reinterpret_cast<const float4*>(&sm.m.t[r * kPitch + base + k])};
+                    multiply4(x, left, &sm.m.t[(base + k) * kPitch + column]);
                 }
             }
             __syncthreads();  // (A_10 has been read)
             if (ok) {
-                float* at = &sm.m.t[(base + 16 + r) * kPitch + column];
-                if (lane < 16) {
-                    *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
-                    *reinterpret_cast<float4*>(at + 4) = make_float4(x[4], x[5], x[6], x[7]);
-                }
+                *reinterpret_cast<float4*>(at) = make_float4(x[0][0].x, x[0][0].y, x[0][1].x, x[0][1].y);
                 __syncwarp();
-                float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+                float2 y[1][2] = {};
 #pragma unroll
                 for (int k = 0; k < 16; k += 4) {
-                    multiply4(y, *reinterpret_cast<const float4*>(&sm.m.t[(base + 16 + r) * kPitch + base + 16 + k]),
-                              &sm.m.t[(base + 16 + k) * kPitch + column]);
+                    const float4 left[1] = {*reinterpret_cast<const float4*>(&sm.m.t[r * kPitch + base + 16 + k])};
+                    multiply4(y, left, &sm.m.t[(base + 16 + k) * kPitch + column]);
                 }
                 __syncwarp();
-                if (lane < 16) {
-                    *reinterpret_cast<float4*>(at) = make_float4(-y[0], -y[1], -y[2], -y[3]);
-                    *reinterpret_cast<float4*>(at + 4) = make_float4(-y[4], -y[5], -y[6], -y[7]);
-                }
+                *reinterpret_cast<float4*>(at) = make_float4(-y[0][0].x, -y[0][0].y, -y[0][1].x, -y[0][1].y);
             }
         }
         __syncthreads();
-        // the block of 32 below: a row per lane, eight columns per warp (T_00 is zero above its diagonal); in blocks of 32
-        // tokens or fewer it is zero, as A is there
+        // the block of 32 below: eight columns per warp, four columns of two rows per lane (T_00 is zero above its
+        // diagonal); in blocks of 32 tokens or fewer it is zero, as A is there
         if (count > 32) {
-            const int column = 8 * warp;
-            float x[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
+            const int column = 8 * warp + 4 * (lane >> 4);
+            const int r = 32 + (lane & 15);
+            float* at = &sm.m.t[r * kPitch + column];
+            float2 x[2][2] = {};
             if (ok) {
-                for (int k = column; k < 32; k += 4) {
-                    multiply4(x, *reinterpret_cast<const float4*>(&sm.m.t[(32 + lane) * kPitch + k]), &sm.m.t[k * kPitch + column]);
+                for (int k = 8 * warp; k < 32; k += 4) {
+                    const float4 left[2] = {*reinterpret_cast<const float4*>(&sm.m.t[r * kPitch + k]),
+                                            *reinterpret_cast<const float4*>(&sm.m.t[(r + 16) * kPitch + k])};
+                    multiply4(x, left, &sm.m.t[k * kPitch + column]);
                 }
             }
             __syncthreads();  // (A_10 has been read)
             if (ok) {
-                float* at = &sm.m.t[(32 + lane) * kPitch + column];
-                *reinterpret_cast<float4*>(at) = make_float4(x[0], x[1], x[2], x[3]);
-                *reinterpret_cast<float4*>(at + 4) = make_float4(x[4], x[5], x[6], x[7]);
-                __syncwarp();
-                float y[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 2
-                for (int k = 0; k < 32; k += 4) {
-                    multiply4(y, *reinterpret_cast<const float4*>(&sm.m.t[(32 + lane) * kPitch + 32 + k]),
-                              &sm.m.t[(32 + k) * kPitch + column]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    *reinterpret_cast<float4*>(at + 16 * i * kPitch) = make_float4(x[i][0].x, x[i][0].y, x[i][1].x, x[i][1].y);
                 }
                 __syncwarp();
-                *reinterpret_cast<float4*>(at) = make_float4(-y[0], -y[1], -y[2], -y[3]);
-                *reinterpret_cast<float4*>(at + 4) = make_float4(-y[4], -y[5], -y[6], -y[7]);
+                float2 y[2][2] = {};
+#pragma unroll 2
+                for (int k = 0; k < 32; k += 4) {
+                    const float4 left[2] = {*reinterpret_cast<const float4*>(&sm.m.t[r * kPitch + 32 + k]),
+                                            *reinterpret_cast<const float4*>(&sm.m.t[(r + 16) * kPitch + 32 + k])};
+                    multiply4(y, left, &sm.m.t[(32 + k) * kPitch + column]);
+                }
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    *reinterpret_cast<float4*>(at + 16 * i * kPitch) = make_float4(-y[i][0].x, -y[i][0].y, -y[i][1].x, -y[i][1].y);
+                }
             }
             __syncthreads();
         }
