@@ -897,6 +897,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 x[4 * i + 3] *= -g.w;
             }
             tmem_store_split(x_at, x_at + 16, x);
+            const float end = decay[kBlock - 1];  // (before x_ready: behind it the place may get the block after next)
             tmem_store_wait();
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
@@ -904,7 +905,6 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 mbar_arrive(&sm.x_ready);
             }
             // the state decays while U' is made
-            const float end = decay[kBlock - 1];
 #pragma unroll 1
             for (int c = 0; c < 2; ++c) {
                 load_columns(held + 32 * c, x);
