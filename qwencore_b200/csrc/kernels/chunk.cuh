@@ -35,56 +35,13 @@ __device__ __forceinline__ float reciprocal_fast(float x) {
     return y;
 }
 
-// Two fp32 operations in one instruction, on registers that lie side by side.
-__device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n"
-        ".reg .b64 a, b, c;\n"
-        "mov.b64 a, {%2, %3};\n"
-        "mov.b64 b, {%4, %5};\n"
-        "mov.b64 c, {%6, %7};\n"
-        "fma.rn.f32x2 a, a, b, c;\n"
-        "mov.b64 {%0, %1}, a;\n"
-        "}\n"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
-    return d;
-}
-
-__device__ __forceinline__ float2 mul_pair(float2 a, float2 b) {
-    float2 d;
-    asm("{\n"
-        ".reg .b64 a, b;\n"
-        "mov.b64 a, {%2, %3};\n"
-        "mov.b64 b, {%4, %5};\n"
-        "mul.rn.f32x2 a, a, b;\n"
-        "mov.b64 {%0, %1}, a;\n"
-        "}\n"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-
-__device__ __forceinline__ float2 add_pair(float2 a, float2 b) {
-    float2 d;
-    asm("{\n"
-        ".reg .b64 a, b;\n"
-        "mov.b64 a, {%2, %3};\n"
-        "mov.b64 b, {%4, %5};\n"
-        "add.rn.f32x2 a, a, b;\n"
-        "mov.b64 {%0, %1}, a;\n"
-        "}\n"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
-    return d;
-}
-
 __device__ __forceinline__ float sigmoid_fast(float x) { return reciprocal_fast(1.0f + exp2_fast(x * -1.4426950408889634f)); }
 
+// (The multiplications and additions of two take one instruction.)
 __device__ __forceinline__ float2 sigmoid_pair(float2 x) {
-    const float2 y = mul_pair(x, {-1.4426950408889634f, -1.4426950408889634f});
-    const float2 z = add_pair({exp2_fast(y.x), exp2_fast(y.y)}, {1.0f, 1.0f});
-    return {reciprocal_fast(z.x), reciprocal_fast(z.y)};
+    const float2 y = __fmul2_rn(x, make_float2(-1.4426950408889634f, -1.4426950408889634f));
+    const float2 z = __fadd2_rn(make_float2(exp2_fast(y.x), exp2_fast(y.y)), make_float2(1.0f, 1.0f));
+    return make_float2(reciprocal_fast(z.x), reciprocal_fast(z.y));
 }
 
 // Every chunk is cut into tiles of `tile_tokens` from its own first row; tile numbers run through the chunks in order.

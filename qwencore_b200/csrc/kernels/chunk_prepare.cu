@@ -171,8 +171,7 @@ __global__ void __launch_bounds__(kPrepareWarps * 32) delta_prepare_chunk_kernel
                 x = multiply_add(taps[j], window[j], x);
                 window[j - 1] = window[j];
             }
-            x = multiply(x, {make_float2(sigmoid_fast(x.lo.x), sigmoid_fast(x.lo.y)),
-                             make_float2(sigmoid_fast(x.hi.x), sigmoid_fast(x.hi.y))});
+            x = multiply(x, {sigmoid_pair(x.lo), sigmoid_pair(x.hi)});
             if (head < 2 * kDeltaKeyHeads) {
                 const float total = warp_sum(x.lo.x * x.lo.x + x.lo.y * x.lo.y + x.hi.x * x.hi.x + x.hi.y * x.hi.y);
                 const float inverse = rsqrtf(total + 1e-6f) * unit;

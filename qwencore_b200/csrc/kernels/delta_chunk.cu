@@ -198,8 +198,8 @@ __device__ __forceinline__ void multiply4(float2 (&x)[kRows][2], const float4 (&
 #pragma unroll
         for (int r = 0; r < kRows; ++r) {
             const float factor = k == 0 ? a[r].x : k == 1 ? a[r].y : k == 2 ? a[r].z : a[r].w;
-            x[r][0] = fma_pair({factor, factor}, {row.x, row.y}, x[r][0]);
-            x[r][1] = fma_pair({factor, factor}, {row.z, row.w}, x[r][1]);
+            x[r][0] = __ffma2_rn({factor, factor}, {row.x, row.y}, x[r][0]);
+            x[r][1] = __ffma2_rn({factor, factor}, {row.z, row.w}, x[r][1]);
         }
     }
 }
@@ -910,7 +910,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 load_columns(held + 32 * c, x);
 #pragma unroll
                 for (int i = 0; i < 32; i += 2) {
-                    const float2 both = mul_pair({x[i], x[i + 1]}, {end, end});
+                    const float2 both = __fmul2_rn({x[i], x[i + 1]}, {end, end});
                     x[i] = both.x;
                     x[i + 1] = both.y;
                 }
@@ -990,8 +990,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const float4 g = *reinterpret_cast<const float4*>(&sm.decay[n & 1][group * 32 + 4 * i]);
-                    const float2 lo = fma_pair({g.x, g.y}, {y[4 * i], y[4 * i + 1]}, {x[4 * i], x[4 * i + 1]});
-                    const float2 hi = fma_pair({g.z, g.w}, {y[4 * i + 2], y[4 * i + 3]}, {x[4 * i + 2], x[4 * i + 3]});
+                    const float2 lo = __ffma2_rn({g.x, g.y}, {y[4 * i], y[4 * i + 1]}, {x[4 * i], x[4 * i + 1]});
+                    const float2 hi = __ffma2_rn({g.z, g.w}, {y[4 * i + 2], y[4 * i + 3]}, {x[4 * i + 2], x[4 * i + 3]});
                     x[4 * i] = lo.x;
                     x[4 * i + 1] = lo.y;
                     x[4 * i + 2] = hi.x;
@@ -1038,10 +1038,10 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 // (the four sums go through the warp side by side)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float2 sums = mul_pair(o[i][0], o[i][0]);
+                    float2 sums = __fmul2_rn(o[i][0], o[i][0]);
 #pragma unroll
                     for (int j = 1; j < 4; ++j) {
-                        sums = fma_pair(o[i][j], o[i][j], sums);
+                        sums = __ffma2_rn(o[i][j], o[i][j], sums);
                     }
                     inverse[i] = sums.x + sums.y;
                 }
@@ -1068,8 +1068,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const float2 z = {__uint_as_float(words[j] << 16), __uint_as_float(words[j] & 0xffff0000u)};
-                        const float2 silu = mul_pair(z, sigmoid_pair(z));
-                        o[i][j] = mul_pair(mul_pair(o[i][j], {inverse[i], inverse[i]}), mul_pair(gain[j], silu));
+                        const float2 silu = __fmul2_rn(z, sigmoid_pair(z));
+                        o[i][j] = __fmul2_rn(__fmul2_rn(o[i][j], {inverse[i], inverse[i]}), __fmul2_rn(gain[j], silu));
                     }
                 }
                 if (token < span.length) {
