@@ -535,7 +535,8 @@ int qwc_cache_copy(const qwc_copy_array* arrays, int array_count, const uint32_t
  * chunk) and sees the positions up to its own; a row that sees none is zero.  Heads, cache layout, scales, gate
  * and gate_stride as qwc_paged_attention_packed_fp8_scaled, except that block_tables u32[sequences, max_blocks] has a
  * row for each sequence.  query, output bf16[tokens, 24, 256].  num_blocks: pages of the cache; a page
- * beyond it reads as zeros.  workspace: qwc_paged_attention_chunk_workspace_bytes() bytes; calls that overlap on
+ * beyond it reads as zeros.  Scales are positive.  A value code that is no number (0x7f, 0xff) counts as 480 times the
+ * scale, a key code makes its row NaN where it is seen.  workspace: qwc_paged_attention_chunk_workspace_bytes() bytes; calls that overlap on
  * the device must not share one.  Pointers of rows, caches and workspace 16-byte aligned.
  * The segment shapes of crates/qwc-cuda/src/ffi.rs:520-537, for a whole batch.
  */
@@ -553,6 +554,7 @@ int qwc_paged_attention_chunk_fp8(const void* query, const void* query_gate_proj
  * mixed_stride % 8 == 0); the convolution starts from the slot's history conv_state f32[capacity, channels, 3] and leaves
  * the chunk's last rows there.  qkv bf16[tokens, channels]: q [16][128] (scaled by 128^-1/2) | k [16][128] |
  * v [heads][128], each rounded once; alpha, beta f32[tokens, heads].  mixed_qkv, conv_weight, conv_state and qkv 16-byte aligned.
+ * conv_weight must not be written by the kernel just before this one.
  */
 int qwc_delta_prepare_chunk(const void* mixed_qkv, const void* a_projection, const void* b_projection,
                             const void* conv_weight, const void* a_log, const void* dt_bias, void* conv_state,

@@ -604,7 +604,7 @@ __device__ __forceinline__ void tmem_store_split(uint32_t upper_at, uint32_t low
 __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
     int8_t* __restrict__ state, float* __restrict__ state_scales, const uint32_t* __restrict__ state_slots,
     const uint32_t* __restrict__ continues, const uint32_t* __restrict__ begins, const __nv_bfloat16* __restrict__ qkv,
-    const Images images, __nv_bfloat16* __restrict__ out, int tokens, int v_heads, int state_capacity,
+    const Images images, int images_blocks, __nv_bfloat16* __restrict__ out, int tokens, int v_heads, int state_capacity,
     const OutputNorm norm, int* status) {
     extern __shared__ unsigned char smem_raw[];
     ChainSmem& sm = *reinterpret_cast<ChainSmem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
@@ -679,7 +679,8 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
         for (; n < blocks && ok; ++n) {
             const int slot_of = n & 1;
             const uint32_t parity = ((n >> 1) & 1) ^ 1;
-            const size_t block = static_cast<size_t>(first_block) + n;
+            // (chunks that overlap have more blocks than there is room for: what they get is nobody's, but it is there)
+            const size_t block = static_cast<size_t>(min(first_block + n, images_blocks - 1));
             ok = wait(&sm.w_empty[slot_of], parity, failed, status);
             if (ok && lane == 0) {
                 mbar_arrive_expect_tx(&sm.w_full[slot_of], kWBytes + kBlock * 4);
@@ -1212,6 +1213,6 @@ extern "C" int qwc_delta_chunk_int8(void* state, float* state_scales, const void
     return launch_chained(delta_chain_kernel, dim3(v_heads, sequences), dim3(kChainThreads), sizeof(ChainSmem) + 1024, stream,
                           static_cast<int8_t*>(state), state_scales, static_cast<const uint32_t*>(state_slots),
                           static_cast<const uint32_t*>(continues), static_cast<const uint32_t*>(chunk_begins),
-                          static_cast<const __nv_bfloat16*>(qkv), images, static_cast<__nv_bfloat16*>(out), tokens, v_heads,
-                          state_capacity, norm, status);
+                          static_cast<const __nv_bfloat16*>(qkv), images, blocks, static_cast<__nv_bfloat16*>(out), tokens,
+                          v_heads, state_capacity, norm, status);
 }

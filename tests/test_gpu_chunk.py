@@ -865,3 +865,44 @@ def test_delta_chunk_a_gate_that_is_no_number(cuda, ops):
     inside[:64, 5] = True
     close = ((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * largest).all(-1)
     assert close[~(reached | inside)].all() and got[64:100, 5].isnan().all() and got[40:64, 5].isnan().all()
+
+
+def test_chunks_that_overlap_or_run_backwards_stay_in_bounds(cuda, ops):
+    """Not what the calls are for: no row of theirs has a meaning, but nothing else is touched and the next call is right."""
+    torch = cuda
+    for begins in ([0, 100, 0, 100, 0, 100, 0, 100], [100, 0, 90, 10, 80, 20, 70, 30], [2 ** 31 - 1, 0, 100, 100, 50, 2 ** 31 - 1, 3, 4]):
+        delta = Delta(torch, 61, [100] + [0] * 6, 32, normed=True, padding=3)
+        delta.first = begins
+        delta.run(ops)
+        assert (delta.out[100:] == 7.0).all() or max(begins) > 103
+        idle = [s for s in range(delta.capacity) if s not in delta.slots]
+        fresh = Delta(torch, 61, [100] + [0] * 6, 32, normed=True, padding=3)
+        assert all(torch.equal(delta.codes[s], fresh.codes[s]) for s in idle)
+        attention = Attention(torch, 62, [100] + [0] * 6, [30] * 7, padding=3)
+        attention.first = begins
+        attention.run(ops)
+        prepared = Prepare(torch, 63, [100] + [0] * 6, 32, padding=3)
+        prepared.first = begins
+        prepared.run(ops)
+        torch.cuda.synchronize()
+    Delta(torch, 64, [100, 70], 32, normed=True).check(ops)
+    Attention(torch, 65, [100, 70], [30, 0]).check(ops)
+    Prepare(torch, 66, [100, 70], 32).check(ops)
+
+
+def test_attention_chunk_value_codes_that_are_no_number(cuda, ops):
+    # seen by every row: 480 times the scale, of either sign
+    case = Attention(cuda, 67, [20], [100], gated=False)
+    page = case.table[0, 1].long()
+    case.caches[1][page, 2, 5, 40:44] = cuda.tensor([0x7f, 0xff, 0x7e, 0xfe], dtype=cuda.uint8, device="cuda")
+    got = case.run(ops).double()[:, 12:18, 40:44]
+    ids = case.table[0, :8].long()
+    k, v = (c[ids].view(cuda.float8_e4m3fn).double().transpose(0, 1).reshape(KV, -1, WIDE)[2, :120] * case.scale[2].double()
+            for c in case.caches)
+    v = v[:, 40:44].nan_to_num(0.0)
+    v[21, :2] = cuda.tensor([480.0, -480.0], dtype=cuda.float64, device="cuda") * case.scale[2].double()
+    scores = case.query[:, 12:18].double().transpose(0, 1) @ k.T / 16.0
+    scores = scores.masked_fill(cuda.arange(120, device="cuda")[None] > (cuda.arange(20, device="cuda") + 100)[:, None], -cuda.inf)
+    weights = cuda.softmax(scores, -1)
+    want, spread = (weights @ v).transpose(0, 1), (weights @ v.abs()).transpose(0, 1)
+    assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * spread).all()
