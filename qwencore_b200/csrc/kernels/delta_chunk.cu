@@ -42,11 +42,13 @@ struct Images {
     uint8_t* qk;    // [block][key head][kQkBytes]
     uint8_t* w;     // [block][value head][kWBytes]
     float* decay;   // [block][value head][kBlock]: from the block's start
+    int4* order;    // the chunks, longest first: sequence, first row, length, first block
 };
 
 inline size_t images_bytes(int blocks, int v_heads) {
     return static_cast<size_t>(blocks) *
-           (static_cast<size_t>(kDeltaKeyHeads) * kQkBytes + static_cast<size_t>(v_heads) * (kWBytes + kBlock * sizeof(float)));
+           (static_cast<size_t>(kDeltaKeyHeads) * kQkBytes + static_cast<size_t>(v_heads) * (kWBytes + kBlock * sizeof(float))) +
+           kMaxChunkSequences * sizeof(int4);
 }
 
 inline Images images_at(void* workspace, int blocks, int v_heads) {
@@ -54,6 +56,7 @@ inline Images images_at(void* workspace, int blocks, int v_heads) {
     at.qk = static_cast<uint8_t*>(workspace);
     at.w = at.qk + static_cast<size_t>(blocks) * kDeltaKeyHeads * kQkBytes;
     at.decay = reinterpret_cast<float*>(at.w + static_cast<size_t>(blocks) * v_heads * kWBytes);
+    at.order = reinterpret_cast<int4*>(at.decay + static_cast<size_t>(blocks) * v_heads * kBlock);
     return at;
 }
 
@@ -183,6 +186,7 @@ struct FactorSmem {
     };
     float2 log[kMaxRatio][kBlock];                // log2 of the decay from the start: a whole number and the rest
     float beta[kMaxRatio][kBlock];
+    int length[kMaxChunkSequences];
     uint64_t done;
     uint32_t tmem_base;
     int failed;
@@ -201,6 +205,28 @@ __device__ __forceinline__ void multiply4(float2 (&x)[kRows][2], const float4 (&
             x[r][0] = __ffma2_rn({factor, factor}, {row.x, row.y}, x[r][0]);
             x[r][1] = __ffma2_rn({factor, factor}, {row.z, row.w}, x[r][1]);
         }
+    }
+}
+
+// The chunks in the order of their length, for the second kernel: what takes longest begins first (20 chunks of 4000 tokens
+// in all 170 -> 166 us).  Of two alike the first is the longer.  By a CTA, a thread for a chunk.
+__device__ __forceinline__ void find_order(int (&length)[kMaxChunkSequences], const uint32_t* begins, int tokens, int sequences,
+                                           int4* order) {
+    static_assert(kFactorThreads >= kMaxChunkSequences, "a thread for a chunk");
+    const int mine = threadIdx.x;
+    ChunkSpan span = {0, 0};
+    if (mine < sequences) {
+        span = chunk_span(begins, mine, tokens);
+        length[mine] = span.length;
+    }
+    __syncthreads();
+    if (mine < sequences) {
+        int rank = 0, blocks_before = 0;
+        for (int i = 0; i < sequences; ++i) {
+            rank += length[i] > span.length || (length[i] == span.length && i < mine) ? 1 : 0;
+            blocks_before += i < mine ? (length[i] + kBlock - 1) / kBlock : 0;
+        }
+        order[rank] = make_int4(mine, span.begin, span.length, blocks_before);
     }
 }
 
@@ -234,6 +260,9 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    }
+    if (blockIdx.x == 0 && block == 0) {
+        find_order(sm.length, begins, tokens, sequences, images.order);
     }
     const ChunkTile tile = find_chunk_tile(begins, sequences, tokens, kBlock, block);
     const bool here = tile.sequence >= 0;
@@ -603,9 +632,8 @@ __device__ __forceinline__ void tmem_store_split(uint32_t upper_at, uint32_t low
 
 __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
     int8_t* __restrict__ state, float* __restrict__ state_scales, const uint32_t* __restrict__ state_slots,
-    const uint32_t* __restrict__ continues, const uint32_t* __restrict__ begins, const __nv_bfloat16* __restrict__ qkv,
-    const Images images, int images_blocks, __nv_bfloat16* __restrict__ out, int tokens, int v_heads, int state_capacity,
-    const OutputNorm norm, int* status) {
+    const uint32_t* __restrict__ continues, const __nv_bfloat16* __restrict__ qkv, const Images images, int images_blocks,
+    __nv_bfloat16* __restrict__ out, int v_heads, int state_capacity, const OutputNorm norm, int* status) {
     extern __shared__ unsigned char smem_raw[];
     ChainSmem& sm = *reinterpret_cast<ChainSmem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     const int lane = threadIdx.x & 31;
@@ -613,9 +641,10 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
     const int head = blockIdx.x;
     const int key_head = head / (v_heads / kDeltaKeyHeads);
     const int channels = (2 * kDeltaKeyHeads + v_heads) * kDim;
-    const int sequence = blockIdx.y;
     pdl_wait();
-    const ChunkSpan span = chunk_span(begins, sequence, tokens);
+    const int4 chosen = __ldcg(images.order + blockIdx.y);
+    const int sequence = chosen.x, first_block = chosen.w;
+    const ChunkSpan span = {chosen.y, chosen.z};
     const uint32_t slot = __ldcg(state_slots + sequence);
     if (span.length == 0) {
         return;
@@ -670,11 +699,6 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
 
     if (warp == kLoadWarp) {
         // ---------------- operands of the blocks -------------------------------------------------------
-        int first_block = 0;  // of this chunk, in the order of the first kernel
-        for (int i = lane; i < sequence; i += 32) {
-            first_block += (chunk_span(begins, i, tokens).length + kBlock - 1) / kBlock;
-        }
-        first_block = static_cast<int>(__reduce_add_sync(0xffffffffu, first_block));
         const __nv_bfloat16* v_rows = qkv + static_cast<size_t>(span.begin) * channels + (2 * kDeltaKeyHeads + head) * kDim;
         for (; n < blocks && ok; ++n) {
             const int slot_of = n & 1;
@@ -1212,7 +1236,6 @@ extern "C" int qwc_delta_chunk_int8(void* state, float* state_scales, const void
                              gate_stride, epsilon};
     return launch_chained(delta_chain_kernel, dim3(v_heads, sequences), dim3(kChainThreads), sizeof(ChainSmem) + 1024, stream,
                           static_cast<int8_t*>(state), state_scales, static_cast<const uint32_t*>(state_slots),
-                          static_cast<const uint32_t*>(continues), static_cast<const uint32_t*>(chunk_begins),
-                          static_cast<const __nv_bfloat16*>(qkv), images, blocks, static_cast<__nv_bfloat16*>(out), tokens,
-                          v_heads, state_capacity, norm, status);
+                          static_cast<const uint32_t*>(continues), static_cast<const __nv_bfloat16*>(qkv), images, blocks,
+                          static_cast<__nv_bfloat16*>(out), v_heads, state_capacity, norm, status);
 }
