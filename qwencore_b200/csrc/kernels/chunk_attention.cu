@@ -30,6 +30,8 @@
 //   warp 12     fetches K and V, rings of three and two stages
 //   warp 13     issues the MMAs (in the pair's first CTA)
 
+#include <algorithm>
+
 #include "chunk.cuh"
 #include "chunk_plan.h"
 #include "tcgen05.cuh"
@@ -1197,7 +1199,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 // Items that were cut: a pair's last item began there and went on with the pairs after it.  A warp per row, eight dims
 // per lane, the pieces in order.
 constexpr int kMergeWarps = 8;
-constexpr int kMergeDepth = 8;  // pieces in flight
+constexpr int kMergeDepth = 4;  // pieces in flight
 
 __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const __grid_constant__ Params p) {
     pdl_launch_dependents();
@@ -1387,6 +1389,7 @@ extern "C" int qwc_paged_attention_chunk_fp8(const void* query, const void* quer
     if (error != cudaSuccess) {
         return error;
     }
-    return launch_chained(chunk_merge_kernel, dim3(setup->pairs, (kItemTokens * kGqaGroup + kMergeWarps - 1) / kMergeWarps),
-                          dim3(kMergeWarps * 32), 0, stream, p);
+    const int item_rows = std::min(kItemTokens, tokens) * kGqaGroup;  // at most
+    return launch_chained(chunk_merge_kernel, dim3(setup->pairs, (item_rows + kMergeWarps - 1) / kMergeWarps), dim3(kMergeWarps * 32),
+                          0, stream, p);
 }
