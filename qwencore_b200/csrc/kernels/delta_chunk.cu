@@ -365,11 +365,15 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
                 if (32 * c <= (t | 31)) {  // (the same for a warp)
                     load_columns(tmem_row + 32 * c, x);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) {
+                    for (int i = 0; i < 32; i += 2) {
                         const int j = 32 * c + i;
-                        const float2 other = sm.log[h][j];
-                        const float decay = exp2_fast((mine.x - other.x) + (mine.y - other.y));
-                        x[i] = j < limit ? strength * decay * x[i] : 0.0f;
+                        const float4 others = *reinterpret_cast<const float4*>(&sm.log[h][j]);
+                        const float2 one = __fadd2_rn(mine, make_float2(-others.x, -others.y));
+                        const float2 two = __fadd2_rn(mine, make_float2(-others.z, -others.w));
+                        const float2 decay = make_float2(exp2_fast(one.x + one.y), exp2_fast(two.x + two.y));
+                        const float2 both = __fmul2_rn(__fmul2_rn(decay, make_float2(strength, strength)), make_float2(x[i], x[i + 1]));
+                        x[i] = j < limit ? both.x : 0.0f;
+                        x[i + 1] = j + 1 < limit ? both.y : 0.0f;
                     }
                 } else {
 #pragma unroll
@@ -486,10 +490,12 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
             for (int i = 0; i < 8; ++i) {
                 const float4 value = *reinterpret_cast<const float4*>(&sm.m.t[row * kPitch + 32 * half + 4 * i]);
                 const float4 strength = *reinterpret_cast<const float4*>(&sm.beta[h][32 * half + 4 * i]);
-                x[4 * i] = value.x * strength.x;
-                x[4 * i + 1] = value.y * strength.y;
-                x[4 * i + 2] = value.z * strength.z;
-                x[4 * i + 3] = value.w * strength.w;
+                const float2 lo = __fmul2_rn(make_float2(value.x, value.y), make_float2(strength.x, strength.y));
+                const float2 hi = __fmul2_rn(make_float2(value.z, value.w), make_float2(strength.z, strength.w));
+                x[4 * i] = lo.x;
+                x[4 * i + 1] = lo.y;
+                x[4 * i + 2] = hi.x;
+                x[4 * i + 3] = hi.y;
             }
         }
         __syncthreads();  // (T has been read)
@@ -519,8 +525,10 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
             const float2 mine = sm.log[h][row], end = sm.log[h][kBlock - 1];
             const float to_end = exp2_fast((end.x - mine.x) + (end.y - mine.y));
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                x[i] *= to_end;
+            for (int i = 0; i < 32; i += 2) {
+                const float2 both = __fmul2_rn(make_float2(x[i], x[i + 1]), make_float2(to_end, to_end));
+                x[i] = both.x;
+                x[i + 1] = both.y;
             }
             ok = wait(&sm.done, (h + 1) & 1, &sm.failed, status);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
