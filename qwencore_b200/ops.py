@@ -9,6 +9,7 @@ here (`data_ptr()`), exactly what `DeviceBuffer<T>` is on the Rust side.
 
 from __future__ import annotations
 
+import ctypes
 import math
 
 import numpy as np
@@ -325,7 +326,8 @@ def cache_copy(table: np.ndarray, pairs: torch.Tensor, count: int) -> None:
     assert table.dtype == np.uint64 and table.ndim == 2 and table.shape[1] == 3 and table.flags.c_contiguous
     assert pairs.numel() >= 2 * count and pairs.element_size() == 4
     _check_here(pairs)
-    abi.check(abi.lib.qwc_cache_copy(table.ctypes.data, table.shape[0], _p(pairs), count, _stream()), "qwc_cache_copy")
+    arrays = ctypes.addressof(ctypes.c_char.from_buffer(table)) if table.flags.writeable else table.ctypes.data
+    abi.check(abi.lib.qwc_cache_copy(arrays, table.shape[0], _p(pairs), count, _stream()), "qwc_cache_copy")
 
 
 def attention_chunk_workspace_bytes() -> int:
