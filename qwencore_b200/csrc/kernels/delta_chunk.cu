@@ -1008,6 +1008,9 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 gain[2 * i + 1] = {__uint_as_float(raw.y << 16), __uint_as_float(raw.y & 0xffff0000u)};
             }
         }
+        const int stride = v_heads * kDim;
+        const int first = (warp - kChainWarps) * 8 + (lane >> 4);  // of a block: this thread's first token
+        __nv_bfloat16* target = out + (static_cast<size_t>(span.begin) + first) * stride + head * kDim + 4 * piece;
         for (; n < blocks; ++n) {
             const uint32_t parity = n & 1;
             ok = wait(&sm.w_full[n & 1], (n >> 1) & 1, failed, status) && wait(&sm.o_done, parity, failed, status);
@@ -1055,7 +1058,6 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 break;
             }
             // rows of the batch: eight tokens of this warp, two at a time
-            const int first = (warp - kChainWarps) * 8 + (lane >> 4);
             float2 o[4][4];
             float inverse[4];
 #pragma unroll
@@ -1106,7 +1108,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                     }
                 }
                 if (token < span.length) {
-                    __nv_bfloat16* to = out + ((static_cast<size_t>(span.begin) + token) * v_heads + head) * kDim + 4 * piece;
+                    __nv_bfloat16* to = target + 2 * i * stride;
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
                         const __nv_bfloat162 lo = __floats2bfloat162_rn(o[i][2 * j].x, o[i][2 * j].y);
@@ -1121,6 +1123,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 mbar_arrive(&sm.rows_free);
                 mbar_arrive(&sm.gate_empty[n & 1]);
             }
+            target += kBlock * stride;
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
