@@ -21,6 +21,7 @@
 // would wait for such a step.  K, Q and V are bf16 as they come; S, X, U' and W are the sum of two bf16, which hold 16 bits,
 // and their products leave out only the lower part times the lower part.
 
+#include <algorithm>
 #include <cstddef>
 
 #include "chunk.cuh"
@@ -43,12 +44,13 @@ struct Images {
     uint8_t* w;     // [block][value head][kWBytes]
     float* decay;   // [block][value head][kBlock]: from the block's start
     int4* order;    // the chunks, longest first: sequence, first row, length, first block
+    int* taken;     // jobs that are not a CTA's first one
 };
 
 inline size_t images_bytes(int blocks, int v_heads) {
     return static_cast<size_t>(blocks) *
            (static_cast<size_t>(kDeltaKeyHeads) * kQkBytes + static_cast<size_t>(v_heads) * (kWBytes + kBlock * sizeof(float))) +
-           kMaxChunkSequences * sizeof(int4);
+           kMaxChunkSequences * sizeof(int4) + sizeof(int);
 }
 
 inline Images images_at(void* workspace, int blocks, int v_heads) {
@@ -57,6 +59,7 @@ inline Images images_at(void* workspace, int blocks, int v_heads) {
     at.w = at.qk + static_cast<size_t>(blocks) * kDeltaKeyHeads * kQkBytes;
     at.decay = reinterpret_cast<float*>(at.w + static_cast<size_t>(blocks) * v_heads * kWBytes);
     at.order = reinterpret_cast<int4*>(at.decay + static_cast<size_t>(blocks) * v_heads * kBlock);
+    at.taken = reinterpret_cast<int*>(at.order + kMaxChunkSequences);
     return at;
 }
 
@@ -263,6 +266,9 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
     }
     if (blockIdx.x == 0 && block == 0) {
         find_order(sm.length, begins, tokens, sequences, images.order);
+        if (tid == 0) {
+            *images.taken = 0;
+        }
     }
     const ChunkTile tile = find_chunk_tile(begins, sequences, tokens, kBlock, block);
     const bool here = tile.sequence >= 0;
@@ -589,6 +595,10 @@ constexpr int kResultColumn = 384;                       // O, U'; then U' split
 constexpr int kUpdateColumn = kResultColumn + kBlock;
 constexpr int kTmemColumns = 512;                        // all of it: the address that the allocation returns is 0
 
+struct ChunkOfJobs {
+    int sequence, begin, length, first_block, slot;
+};
+
 struct ChainSmem {
     uint8_t qk[2][kQkBytes];
     uint8_t w[2][kWBytes];
@@ -596,10 +606,14 @@ struct ChainSmem {
     float rows[kBlock * kDim];          // outputs of a block
     uint8_t gate[2][kBlock * kDim * 2]; // [token][256 bytes]
     float decay[2][kBlock];
-    float peak[2][kDim];
+    float peak[2][2][kDim];             // of every second job, by group
+    ChunkOfJobs chunk[kMaxChunkSequences];  // longest first
     uint64_t qk_full[2], qk_empty[2], w_full[2], w_empty[2], v_full, v_empty;
     uint64_t s_ready, x_done, x_ready, u_done, u_ready, o_done, o_free, s_done;
     uint64_t rows_ready, rows_free, gate_full[2], gate_empty[2];
+    uint64_t chain_met;                 // of the chain's warps
+    uint64_t job_full[2], job_empty[2];
+    int job[2];
     uint32_t tmem_base;
     int failed;
 };
@@ -641,31 +655,13 @@ __device__ __forceinline__ void tmem_store_split(uint32_t upper_at, uint32_t low
 __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
     int8_t* __restrict__ state, float* __restrict__ state_scales, const uint32_t* __restrict__ state_slots,
     const uint32_t* __restrict__ continues, const __nv_bfloat16* __restrict__ qkv, const Images images, int images_blocks,
-    __nv_bfloat16* __restrict__ out, int v_heads, int state_capacity, const OutputNorm norm, int* status) {
+    __nv_bfloat16* __restrict__ out, int sequences, int v_heads, int state_capacity, const OutputNorm norm, int* status) {
     extern __shared__ unsigned char smem_raw[];
     ChainSmem& sm = *reinterpret_cast<ChainSmem*>(smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u));
     const int lane = threadIdx.x & 31;
     const int warp = threadIdx.x >> 5;
-    const int head = blockIdx.x;
-    const int key_head = head / (v_heads / kDeltaKeyHeads);
     const int channels = (2 * kDeltaKeyHeads + v_heads) * kDim;
     pdl_wait();
-    const int4 chosen = __ldcg(images.order + blockIdx.y);
-    const int sequence = chosen.x, first_block = chosen.w;
-    const ChunkSpan span = {chosen.y, chosen.z};
-    const uint32_t slot = __ldcg(state_slots + sequence);
-    if (span.length == 0) {
-        return;
-    }
-    if (slot >= static_cast<uint32_t>(state_capacity)) {
-        // a slot beyond the pool: nothing of this chunk is read or written, the host learns of it through the status
-        // word (the whole CTA takes this branch)
-        if (threadIdx.x == 0) {
-            atomicCAS(status, 0, kStatusStateSlotRange);
-        }
-        return;
-    }
-    const int blocks = (span.length + kBlock - 1) / kBlock;
     if (warp == kLoadWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem_base)),
                      "r"(kTmemColumns)
@@ -673,13 +669,28 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     }
-    if (threadIdx.x == 0) {
+    bool any = false;  // rows of the chunk that this thread looks at
+    if (threadIdx.x < sequences) {
+        const int4 chunk = __ldcg(images.order + threadIdx.x);
+        any = chunk.z > 0;
+        const uint32_t slot = __ldcg(state_slots + chunk.x);
+        const bool there = slot < static_cast<uint32_t>(state_capacity);
+        if (!there && chunk.z > 0) {
+            // a slot beyond the pool: nothing of this chunk is read or written, the host learns of it through the status
+            // word
+            atomicCAS(status, 0, kStatusStateSlotRange);
+        }
+        sm.chunk[threadIdx.x] = {chunk.x, chunk.y, there ? chunk.z : 0, chunk.w, static_cast<int>(slot)};
+    }
+    if (threadIdx.x == kMmaWarp * 32) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm.qk_full[i], 1);
             mbar_init(&sm.qk_empty[i], 1);
             mbar_init(&sm.w_full[i], 1);
             mbar_init(&sm.w_empty[i], 1 + kOutputWarps);  // the MMAs, and who reads the decays
             mbar_init(&sm.gate_full[i], 1);
+            mbar_init(&sm.job_full[i], 1);
+            mbar_init(&sm.job_empty[i], kChainWarps + kOutputWarps + 2);
             mbar_init(&sm.gate_empty[i], kOutputWarps);
         }
         mbar_init(&sm.s_ready, kChainWarps);
@@ -694,85 +705,139 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
         mbar_init(&sm.rows_free, kOutputWarps);
         mbar_init(&sm.v_full, 1);
         mbar_init(&sm.v_empty, 1);
+        mbar_init(&sm.chain_met, kChainWarps);
         sm.failed = 0;
         mbar_fence_init();
     }
     fence_proxy_async();
-    __syncthreads();
+    const int chunks = __syncthreads_count(any ? 1 : 0);  // the first ones
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     pdl_launch_dependents();  // (this CTA has its tensor memory)
     int* const failed = &sm.failed;
     bool ok = true;
     int n = 0;  // blocks so far
+    // A job is a chunk with a value head, the longest first.  A CTA's first one is its own, then whoever is done takes the next;
+    // the warp that loads takes it, and says which to the others.  -1: there is none.  (40 chunks of 1000 tokens in all: 192 us
+    // with a CTA for each job, 174 so; 128 chunks of 4000: 592 and 534; one chunk of 4096: 225 and 226.)
+    const int jobs = chunks * v_heads;
+    int round = 0;
+    const auto next_job = [&]() {
+        const int slot = round & 1;
+        int job = -1;
+        if (wait(&sm.job_full[slot], (round >> 1) & 1, failed, status)) {
+            job = sm.job[slot];
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.job_empty[slot]);
+            }
+        } else {
+            ok = false;
+        }
+        ++round;
+        return job;
+    };
 
     if (warp == kLoadWarp) {
         // ---------------- operands of the blocks -------------------------------------------------------
-        const __nv_bfloat16* v_rows = qkv + static_cast<size_t>(span.begin) * channels + (2 * kDeltaKeyHeads + head) * kDim;
-        for (; n < blocks && ok; ++n) {
-            const int slot_of = n & 1;
-            const uint32_t parity = ((n >> 1) & 1) ^ 1;
-            // (chunks that overlap have more blocks than there is room for: what they get is nobody's, but it is there)
-            const size_t block = static_cast<size_t>(min(first_block + n, images_blocks - 1));
-            ok = wait(&sm.w_empty[slot_of], parity, failed, status);
+        for (int job = blockIdx.x; ok; ++round) {
+            const auto take = [&]() {
+                const int taken = lane == 0 ? static_cast<int>(gridDim.x) + atomicAdd(images.taken, 1) : 0;
+                return __shfl_sync(0xffffffffu, taken, 0);
+            };
+            while (job < jobs && sm.chunk[job / v_heads].length == 0) {
+                job = take();  // (a chunk whose slot is beyond the pool)
+            }
+            const bool there = job < jobs;
+            ok = wait(&sm.job_empty[round & 1], ((round >> 1) & 1) ^ 1, failed, status);
             if (ok && lane == 0) {
-                mbar_arrive_expect_tx(&sm.w_full[slot_of], kWBytes + kBlock * 4);
-                bulk_g2s(sm.w[slot_of], images.w + (block * v_heads + head) * kWBytes, kWBytes, &sm.w_full[slot_of]);
-                bulk_g2s(sm.decay[slot_of], images.decay + (block * v_heads + head) * kBlock, kBlock * 4, &sm.w_full[slot_of]);
+                sm.job[round & 1] = there ? job : -1;
+                mbar_arrive(&sm.job_full[round & 1]);
             }
             __syncwarp();
-            ok = ok && wait(&sm.v_empty, (n & 1) ^ 1, failed, status);
-            if (ok) {
-                // rows of v, zeros behind the chunk: sixteen lanes to a row
-                const int piece = lane & 15;
-#pragma unroll 8
-                for (int i = 0; i < kBlock / 2; ++i) {
-                    const int t = 2 * i + (lane >> 4);
-                    const int token = n * kBlock + t;
-                    const bool live = token < span.length;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                     smem_u32(sm.v + (piece >> 3) * (kVBytes / 2) + swizzled(t, piece & 7))),
-                                 "l"(v_rows + static_cast<size_t>(live ? token : 0) * channels + 8 * piece), "r"(live ? 16 : 0)
-                                 : "memory");
+            if (!ok || !there) {
+                break;
+            }
+            const ChunkOfJobs& chunk = sm.chunk[job / v_heads];
+            const int head = job % v_heads;
+            const int length = chunk.length, first_block = chunk.first_block;
+            const int key_head = head / (v_heads / kDeltaKeyHeads);
+            const __nv_bfloat16* v_rows = qkv + static_cast<size_t>(chunk.begin) * channels + (2 * kDeltaKeyHeads + head) * kDim;
+            const int blocks = (length + kBlock - 1) / kBlock;
+            for (int at = 0; at < blocks && ok; ++at, ++n) {
+                const int slot_of = n & 1;
+                const uint32_t parity = ((n >> 1) & 1) ^ 1;
+                // (chunks that overlap have more blocks than there is room for: what they get is nobody's, but it is there)
+                const size_t block = static_cast<size_t>(min(first_block + at, images_blocks - 1));
+                ok = wait(&sm.w_empty[slot_of], parity, failed, status);
+                if (ok && lane == 0) {
+                    mbar_arrive_expect_tx(&sm.w_full[slot_of], kWBytes + kBlock * 4);
+                    bulk_g2s(sm.w[slot_of], images.w + (block * v_heads + head) * kWBytes, kWBytes, &sm.w_full[slot_of]);
+                    bulk_g2s(sm.decay[slot_of], images.decay + (block * v_heads + head) * kBlock, kBlock * 4, &sm.w_full[slot_of]);
                 }
+                __syncwarp();
+                ok = ok && wait(&sm.v_empty, (n & 1) ^ 1, failed, status);
+                if (ok) {
+                    // rows of v, zeros behind the chunk: sixteen lanes to a row
+                    const int piece = lane & 15;
+#pragma unroll 8
+                    for (int i = 0; i < kBlock / 2; ++i) {
+                        const int t = 2 * i + (lane >> 4);
+                        const int token = at * kBlock + t;
+                        const bool live = token < length;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                                         smem_u32(sm.v + (piece >> 3) * (kVBytes / 2) + swizzled(t, piece & 7))),
+                                     "l"(v_rows + static_cast<size_t>(live ? token : 0) * channels + 8 * piece), "r"(live ? 16 : 0)
+                                     : "memory");
+                    }
+                }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                ok = ok && wait(&sm.qk_empty[slot_of], parity, failed, status);
+                if (ok && lane == 0) {
+                    mbar_arrive_expect_tx(&sm.qk_full[slot_of], kQkBytes);
+                    bulk_g2s(sm.qk[slot_of], images.qk + (block * kDeltaKeyHeads + key_head) * kQkBytes, kQkBytes, &sm.qk_full[slot_of]);
+                }
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                fence_proxy_async();
+                __syncwarp();
+                if (ok && lane == 0) {
+                    mbar_arrive(&sm.v_full);
+                }
+                __syncwarp();
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            ok = ok && wait(&sm.qk_empty[slot_of], parity, failed, status);
-            if (ok && lane == 0) {
-                mbar_arrive_expect_tx(&sm.qk_full[slot_of], kQkBytes);
-                bulk_g2s(sm.qk[slot_of], images.qk + (block * kDeltaKeyHeads + key_head) * kQkBytes, kQkBytes, &sm.qk_full[slot_of]);
-            }
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            fence_proxy_async();
-            __syncwarp();
-            if (ok && lane == 0) {
-                mbar_arrive(&sm.v_full);
-            }
-            __syncwarp();
+            job = take();  // (not before: who has a long job would have the next one too)
         }
     } else if (warp == kGateWarp) {
         // ---------------- gates of the blocks' rows ---------------------------------------------------------
         const int piece = lane & 15;
-        const __nv_bfloat16* rows = norm.gate + static_cast<size_t>(span.begin) * norm.gate_stride + head * kDim + 8 * piece;
-        for (; norm.gate != nullptr && n < blocks && ok; ++n) {
-            ok = wait(&sm.gate_empty[n & 1], ((n >> 1) & 1) ^ 1, failed, status);
-            if (ok) {
+        for (int job = next_job(); job >= 0; job = ok ? next_job() : -1) {
+            if (norm.gate == nullptr) {
+                continue;
+            }
+            const ChunkOfJobs& chunk = sm.chunk[job / v_heads];
+            const int head = job % v_heads, length = chunk.length;
+            const __nv_bfloat16* rows = norm.gate + static_cast<size_t>(chunk.begin) * norm.gate_stride + head * kDim + 8 * piece;
+            const int blocks = (length + kBlock - 1) / kBlock;
+            for (int at = 0; at < blocks && ok; ++at, ++n) {
+                ok = wait(&sm.gate_empty[n & 1], ((n >> 1) & 1) ^ 1, failed, status);
+                if (ok) {
 #pragma unroll 4
-                for (int i = 0; i < kBlock / 2; ++i) {
-                    const int t = 2 * i + (lane >> 4);
-                    const int token = n * kBlock + t;
-                    const bool live = token < span.length;
-                    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(sm.gate[n & 1] + t * (kDim * 2) + 16 * piece)),
-                                 "l"(rows + static_cast<size_t>(live ? token : 0) * norm.gate_stride), "r"(live ? 16 : 0)
-                                 : "memory");
+                    for (int i = 0; i < kBlock / 2; ++i) {
+                        const int t = 2 * i + (lane >> 4);
+                        const int token = at * kBlock + t;
+                        const bool live = token < length;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(sm.gate[n & 1] + t * (kDim * 2) + 16 * piece)),
+                                     "l"(rows + static_cast<size_t>(live ? token : 0) * norm.gate_stride), "r"(live ? 16 : 0)
+                                     : "memory");
+                    }
                 }
+                asm volatile("cp.async.commit_group;" ::: "memory");
+                asm volatile("cp.async.wait_group 0;" ::: "memory");
+                __syncwarp();
+                if (ok && lane == 0) {
+                    mbar_arrive(&sm.gate_full[n & 1]);
+                }
+                __syncwarp();
             }
-            asm volatile("cp.async.commit_group;" ::: "memory");
-            asm volatile("cp.async.wait_group 0;" ::: "memory");
-            __syncwarp();
-            if (ok && lane == 0) {
-                mbar_arrive(&sm.gate_full[n & 1]);
-            }
-            __syncwarp();
         }
     } else if (warp == kMmaWarp) {
         // ---------------- tensor-core issue ------------------------------------------------------------
@@ -802,8 +867,13 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             __syncwarp();
             return true;
         };
-        ok = issue_values(0);
-        for (; n < blocks && ok; ++n) {
+        const auto next_blocks = [&]() {
+            const int job = next_job();
+            return job < 0 ? 0 : (sm.chunk[job / v_heads].length + kBlock - 1) / kBlock;
+        };
+        int end = next_blocks();  // of the blocks of the job at hand
+        ok = ok && (end == 0 || issue_values(0));
+        for (; n < end && ok; ++n) {
             const uint32_t parity = n & 1;
             const uint32_t qk_offset = (n & 1) * (kQkBytes >> 4);
             const uint32_t qk_base = qk_operand + qk_offset, w_base = w_operand + (n & 1) * (kWBytes >> 4);
@@ -871,7 +941,10 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 umma_commit(&sm.qk_empty[n & 1]);
             }
             __syncwarp();
-            if (n + 1 < blocks) {
+            if (n + 1 == end) {
+                end += next_blocks();
+            }
+            if (ok && n + 1 < end) {
                 ok = issue_values(n + 1);
             }
         }
@@ -884,114 +957,153 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
         const uint32_t held = tmem + kStateColumn + group * 64;                // 64 key dims of the row
         const uint32_t upper = tmem + kSplitColumn + group * 32, lower = upper + 64;
         const uint32_t x_at = tmem + kKeyColumn + group * 32, u_at = tmem + kUpdateColumn + group * 32;
-        const size_t state_row = (static_cast<size_t>(slot) * v_heads + head) * kDim + row;
-        {
-            const bool holds = continues == nullptr || __ldcg(continues + sequence) != 0;
-            const float scale = holds ? state_scales[state_row] : 0.0f;
-            const uint4* codes = reinterpret_cast<const uint4*>(state + state_row * kDim + group * 64);
+        int done = 0;  // jobs
+        for (int job = next_job(); job >= 0; job = next_job()) {
+            const ChunkOfJobs& chunk = sm.chunk[job / v_heads];
+            const int blocks = (chunk.length + kBlock - 1) / kBlock;
+            const size_t state_row = (static_cast<size_t>(chunk.slot) * v_heads + job % v_heads) * kDim + row;
+            {
+                const bool holds = continues == nullptr || __ldcg(continues + chunk.sequence) != 0;
+                const float scale = holds ? state_scales[state_row] : 0.0f;
+                const uint4* codes = reinterpret_cast<const uint4*>(state + state_row * kDim + group * 64);
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                float s[32];
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint4 raw = codes[2 * c + i];
-                    const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        s[16 * i + j] = holds ? static_cast<float>(static_cast<int8_t>(words[j >> 2] >> (8 * (j & 3)))) * scale : 0.0f;
-                    }
-                }
-                tmem_store_columns(held + 32 * c, s);
-                tmem_store_split(upper + 16 * c, lower + 16 * c, s);
-            }
-        }
-        tmem_store_wait();
-        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-        __syncwarp();
-        if (lane == 0) {
-            mbar_arrive(&sm.s_ready);
-        }
-        for (; n < blocks; ++n) {
-            const uint32_t parity = n & 1;
-            const float* decay = sm.decay[n & 1];
-            float x[32];
-            ok = wait(&sm.w_full[n & 1], (n >> 1) & 1, failed, status) && wait(&sm.x_done, parity, failed, status);
-            if (!ok) {
-                break;
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            load_columns(x_at, x);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float4 g = *reinterpret_cast<const float4*>(decay + group * 32 + 4 * i);
-                x[4 * i] *= -g.x;
-                x[4 * i + 1] *= -g.y;
-                x[4 * i + 2] *= -g.z;
-                x[4 * i + 3] *= -g.w;
-            }
-            tmem_store_split(x_at, x_at + 16, x);
-            const float end = decay[kBlock - 1];  // (before x_ready: behind it the place may get the block after next)
-            tmem_store_wait();
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&sm.x_ready);
-            }
-            // the state decays while U' is made
-#pragma unroll 1
-            for (int c = 0; c < 2; ++c) {
-                load_columns(held + 32 * c, x);
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const float2 both = __fmul2_rn({x[i], x[i + 1]}, {end, end});
-                    x[i] = both.x;
-                    x[i + 1] = both.y;
-                }
-                tmem_store_columns(held + 32 * c, x);
-            }
-            ok = wait(&sm.u_done, parity, failed, status);
-            if (!ok) {
-                break;
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            load_columns(u_at, x);
-            tmem_store_split(u_at, u_at + 16, x);
-            tmem_store_wait();
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&sm.u_ready);
-            }
-            ok = wait(&sm.s_done, parity, failed, status);
-            if (!ok) {
-                break;
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            if (n + 1 < blocks) {
-#pragma unroll 1
                 for (int c = 0; c < 2; ++c) {
-                    load_columns(held + 32 * c, x);
-                    tmem_store_split(upper + 16 * c, lower + 16 * c, x);
+                    float s[32];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint4 raw = codes[2 * c + i];
+                        const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            s[16 * i + j] = holds ? static_cast<float>(static_cast<int8_t>(words[j >> 2] >> (8 * (j & 3)))) * scale : 0.0f;
+                        }
+                    }
+                    tmem_store_columns(held + 32 * c, s);
+                    tmem_store_split(upper + 16 * c, lower + 16 * c, s);
                 }
+            }
+            tmem_store_wait();
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.s_ready);
+            }
+            for (int at = 0; at < blocks; ++at, ++n) {
+                const uint32_t parity = n & 1;
+                const float* decay = sm.decay[n & 1];
+                float x[32];
+                ok = wait(&sm.w_full[n & 1], (n >> 1) & 1, failed, status) && wait(&sm.x_done, parity, failed, status);
+                if (!ok) {
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                load_columns(x_at, x);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float4 g = *reinterpret_cast<const float4*>(decay + group * 32 + 4 * i);
+                    x[4 * i] *= -g.x;
+                    x[4 * i + 1] *= -g.y;
+                    x[4 * i + 2] *= -g.z;
+                    x[4 * i + 3] *= -g.w;
+                }
+                tmem_store_split(x_at, x_at + 16, x);
+                const float end = decay[kBlock - 1];  // (before x_ready: behind it the place may get the block after next)
                 tmem_store_wait();
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) {
-                    mbar_arrive(&sm.s_ready);
+                    mbar_arrive(&sm.x_ready);
+                }
+                // the state decays while U' is made
+#pragma unroll 1
+                for (int c = 0; c < 2; ++c) {
+                    load_columns(held + 32 * c, x);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float2 both = __fmul2_rn({x[i], x[i + 1]}, {end, end});
+                        x[i] = both.x;
+                        x[i + 1] = both.y;
+                    }
+                    tmem_store_columns(held + 32 * c, x);
+                }
+                ok = wait(&sm.u_done, parity, failed, status);
+                if (!ok) {
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                load_columns(u_at, x);
+                tmem_store_split(u_at, u_at + 16, x);
+                tmem_store_wait();
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&sm.u_ready);
+                }
+                ok = wait(&sm.s_done, parity, failed, status);
+                if (!ok) {
+                    break;
+                }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                if (at + 1 < blocks) {
+#pragma unroll 1
+                    for (int c = 0; c < 2; ++c) {
+                        load_columns(held + 32 * c, x);
+                        tmem_store_split(upper + 16 * c, lower + 16 * c, x);
+                    }
+                    tmem_store_wait();
+                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(&sm.s_ready);
+                    }
                 }
             }
-        }
-        float peak = 0.0f;
+            if (!ok) {
+                break;
+            }
+            // the state's eight bits, 64 of a row
+            float peak = 0.0f;
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+                float s[32];
+                load_columns(held + 32 * c, s);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            float s[32];
-            load_columns(held + 32 * c, s);
+                for (int i = 0; i < 32; ++i) {
+                    peak = fmaxf(peak, fabsf(s[i]));
+                }
+            }
+            sm.peak[done & 1][group][row] = peak;
+            __syncwarp();
+            if (lane == 0) {
+                mbar_arrive(&sm.chain_met);
+            }
+            // (bounded as everything: a warp that has given up does not come)
+            ok = wait(&sm.chain_met, done & 1, failed, status);
+            if (!ok) {
+                break;
+            }
+            peak = fmaxf(peak, sm.peak[done & 1][group ^ 1][row]);
+            ++done;
+            const float inverse = peak == 0.0f ? 0.0f : __fdiv_rn(127.0f, peak);
+            uint4* codes = reinterpret_cast<uint4*>(state + state_row * kDim + group * 64);
+#pragma unroll 1
+            for (int c = 0; c < 2; ++c) {
+                float s[32];
+                load_columns(held + 32 * c, s);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                peak = fmaxf(peak, fabsf(s[i]));
+                for (int i = 0; i < 2; ++i) {
+                    uint32_t words[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        words[j >> 2] |= (static_cast<uint32_t>(__float2int_rn(s[16 * i + j] * inverse)) & 0xffu) << (8 * (j & 3));
+                    }
+                    codes[2 * c + i] = make_uint4(words[0], words[1], words[2], words[3]);
+                }
+            }
+            if (group == 0) {
+                state_scales[state_row] = __fmul_rn(peak, 1.0f / 127.0f);
             }
         }
-        sm.peak[group][row] = peak;
     } else {
         // ---------------- outputs ----------------------------------------------------------------------
         const int quarter = warp & 3;
@@ -1010,120 +1122,122 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
         }
         const int stride = v_heads * kDim;
         const int first = (warp - kChainWarps) * 8 + (lane >> 4);  // of a block: this thread's first token
-        __nv_bfloat16* target = out + (static_cast<size_t>(span.begin) + first) * stride + head * kDim + 4 * piece;
-        for (; n < blocks; ++n) {
-            const uint32_t parity = n & 1;
-            ok = wait(&sm.w_full[n & 1], (n >> 1) & 1, failed, status) && wait(&sm.o_done, parity, failed, status);
-            if (!ok) {
-                break;
-            }
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            float x[32];
-            {
-                float y[32];
-                load_columns(tmem + kResultColumn, x);
-                load_columns(tmem + kQueryColumn, y);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float4 g = *reinterpret_cast<const float4*>(&sm.decay[n & 1][group * 32 + 4 * i]);
-                    const float2 lo = __ffma2_rn({g.x, g.y}, {y[4 * i], y[4 * i + 1]}, {x[4 * i], x[4 * i + 1]});
-                    const float2 hi = __ffma2_rn({g.z, g.w}, {y[4 * i + 2], y[4 * i + 3]}, {x[4 * i + 2], x[4 * i + 3]});
-                    x[4 * i] = lo.x;
-                    x[4 * i + 1] = lo.y;
-                    x[4 * i + 2] = hi.x;
-                    x[4 * i + 3] = hi.y;
+        for (int job = next_job(); job >= 0; job = ok ? next_job() : -1) {
+            const ChunkOfJobs& chunk = sm.chunk[job / v_heads];
+            __nv_bfloat16* target = out + (static_cast<size_t>(chunk.begin) + first) * stride + job % v_heads * kDim + 4 * piece;
+            for (int left = chunk.length; left > 0; left -= kBlock, ++n) {
+                const uint32_t parity = n & 1;
+                ok = wait(&sm.w_full[n & 1], (n >> 1) & 1, failed, status) && wait(&sm.o_done, parity, failed, status);
+                if (!ok) {
+                    break;
                 }
-            }
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&sm.o_free);
-                mbar_arrive(&sm.w_empty[n & 1]);
-            }
-            ok = wait(&sm.rows_free, parity ^ 1, failed, status);
-            if (!ok) {
-                break;
-            }
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                float x[32];
+                {
+                    float y[32];
+                    load_columns(tmem + kResultColumn, x);
+                    load_columns(tmem + kQueryColumn, y);
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                sm.rows[(group * 32 + i) * kDim + row] = x[i];
-            }
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&sm.rows_ready);
-            }
-            ok = wait(&sm.rows_ready, parity, failed, status) &&
-                 (norm.gate == nullptr || wait(&sm.gate_full[n & 1], (n >> 1) & 1, failed, status));
-            if (!ok) {
-                break;
-            }
-            // rows of the batch: eight tokens of this warp, two at a time
-            float2 o[4][4];
-            float inverse[4];
+                    for (int i = 0; i < 8; ++i) {
+                        const float4 g = *reinterpret_cast<const float4*>(&sm.decay[n & 1][group * 32 + 4 * i]);
+                        const float2 lo = __ffma2_rn({g.x, g.y}, {y[4 * i], y[4 * i + 1]}, {x[4 * i], x[4 * i + 1]});
+                        const float2 hi = __ffma2_rn({g.z, g.w}, {y[4 * i + 2], y[4 * i + 3]}, {x[4 * i + 2], x[4 * i + 3]});
+                        x[4 * i] = lo.x;
+                        x[4 * i + 1] = lo.y;
+                        x[4 * i + 2] = hi.x;
+                        x[4 * i + 3] = hi.y;
+                    }
+                }
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&sm.o_free);
+                    mbar_arrive(&sm.w_empty[n & 1]);
+                }
+                ok = wait(&sm.rows_free, parity ^ 1, failed, status);
+                if (!ok) {
+                    break;
+                }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float4 lo = *reinterpret_cast<const float4*>(&sm.rows[(first + 2 * i) * kDim + 4 * piece]);
-                const float4 hi = *reinterpret_cast<const float4*>(&sm.rows[(first + 2 * i) * kDim + 64 + 4 * piece]);
-                o[i][0] = {lo.x, lo.y};
-                o[i][1] = {lo.z, lo.w};
-                o[i][2] = {hi.x, hi.y};
-                o[i][3] = {hi.z, hi.w};
-            }
-            if (norm.gate != nullptr) {
-                // (the four sums go through the warp side by side)
+                for (int i = 0; i < 32; ++i) {
+                    sm.rows[(group * 32 + i) * kDim + row] = x[i];
+                }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&sm.rows_ready);
+                }
+                ok = wait(&sm.rows_ready, parity, failed, status) &&
+                     (norm.gate == nullptr || wait(&sm.gate_full[n & 1], (n >> 1) & 1, failed, status));
+                if (!ok) {
+                    break;
+                }
+                // rows of the batch: eight tokens of this warp, two at a time
+                float2 o[4][4];
+                float inverse[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    float2 sums = __fmul2_rn(o[i][0], o[i][0]);
-#pragma unroll
-                    for (int j = 1; j < 4; ++j) {
-                        sums = __ffma2_rn(o[i][j], o[i][j], sums);
-                    }
-                    inverse[i] = sums.x + sums.y;
+                    const float4 lo = *reinterpret_cast<const float4*>(&sm.rows[(first + 2 * i) * kDim + 4 * piece]);
+                    const float4 hi = *reinterpret_cast<const float4*>(&sm.rows[(first + 2 * i) * kDim + 64 + 4 * piece]);
+                    o[i][0] = {lo.x, lo.y};
+                    o[i][1] = {lo.z, lo.w};
+                    o[i][2] = {hi.x, hi.y};
+                    o[i][3] = {hi.z, hi.w};
                 }
-#pragma unroll
-                for (int offset = 1; offset < 16; offset <<= 1) {
+                if (norm.gate != nullptr) {
+                    // (the four sums go through the warp side by side)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        inverse[i] += __shfl_xor_sync(0xffffffffu, inverse[i], offset);
+                        float2 sums = __fmul2_rn(o[i][0], o[i][0]);
+#pragma unroll
+                        for (int j = 1; j < 4; ++j) {
+                            sums = __ffma2_rn(o[i][j], o[i][j], sums);
+                        }
+                        inverse[i] = sums.x + sums.y;
+                    }
+#pragma unroll
+                    for (int offset = 1; offset < 16; offset <<= 1) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            inverse[i] += __shfl_xor_sync(0xffffffffu, inverse[i], offset);
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        inverse[i] = rsqrtf(inverse[i] / static_cast<float>(kDim) + norm.epsilon);
                     }
                 }
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    inverse[i] = rsqrtf(inverse[i] / static_cast<float>(kDim) + norm.epsilon);
-                }
-            }
+                    const int t = first + 2 * i;
+                    if (norm.gate != nullptr) {
+                        const uint2 gate_lo = *reinterpret_cast<const uint2*>(sm.gate[n & 1] + t * (kDim * 2) + 8 * piece);
+                        const uint2 gate_hi = *reinterpret_cast<const uint2*>(sm.gate[n & 1] + t * (kDim * 2) + kDim + 8 * piece);
+                        const uint32_t words[4] = {gate_lo.x, gate_lo.y, gate_hi.x, gate_hi.y};
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int t = first + 2 * i;
-                const int token = n * kBlock + t;
-                if (norm.gate != nullptr) {
-                    const uint2 gate_lo = *reinterpret_cast<const uint2*>(sm.gate[n & 1] + t * (kDim * 2) + 8 * piece);
-                    const uint2 gate_hi = *reinterpret_cast<const uint2*>(sm.gate[n & 1] + t * (kDim * 2) + kDim + 8 * piece);
-                    const uint32_t words[4] = {gate_lo.x, gate_lo.y, gate_hi.x, gate_hi.y};
+                        for (int j = 0; j < 4; ++j) {
+                            const float2 z = {__uint_as_float(words[j] << 16), __uint_as_float(words[j] & 0xffff0000u)};
+                            const float2 silu = __fmul2_rn(z, sigmoid_pair(z));
+                            o[i][j] = __fmul2_rn(__fmul2_rn(o[i][j], {inverse[i], inverse[i]}), __fmul2_rn(gain[j], silu));
+                        }
+                    }
+                    if (t < left) {
+                        __nv_bfloat16* to = target + 2 * i * stride;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float2 z = {__uint_as_float(words[j] << 16), __uint_as_float(words[j] & 0xffff0000u)};
-                        const float2 silu = __fmul2_rn(z, sigmoid_pair(z));
-                        o[i][j] = __fmul2_rn(__fmul2_rn(o[i][j], {inverse[i], inverse[i]}), __fmul2_rn(gain[j], silu));
+                        for (int j = 0; j < 2; ++j) {
+                            const __nv_bfloat162 lo = __floats2bfloat162_rn(o[i][2 * j].x, o[i][2 * j].y);
+                            const __nv_bfloat162 hi = __floats2bfloat162_rn(o[i][2 * j + 1].x, o[i][2 * j + 1].y);
+                            *reinterpret_cast<uint2*>(to + 64 * j) =
+                                make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+                        }
                     }
                 }
-                if (token < span.length) {
-                    __nv_bfloat16* to = target + 2 * i * stride;
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        const __nv_bfloat162 lo = __floats2bfloat162_rn(o[i][2 * j].x, o[i][2 * j].y);
-                        const __nv_bfloat162 hi = __floats2bfloat162_rn(o[i][2 * j + 1].x, o[i][2 * j + 1].y);
-                        *reinterpret_cast<uint2*>(to + 64 * j) =
-                            make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-                    }
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&sm.rows_free);
+                    mbar_arrive(&sm.gate_empty[n & 1]);
                 }
+                target += kBlock * stride;
             }
-            __syncwarp();
-            if (lane == 0) {
-                mbar_arrive(&sm.rows_free);
-                mbar_arrive(&sm.gate_empty[n & 1]);
-            }
-            target += kBlock * stride;
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1136,7 +1250,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             }
         };
         if (warp == kLoadWarp) {
-            for (int i = n > 2 ? n - 2 : 0; i <= n && i < blocks; ++i) {
+            for (int i = n > 2 ? n - 2 : 0; i <= n; ++i) {
                 arrived(&sm.qk_full[i & 1], (i >> 1) & 1);
                 arrived(&sm.w_full[i & 1], (i >> 1) & 1);
             }
@@ -1144,32 +1258,6 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             arrived(&sm.v_empty, n & 1);
             arrived(&sm.o_done, n & 1);
             arrived(&sm.s_done, n & 1);
-        }
-    } else if (warp < kChainWarps) {
-        // the state's eight bits: 64 of a row
-        const int quarter = warp & 3, group = warp >> 2;
-        const int row = quarter * 32 + lane;
-        const uint32_t held = (static_cast<uint32_t>(quarter * 32) << 16) + kStateColumn + group * 64;
-        const size_t state_row = (static_cast<size_t>(slot) * v_heads + head) * kDim + row;
-        const float peak = fmaxf(sm.peak[0][row], sm.peak[1][row]);
-        const float inverse = peak == 0.0f ? 0.0f : __fdiv_rn(127.0f, peak);
-        uint4* codes = reinterpret_cast<uint4*>(state + state_row * kDim + group * 64);
-#pragma unroll
-        for (int c = 0; c < 2; ++c) {
-            float s[32];
-            load_columns(held + 32 * c, s);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                uint32_t words[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
-                for (int j = 0; j < 16; ++j) {
-                    words[j >> 2] |= (static_cast<uint32_t>(__float2int_rn(s[16 * i + j] * inverse)) & 0xffu) << (8 * (j & 3));
-                }
-                codes[2 * c + i] = make_uint4(words[0], words[1], words[2], words[3]);
-            }
-        }
-        if (group == 0) {
-            state_scales[state_row] = __fmul_rn(peak, 1.0f / 127.0f);
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -1217,21 +1305,33 @@ extern "C" int qwc_delta_chunk_int8(void* state, float* state_scales, const void
     if (status == nullptr) {
         return cudaErrorInvalidValue;
     }
-    static PerDevice<cudaError_t> per_device;
-    const cudaError_t* setup = per_device.get([]() {
-        cudaError_t error = cudaFuncSetAttribute(delta_factor_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                                 static_cast<int>(sizeof(FactorSmem)) + 1024);
-        if (error == cudaSuccess) {
-            error = cudaFuncSetAttribute(delta_chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         static_cast<int>(sizeof(ChainSmem)) + 1024);
+    struct Setup {
+        cudaError_t error;
+        int sms;
+    };
+    static PerDevice<Setup> per_device;
+    const Setup* setup = per_device.get([]() {
+        Setup found = {cudaSuccess, 0};
+        int device = 0;
+        found.error = cudaFuncSetAttribute(delta_factor_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                           static_cast<int>(sizeof(FactorSmem)) + 1024);
+        if (found.error == cudaSuccess) {
+            found.error = cudaFuncSetAttribute(delta_chain_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                               static_cast<int>(sizeof(ChainSmem)) + 1024);
         }
-        return error;
+        if (found.error == cudaSuccess) {
+            found.error = cudaGetDevice(&device);
+        }
+        if (found.error == cudaSuccess) {
+            found.error = cudaDeviceGetAttribute(&found.sms, cudaDevAttrMultiProcessorCount, device);
+        }
+        return found;
     });
     if (setup == nullptr) {
         return cudaErrorInvalidDevice;
     }
-    if (*setup != cudaSuccess) {
-        return *setup;
+    if (setup->error != cudaSuccess) {
+        return setup->error;
     }
     const int blocks = most_chunk_tiles(tokens, sequences, kBlock);
     const Images images = images_at(workspace, blocks, v_heads);
@@ -1245,8 +1345,8 @@ extern "C" int qwc_delta_chunk_int8(void* state, float* state_scales, const void
     }
     const OutputNorm norm = {static_cast<const __nv_bfloat16*>(gate), static_cast<const __nv_bfloat16*>(norm_weight),
                              gate_stride, epsilon};
-    return launch_chained(delta_chain_kernel, dim3(v_heads, sequences), dim3(kChainThreads), sizeof(ChainSmem) + 1024, stream,
+    return launch_chained(delta_chain_kernel, dim3(std::min(v_heads * sequences, setup->sms)), dim3(kChainThreads), sizeof(ChainSmem) + 1024, stream,
                           static_cast<int8_t*>(state), state_scales, static_cast<const uint32_t*>(state_slots),
                           static_cast<const uint32_t*>(continues), static_cast<const __nv_bfloat16*>(qkv), images, blocks,
-                          static_cast<__nv_bfloat16*>(out), v_heads, state_capacity, norm, status);
+                          static_cast<__nv_bfloat16*>(out), sequences, v_heads, state_capacity, norm, status);
 }
