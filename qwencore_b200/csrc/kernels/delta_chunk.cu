@@ -759,6 +759,11 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             }
             const ChunkOfJobs& chunk = sm.chunk[job / v_heads];
             const int head = job % v_heads;
+            if (lane == 0) {
+                // (the chain asks for the state when it is done with the job before)
+                bulk_prefetch_l2(state + (static_cast<size_t>(chunk.slot) * v_heads + head) * (kDim * kDim), kDim * kDim);
+            }
+            __syncwarp();
             const int length = chunk.length, first_block = chunk.first_block;
             const int key_head = head / (v_heads / kDeltaKeyHeads);
             const __nv_bfloat16* v_rows = qkv + static_cast<size_t>(chunk.begin) * channels + (2 * kDeltaKeyHeads + head) * kDim;
