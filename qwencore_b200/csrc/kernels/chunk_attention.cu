@@ -766,16 +766,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         };
         for (bool first = true; ok && next_piece(walk, first, p.sequences, info, piece); first = false) {
             const int first_token = walk.tile * kItemTokens + rank * kRowTokens;
+            // row r of the CTA: token r / 6, head r % 6 of the group
+            const uint4* queries = reinterpret_cast<const uint4*>(
+                                       p.query + ((static_cast<size_t>(walk.info.begin) + first_token) * kQueryHeads +
+                                                  walk.head * kGqaGroup) * kHeadDim) + lane;
+            const int live_rows = min(kRowTokens, walk.info.length - first_token) * kGqaGroup;
             const auto fetch_row = [&](int index) {
-                const int r = me * kWarpRows + index;
-                const int token = first_token + r / kGqaGroup;
-                uint4 raw = make_uint4(0, 0, 0, 0);
-                if (index < kWarpRows && r < kRowTokens * kGqaGroup && token < walk.info.length) {
-                    raw = __ldg(reinterpret_cast<const uint4*>(
-                                    p.query + ((static_cast<size_t>(walk.info.begin) + token) * kQueryHeads +
-                                               walk.head * kGqaGroup + r % kGqaGroup) * kHeadDim) + lane);
-                }
-                return raw;
+                const uint32_t r = me * kWarpRows + index;
+                constexpr uint32_t kRow = kHeadDim / 8, kToken = (kQueryHeads - kGqaGroup) * kRow;  // in uint4
+                return index < kWarpRows && static_cast<int>(r) < live_rows ? __ldg(queries + (r * kRow + r / kGqaGroup * kToken))
+                                                                            : make_uint4(0, 0, 0, 0);
             };
             // The row's numbers with its largest in [2^top, 2^(top + 1)), and what they are multiplied with to be what they
             // were; infinities and NaN stay what they are, and rows that are (nearly) zero are not blown up without end.
@@ -1087,6 +1087,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             const int first_dim = half * (kHeadDim / 2);
             const bool gated = whole && p.gate != nullptr && live;
             const __nv_bfloat16* gate_row = p.gate + row * p.gate_stride + head * (2 * kHeadDim) + kHeadDim + first_dim;
+            void* const target = whole ? static_cast<void*>(p.output + (row * kQueryHeads + head) * kHeadDim + first_dim)
+                                       : static_cast<void*>(p.partial_out + partial_row * kHeadDim + first_dim);
             uint4 gates[4] = {};
             if (gated) {
                 load64(gate_row, p.wide_rows, gates);
@@ -1131,7 +1133,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                                            pack_f16(value[8 * i + 4] * inverse, value[8 * i + 5] * inverse),
                                            pack_f16(value[8 * i + 6] * inverse, value[8 * i + 7] * inverse));
                     }
-                    store64(p.partial_out + partial_row * kHeadDim + first_dim + c * 32, p.wide_rows, out);
+                    store64(static_cast<__half*>(target) + c * 32, p.wide_rows, out);
                 } else if (live) {
                     uint4 out[4];
 #pragma unroll
@@ -1150,7 +1152,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         }
                         out[i] = make_uint4(words[0], words[1], words[2], words[3]);
                     }
-                    store64(p.output + (row * kQueryHeads + head) * kHeadDim + first_dim + c * 32, p.wide_rows, out);
+                    store64(static_cast<__nv_bfloat16*>(target) + c * 32, p.wide_rows, out);
                 }
                 __syncwarp();
             }
