@@ -781,18 +781,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             // were; infinities and NaN stay what they are, and rows that are (nearly) zero are not blown up without end.
             const auto scale_row = [&](const uint4& raw, int top, float (&x)[8]) {
                 const uint32_t words[4] = {raw.x, raw.y, raw.z, raw.w};
-                uint32_t highest = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    highest = max(highest, max(words[i] & 0x7fffu, (words[i] >> 16) & 0x7fffu));
-                }
-                highest = __reduce_max_sync(0xffffffffu, highest);
+                const uint32_t both = __vmaxu2(__vmaxu2(words[0] & 0x7fff7fffu, words[1] & 0x7fff7fffu),
+                                               __vmaxu2(words[2] & 0x7fff7fffu, words[3] & 0x7fff7fffu));
+                const uint32_t highest = __reduce_max_sync(0xffffffffu, max(both & 0xffffu, both >> 16));
                 const uint32_t exponent = max(highest >> 7, 64u);
                 const float up = exponent == 255u ? 1.0f : __uint_as_float((254u + top - exponent) << 23);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    x[2 * i] = __uint_as_float(words[i] << 16) * up;
-                    x[2 * i + 1] = __uint_as_float(words[i] & 0xffff0000u) * up;
+                    const float2 scaled = __fmul2_rn(make_float2(__uint_as_float(words[i] << 16), __uint_as_float(words[i] & 0xffff0000u)),
+                                                     make_float2(up, up));
+                    x[2 * i] = scaled.x;
+                    x[2 * i + 1] = scaled.y;
                 }
                 return exponent == 255u ? 1.0f : __uint_as_float((exponent - top) << 23);
             };
