@@ -784,14 +784,15 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 if (ok) {
                     // rows of v, zeros behind the chunk: sixteen lanes to a row
                     const int piece = lane & 15;
+                    const int left = length - at * kBlock - (lane >> 4);
+                    const __nv_bfloat16* from = v_rows + static_cast<size_t>(at * kBlock + (lane >> 4)) * channels + 8 * piece;
+                    const uint32_t to = smem_u32(sm.v + (piece >> 3) * (kVBytes / 2));
 #pragma unroll 8
                     for (int i = 0; i < kBlock / 2; ++i) {
-                        const int t = 2 * i + (lane >> 4);
-                        const int token = at * kBlock + t;
-                        const bool live = token < length;
+                        const bool live = 2 * i < left;
                         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
-                                         smem_u32(sm.v + (piece >> 3) * (kVBytes / 2) + swizzled(t, piece & 7))),
-                                     "l"(v_rows + static_cast<size_t>(live ? token : 0) * channels + 8 * piece), "r"(live ? 16 : 0)
+                                         to + swizzled(2 * i + (lane >> 4), piece & 7)),
+                                     "l"(live ? from + 2 * i * channels : v_rows), "r"(live ? 16 : 0)
                                      : "memory");
                     }
                 }
