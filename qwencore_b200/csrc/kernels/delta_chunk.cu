@@ -826,14 +826,16 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             for (int at = 0; at < blocks && ok; ++at, ++n) {
                 ok = wait(&sm.gate_empty[n & 1], ((n >> 1) & 1) ^ 1, failed, status);
                 if (ok) {
+                    const int left = length - at * kBlock - (lane >> 4);
+                    const __nv_bfloat16* from = rows + static_cast<size_t>(at * kBlock + (lane >> 4)) * norm.gate_stride;
+                    const uint32_t to = smem_u32(sm.gate[n & 1] + (lane >> 4) * (kDim * 2) + 16 * piece);
 #pragma unroll 4
                     for (int i = 0; i < kBlock / 2; ++i) {
-                        const int t = 2 * i + (lane >> 4);
-                        const int token = at * kBlock + t;
-                        const bool live = token < length;
-                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(sm.gate[n & 1] + t * (kDim * 2) + 16 * piece)),
-                                     "l"(rows + static_cast<size_t>(live ? token : 0) * norm.gate_stride), "r"(live ? 16 : 0)
+                        const bool live = 2 * i < left;
+                        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to + i * (kDim * 4)), "l"(live ? from : rows),
+                                     "r"(live ? 16 : 0)
                                      : "memory");
+                        from += 2 * static_cast<size_t>(norm.gate_stride);
                     }
                 }
                 asm volatile("cp.async.commit_group;" ::: "memory");
