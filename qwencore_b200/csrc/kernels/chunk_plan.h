@@ -3,7 +3,7 @@
 // An item is a tile of kItemTokens tokens of one chunk with one KV head; its units are the 128 positions of cache that go
 // through the tensor cores at once, up to the last position that the tile's last token sees.  All items lie on a line,
 // (sequence, head, tile) in order, each a lead of kItemLead and then its units: the lead is what an item costs besides, in
-// units (2048 tokens: 88 us with a lead of 8, 111 with 2, 92 with 12; 13 chunks of a ragged batch: 94, 119, 105).
+// units (2048 tokens: 80.5 us with a lead of 8, 81.9 with 6, 81.7 with 10; 13 chunks of a ragged batch: 86.4, 93.8, 91.7).
 // Worker w of n has positions total * w / n .. total * (w + 1) / n: every worker the same work, whatever the lengths are
 // (of a short line fewer workers have kSmallestShare each).  What of an item's units lies in a worker's share is a piece;
 // pieces of an item that is cut are merged afterwards.  The lead stands in front, so the workers that have pieces of

@@ -172,8 +172,8 @@ constexpr int kPitch = 68;  // floats of a row of the matrices in shared memory:
 
 constexpr int kMaxRatio = 3;  // value heads of a key head
 // Below this many blocks of a call a CTA takes one value head, from there on all of a key head, which share [Q ; K] K^T:
-// 48 heads, 64 tokens 31.1 us with one head and 40.5 with three, 512 tokens 55 and 60, 1280 tokens 102 and 106, 1600
-// tokens 123 and 121, 4 x 2048 tokens 352 and 335; 32 heads, 704 tokens 58.8 and 62.1, 1600 tokens 108.4 and 107.7.
+// 48 heads, 64 tokens 30.2 us with one head and 39.3 with three, 512 tokens 54 and 58, 1280 tokens 99 and 102, 1600
+// tokens 119 and 116, 4 chunks of 8192 in all 338 and 319; 32 heads, 704 tokens 56.7 and 59.6, 1600 tokens 104.7 and 103.8.
 constexpr int kFewBlocks = 24;
 
 struct FactorSmem {
@@ -212,7 +212,7 @@ __device__ __forceinline__ void multiply4(float2 (&x)[kRows][2], const float4 (&
 }
 
 // The chunks in the order of their length, for the second kernel: what takes longest begins first (20 chunks of 4000 tokens
-// in all 170 -> 166 us).  Of two alike the first is the longer.  By a CTA, a thread for a chunk.
+// in all 164.5 us, 170 in the order of the batch, a CTA for each).  Of two alike the first is the longer.  By a CTA, a thread for a chunk.
 __device__ __forceinline__ void find_order(int (&length)[kMaxChunkSequences], const uint32_t* begins, int tokens, int sequences,
                                            int4* order) {
     static_assert(kFactorThreads >= kMaxChunkSequences, "a thread for a chunk");
@@ -718,7 +718,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
     int n = 0;  // blocks so far
     // A job is a chunk with a value head, the longest first.  A CTA's first one is its own, then whoever is done takes the next;
     // the warp that loads takes it, and says which to the others.  -1: there is none.  (40 chunks of 1000 tokens in all: 192 us
-    // with a CTA for each job, 174 so; 128 chunks of 4000: 592 and 534; one chunk of 4096: 225 and 226.)
+    // with a CTA for each job, 173 so; 128 chunks of 4000: 592 and 529; one chunk of 4096: 225 and 226.)
     const int jobs = chunks * v_heads;
     int round = 0;
     const auto next_job = [&]() {
