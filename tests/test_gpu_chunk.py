@@ -906,3 +906,30 @@ def test_attention_chunk_value_codes_that_are_no_number(cuda, ops):
     weights = cuda.softmax(scores, -1)
     want, spread = (weights @ v).transpose(0, 1), (weights @ v.abs()).transpose(0, 1)
     assert ((got - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * spread).all()
+
+
+@pytest.mark.parametrize("heads", [32, 48])
+def test_delta_chunk_more_jobs_than_sms_and_slots_beyond_the_pool(cuda, ops, heads):
+    """Every CTA takes several (chunk, value head) pairs, some of which are left out."""
+    from qwencore_b200 import abi
+    lengths = [5, 200, 0, 64, 130, 1, 70, 65, 128, 3, 17, 90, 33, 64]
+    case = Delta(cuda, 71 + heads, lengths, heads, normed=True, continues=[i % 3 != 0 for i in range(len(lengths))])
+    whole = Delta(cuda, 71 + heads, lengths, heads, normed=True, continues=[i % 3 != 0 for i in range(len(lengths))])
+    whole.check(ops)
+    lost = [1, 5, 8]  # the longest among them
+    before = case.codes.clone(), case.scales.clone()
+    kept = [s for s in range(len(lengths)) if s not in lost]
+    good = list(case.slots)
+    for s in lost:
+        case.slots[s] = case.capacity + s
+    case.run(ops)
+    assert abi.lib.qwc_device_status() == 0x105
+    abi.check(abi.lib.qwc_device_status_reset(), "reset")
+    for s, n in enumerate(lengths):
+        rows = slice(case.first[s], case.first[s] + n)
+        if s in kept:
+            assert cuda.equal(case.out[rows], whole.out[rows])
+            assert cuda.equal(case.codes[good[s]], whole.codes[good[s]]) and cuda.equal(case.scales[good[s]], whole.scales[good[s]])
+        else:
+            assert (case.out[rows] == 7.0).all()
+            assert cuda.equal(case.codes[good[s]], before[0][good[s]]) and cuda.equal(case.scales[good[s]], before[1][good[s]])
