@@ -766,15 +766,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         };
         for (bool first = true; ok && next_piece(walk, first, p.sequences, info, piece); first = false) {
             const int first_token = walk.tile * kItemTokens + rank * kRowTokens;
-            // row r of the CTA: token r / 6, head r % 6 of the group
+            // row r of the CTA: token r / 6, head r % 6 of the group; the warps take rows in turn
             const uint4* queries = reinterpret_cast<const uint4*>(
                                        p.query + ((static_cast<size_t>(walk.info.begin) + first_token) * kQueryHeads +
                                                   walk.head * kGqaGroup) * kHeadDim) + lane;
             const int live_rows = min(kRowTokens, walk.info.length - first_token) * kGqaGroup;
             const auto fetch_row = [&](int index) {
-                const uint32_t r = me * kWarpRows + index;
+                const uint32_t r = index * kWidenWarps + me;
                 constexpr uint32_t kRow = kHeadDim / 8, kToken = (kQueryHeads - kGqaGroup) * kRow;  // in uint4
-                return index < kWarpRows && static_cast<int>(r) < live_rows ? __ldg(queries + (r * kRow + r / kGqaGroup * kToken))
+                return static_cast<int>(r) < live_rows ? __ldg(queries + (r * kRow + r / kGqaGroup * kToken))
                                                                             : make_uint4(0, 0, 0, 0);
             };
             // The row's numbers with its largest in [2^top, 2^(top + 1)), and what they are multiplied with to be what they
@@ -811,6 +811,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             float largest_scale = 0.0f;
 #pragma unroll 1
             for (int base = 0; base < kWarpRows; base += 4) {
+                if (base * kWidenWarps + me >= live_rows) {
+                    // none of these rows, nor of those behind: zeros
+                    for (int r = base * kWidenWarps + me; r < kRows; r += kWidenWarps) {
+                        uint8_t* to = sm.q + (lane >> 4) * kQueryBlock + r * 128 + (lane & 15) * 8;
+                        *reinterpret_cast<uint2*>(to) = make_uint2(0u, 0u);
+                        *reinterpret_cast<uint2*>(to + kDigitBytes) = make_uint2(0u, 0u);
+                        if (lane == 0) {
+                            sm.row_scale[r] = 1.0f;
+                        }
+                    }
+                    break;
+                }
                 const uint4 now[4] = {raw[0], raw[1], raw[2], raw[3]};
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -819,7 +831,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 }
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const int r = me * kWarpRows + base + j;
+                    const int r = (base + j) * kWidenWarps + me;
                     float x[8];
                     const float scale = scale_row(now[j], 7, x);
                     uint32_t d0[4], d1[4];
@@ -869,7 +881,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             if (widened) {
 #pragma unroll 2
                 for (int j = 0; j < kWarpRows; ++j) {
-                    const int r = me * kWarpRows + j;
+                    const int r = j * kWidenWarps + me;
                     float x[8];
                     const float scale = scale_row(fetch_row(j), 14, x);
                     // (the dims in the order in which widened keys have them)
@@ -902,7 +914,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 if (p.gate != nullptr) {
                     const int r = me * kWarpRows + lane;
                     const int token = first_token + r / kGqaGroup;
-                    if (r < kRowTokens * kGqaGroup && token < walk.info.length) {
+                    if (r < live_rows) {
                         bulk_prefetch_l2(p.gate + (static_cast<size_t>(walk.info.begin) + token) * p.gate_stride +
                                              (walk.head * kGqaGroup + r % kGqaGroup) * (2 * kHeadDim) + kHeadDim,
                                          kHeadDim * 2);
