@@ -806,7 +806,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             }
             const float largest_key = 448.0f * p.softmax_scale * (p.key_scales ? fabsf(p.key_scales[walk.head]) : 1.0f);
             // (Four rows at a time.  With all of them unrolled the warps waited for instructions: 30000 to 45000 cycles an
-            // item, now 13000.)
+            // item, 13000 so and less since.)
             float lost = 0.0f;  // by this lane's elements, over all rows
             float largest_scale = 0.0f;
 #pragma unroll 1
