@@ -20,9 +20,11 @@
 //     where a probability is zero.  The masks take bytes 0 and 2, 1 and 3 of a word together, so the columns of O lie in
 //     that order, and are put right when it is stored;
 //   * two threads share a row of S, 64 columns each.  Probabilities go back as f16 into the tensor memory of their scores, as
-//     the A operand of P V (rounded to eleven bits; their fp32 values are summed).  The running maximum that they refer to
-//     follows the scores only when these have grown by 2^8, so that O, which stays in tensor memory for the whole
-//     item, is hardly ever rescaled;
+//     the A operand of P V (their fp32 values are summed).  What they refer to follows the running maximum only when that has
+//     grown by 2^4, so that O, which stays in tensor memory for the whole item, is hardly ever rescaled.  The largest is put
+//     at 2^11 .. 2^15, near the upper end of what f16 holds: weights down to 2^-25 of the row's largest have eleven bits,
+//     smaller ones are off by up to 2^-36 of the largest (a first token that draws the weight and has no value, with thousands
+//     of others behind it, is their mean);
 //   * tensor memory: two buffers of scores (2 x 128 columns) and O (256 columns).  S of unit n + 1 is issued before P V of unit n.
 //
 //   warps 0-7   softmax, and the item's result
@@ -62,7 +64,9 @@ constexpr int kTmemColumns = 512;
 constexpr int kOutputColumn = 2 * kUnit;
 constexpr int kMaxPairs = 96;
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kRescaleAbove = 8.0f;                    // log2
+constexpr float kLargest = 11.0f;                        // log2 of a row's largest probability, when its reference is set ...
+constexpr float kRescaleAbove = 15.0f;                   // ... and where the reference has to be set again
+constexpr float kPartialScale = 128.0f;                  // of partial results: a value code is at most 480
 constexpr float kScoreError = 1.0f / 8192.0f;            // of a score, by digits that leave something
 static_assert(kPlanHeads == kKvHeads && kRowTokens * kGqaGroup <= kRows, "the plan's items");
 
@@ -96,7 +100,8 @@ struct Smem {
 };
 static_assert(sizeof(Smem) + 1024 <= 232448, "shared memory of a CTA");
 
-// What a pair leaves of an item that is cut: statistics and normalised rows of both CTAs, two slots for each pair.
+// What a pair leaves of an item that is cut: statistics and normalised rows of both CTAs, two slots for each pair.  The
+// rows are f16, in units of the value scale / 128: eleven bits, and nothing below 2^-32 of the scale.
 struct PartialStats {
     float maximum;  // log2
     float sum;
@@ -1024,9 +1029,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                 const float top = fmaxf(mine, sm.row_max[buffer][half ^ 1][r]) * scale;
                 // (a row without any score keeps its reference, and none at all counts as 0)
-                const bool grown = top > reference + kRescaleAbove;
+                const bool grown = top - reference > kRescaleAbove;
                 if (__any_sync(0xffffffffu, grown)) {
-                    const float factor = grown ? exp2_fast(reference - top) : 1.0f;
+                    const float lowered = top - kLargest;  // (beyond 2^27 a float may take more than that away)
+                    const float moved = top - lowered > kRescaleAbove ? top : lowered;
+                    const float factor = grown ? exp2_fast(reference - moved) : 1.0f;
                     if (unit > piece.unit_begin) {
                         // the first unit's O is not added to anything; after it, wait for the one before this
                         ok = wait(&sm.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, sm, p.status);
@@ -1049,7 +1056,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                         tmem_store_wait();
                     }
                     sum *= factor;
-                    reference = grown ? top : reference;
+                    reference = grown ? moved : reference;
                 }
                 const float minus = reference == -INFINITY ? 0.0f : -reference;
                 float sums[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -1111,6 +1118,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             sum += sm.row_sum[half ^ 1][r];
             const float inverse = sum > 0.0f || isnan(sum) ? 256.0f / sum : 0.0f;  // (values are 2^-8 of themselves)
             const float v_scale = inverse * (p.value_scales ? p.value_scales[walk.head] : 1.0f);
+            const float partial_scale = inverse * kPartialScale;
             // (a barrier for every second unit: P V of the unit before may still run, and on one barrier the parity of
             // this one would be that of the one before it)
             ok = wait(&sm.o_done[(g - 1) & 1], ((g - 1) >> 1) & 1, sm, p.status);
@@ -1139,10 +1147,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
                     uint4 out[4];
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        out[i] = make_uint4(pack_f16(value[8 * i] * inverse, value[8 * i + 1] * inverse),
-                                           pack_f16(value[8 * i + 2] * inverse, value[8 * i + 3] * inverse),
-                                           pack_f16(value[8 * i + 4] * inverse, value[8 * i + 5] * inverse),
-                                           pack_f16(value[8 * i + 6] * inverse, value[8 * i + 7] * inverse));
+                        out[i] = make_uint4(pack_f16(value[8 * i] * partial_scale, value[8 * i + 1] * partial_scale),
+                                           pack_f16(value[8 * i + 2] * partial_scale, value[8 * i + 3] * partial_scale),
+                                           pack_f16(value[8 * i + 4] * partial_scale, value[8 * i + 5] * partial_scale),
+                                           pack_f16(value[8 * i + 6] * partial_scale, value[8 * i + 7] * partial_scale));
                     }
                     store64(static_cast<__half*>(target) + c * 32, p.wide_rows, out);
                 } else if (live) {
@@ -1294,7 +1302,7 @@ __global__ void __launch_bounds__(kMergeWarps * 32) chunk_merge_kernel(const __g
             }
         }
     }
-    const float v_scale = p.value_scales ? p.value_scales[item.head] : 1.0f;
+    const float v_scale = (p.value_scales ? p.value_scales[item.head] : 1.0f) / kPartialScale;
     const float inverse = denominator > 0.0f || isnan(denominator) ? v_scale / denominator : 0.0f;
     const uint32_t gate_words[4] = {gates.x, gates.y, gates.z, gates.w};
     uint32_t words[4];

@@ -933,3 +933,26 @@ def test_delta_chunk_more_jobs_than_sms_and_slots_beyond_the_pool(cuda, ops, hea
         else:
             assert (case.out[rows] == 7.0).all()
             assert cuda.equal(case.codes[good[s]], before[0][good[s]]) and cuda.equal(case.scales[good[s]], before[1][good[s]])
+
+
+@pytest.mark.parametrize("lead", [9.0, 14.0, 18.0])
+@pytest.mark.parametrize("tokens,past,at", [(40, 8000, 0), (40, 8000, 8000), (3, 200, 0), (1000, 0, 0)])
+def test_attention_chunk_small_weights_decide(cuda, ops, tokens, past, at, lead):
+    """A token that draws nearly all of the weight and has no value: the result is what thousands of small weights say.
+
+    Probabilities are off by 2^-36 of the largest, partial results by 2^-32 of the value scale (which is 1 here)."""
+    torch = cuda
+    case = Attention(torch, 81, [tokens], [past], 16, gated=False, scaled=False, query_std=0.5)
+    keys, values = case.caches
+    keys[..., 0] = 0
+    case.query[..., 0] = 16.0
+    values[:] = (values.view(torch.float8_e4m3fn).float().abs() + 0.5).to(torch.float8_e4m3fn).view(torch.uint8)
+    page = case.table[0, at // 16].long()
+    keys[page, :, at % 16] = 0
+    keys[page, :, at % 16, 0] = torch.tensor([lead], device="cuda").to(torch.float8_e4m3fn).view(torch.uint8)
+    values[page, :, at % 16] = 0
+    got = case.run(ops).double()
+    want, spread = case.want()
+    largest = float(values[case.table[0].long()].view(torch.float8_e4m3fn).float().max())
+    bound = 2.0 ** -8 * want.abs() + 2.0 ** -10 * spread + 2.0 ** -36 * (tokens + past) * largest + 2.0 ** -32
+    assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
