@@ -307,11 +307,23 @@ def pack_decode_batch(row_slots, slot_active, seq_tokens, seq_blocks, rope_table
 
 # ---- chunks of new tokens and shared prefixes (additive entry points) ------------------------------
 
-def _check_here(*tensors) -> None:
-    """The launch goes to the current device: every tensor has to be there."""
-    device = torch.cuda.current_device()
-    for tensor in tensors:
-        assert tensor is None or (tensor.get_device() == device and tensor.is_contiguous())
+_U32 = (torch.int32, torch.uint32)
+_F32 = (torch.float32,)
+_BF16 = (torch.bfloat16,)
+_I8 = (torch.int8,)
+_E4M3 = (torch.uint8, torch.float8_e4m3fn, torch.int8)  # as codes or as bytes
+
+
+def _check_operands(*operands) -> int:
+    """Every operand is (tensor, its types, None for any, and the elements that it has at least); one left out is None.
+
+    The launch goes to the current device: every tensor has to be there.  Returns its current stream."""
+    device = operands[0][0].get_device()
+    for tensor, types, elements in operands:
+        assert tensor is None or ((types is None or tensor.dtype in types) and tensor.numel() >= elements and
+                                  tensor.get_device() == device and tensor.is_contiguous())
+    assert device == torch.cuda.current_device()
+    return torch._C._cuda_getCurrentRawStream(device)
 
 
 def copy_table(tensors, units: int) -> np.ndarray:
@@ -324,10 +336,9 @@ def copy_table(tensors, units: int) -> np.ndarray:
 def cache_copy(table: np.ndarray, pairs: torch.Tensor, count: int) -> None:
     """Unit `source` of every array becomes unit `target` for the first `count` rows of `pairs` (source, target)."""
     assert table.dtype == np.uint64 and table.ndim == 2 and table.shape[1] == 3 and table.flags.c_contiguous
-    assert pairs.numel() >= 2 * count and pairs.element_size() == 4
-    _check_here(pairs)
+    stream = _check_operands((pairs, _U32, 2 * count))
     arrays = ctypes.addressof(ctypes.c_char.from_buffer(table)) if table.flags.writeable else table.ctypes.data
-    abi.check(abi.lib.qwc_cache_copy(arrays, table.shape[0], _p(pairs), count, _stream()), "qwc_cache_copy")
+    abi.check(abi.lib.qwc_cache_copy(arrays, table.shape[0], _p(pairs), count, stream), "qwc_cache_copy")
 
 
 def attention_chunk_workspace_bytes() -> int:
@@ -342,30 +353,31 @@ def paged_attention_chunk(query, query_gate_projection, key_cache, value_cache, 
 
     Rows chunk_begins[s] .. chunk_begins[s + 1] are the newest tokens of sequence s; context_lengths count them.
     """
-    assert query.numel() >= tokens * NUM_ATTN_HEADS * ATTN_HEAD_DIM and query.dtype == torch.bfloat16
-    assert output.numel() >= tokens * NUM_ATTN_HEADS * ATTN_HEAD_DIM and output.dtype == torch.bfloat16
-    assert context_lengths.numel() >= sequences and chunk_begins.numel() > sequences
-    for scales in (key_scales, value_scales):
-        assert scales is None or (scales.numel() >= NUM_KV_HEADS and scales.dtype == torch.float32)
-    assert block_tables.numel() >= sequences * max_blocks_per_sequence
-    for cache in (key_cache, value_cache):
-        assert cache.numel() * cache.element_size() >= num_blocks * NUM_KV_HEADS * page_size * ATTN_HEAD_DIM
-    if query_gate_projection is not None:
-        stride = gate_stride or NUM_ATTN_HEADS * 2 * ATTN_HEAD_DIM
-        assert query_gate_projection.numel() >= (tokens - 1) * stride + NUM_ATTN_HEADS * 2 * ATTN_HEAD_DIM
-        assert query_gate_projection.dtype == torch.bfloat16
-    _check_here(query, query_gate_projection, key_cache, value_cache, block_tables, context_lengths, chunk_begins, output,
-                workspace, key_scales, value_scales)
+    rows = tokens * NUM_ATTN_HEADS * ATTN_HEAD_DIM
+    cache = num_blocks * NUM_KV_HEADS * page_size * ATTN_HEAD_DIM
+    gates = NUM_ATTN_HEADS * 2 * ATTN_HEAD_DIM
+    stream = _check_operands(
+        (query, _BF16, rows), (output, _BF16, rows), (key_cache, _E4M3, cache), (value_cache, _E4M3, cache),
+        (query_gate_projection, _BF16, (tokens - 1) * (gate_stride or gates) + gates),
+        (block_tables, _U32, sequences * max_blocks_per_sequence), (context_lengths, _U32, sequences),
+        (chunk_begins, _U32, sequences + 1), (key_scales, _F32, NUM_KV_HEADS), (value_scales, _F32, NUM_KV_HEADS),
+        (workspace, None, 0))
     workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     abi.check(abi.lib.qwc_paged_attention_chunk_fp8(
-        _p(query), _p(query_gate_projection), _p(key_cache), _p(value_cache), _p(block_tables), _p(context_lengths),
-        _p(chunk_begins), _p(key_scales), _p(value_scales), _p(output), _p(workspace), workspace_bytes, tokens, sequences,
-        max_blocks_per_sequence, page_size, num_blocks, gate_stride, 1.0 / math.sqrt(ATTN_HEAD_DIM), _stream()),
+        query.data_ptr(), _p(query_gate_projection), key_cache.data_ptr(), value_cache.data_ptr(),
+        block_tables.data_ptr(), context_lengths.data_ptr(), chunk_begins.data_ptr(), _p(key_scales), _p(value_scales),
+        output.data_ptr(), _p(workspace), workspace_bytes, tokens, sequences, max_blocks_per_sequence, page_size,
+        num_blocks, gate_stride, 1.0 / math.sqrt(ATTN_HEAD_DIM), stream),
         "qwc_paged_attention_chunk_fp8")
 
 
+_shape = abi.Shape()
+_shape_address = ctypes.byref(_shape)
+
+
 def _delta_channels() -> tuple[int, int]:
-    heads = abi.get_shape()[0]
+    abi.lib.qwc_get_shape(_shape_address)
+    heads = _shape.delta_value_heads
     return heads, (2 * LA_NUM_K_HEADS + heads) * LA_HEAD_DIM
 
 
@@ -374,20 +386,19 @@ def delta_prepare_chunk(mixed, a_offset: int, b_offset: int, conv_weight, a_log,
                         mixed_stride: int) -> None:
     """Convolution, norms and gates for chunks; a/b are strided views of the mixed row, as in `delta_prepare_decode`."""
     heads, channels = _delta_channels()
-    assert mixed.numel() >= (tokens - 1) * mixed_stride + max(channels, a_offset + heads, b_offset + heads)
-    assert qkv.numel() >= tokens * channels and alpha.numel() >= tokens * heads and beta.numel() >= tokens * heads
-    assert conv_state.numel() >= state_capacity * channels * 3 and conv_weight.numel() >= channels * 4
-    assert mixed.dtype == torch.bfloat16 and qkv.dtype == torch.bfloat16 and conv_state.dtype == torch.float32
-    assert alpha.dtype == torch.float32 and beta.dtype == torch.float32 and conv_weight.dtype == torch.bfloat16
-    assert state_slots.numel() >= sequences and chunk_begins.numel() > sequences
-    assert continues is None or continues.numel() >= sequences
-    _check_here(mixed, conv_weight, a_log, dt_bias, conv_state, state_slots, continues, chunk_begins, qkv, alpha, beta)
+    assert a_offset >= 0 and b_offset >= 0
+    stream = _check_operands(
+        (mixed, _BF16, (tokens - 1) * mixed_stride + max(channels, a_offset + heads, b_offset + heads)),
+        (conv_weight, _BF16, channels * 4), (a_log, _BF16, heads), (dt_bias, _BF16, heads),
+        (conv_state, _F32, state_capacity * channels * 3), (state_slots, _U32, sequences),
+        (continues, _U32, sequences), (chunk_begins, _U32, sequences + 1), (qkv, _BF16, tokens * channels),
+        (alpha, _F32, tokens * heads), (beta, _F32, tokens * heads))
     base = mixed.data_ptr()
-    abi.check(abi.lib.qwc_delta_prepare_chunk(base, base + 2 * a_offset, base + 2 * b_offset, _p(conv_weight), _p(a_log),
-                                              _p(dt_bias), _p(conv_state), _p(state_slots), _p(continues),
-                                              _p(chunk_begins), _p(qkv), _p(alpha), _p(beta), state_capacity, tokens,
-                                              sequences, mixed_stride, mixed_stride, _stream()),
-              "qwc_delta_prepare_chunk")
+    abi.check(abi.lib.qwc_delta_prepare_chunk(
+        base, base + 2 * a_offset, base + 2 * b_offset, conv_weight.data_ptr(), a_log.data_ptr(), dt_bias.data_ptr(),
+        conv_state.data_ptr(), state_slots.data_ptr(), _p(continues), chunk_begins.data_ptr(), qkv.data_ptr(),
+        alpha.data_ptr(), beta.data_ptr(), state_capacity, tokens, sequences, mixed_stride, mixed_stride, stream),
+        "qwc_delta_prepare_chunk")
 
 
 def delta_chunk_workspace_bytes(tokens: int, sequences: int) -> int:
@@ -401,22 +412,17 @@ def delta_chunk(state, state_scales, state_slots, continues, chunk_begins, qkv, 
 
     With `gate` (bf16 rows, z at column gate_offset) and `norm_weight` the gated RMSNorm is applied to the result."""
     heads, channels = _delta_channels()
-    assert state.dtype == torch.int8 and state_scales.dtype == torch.float32 and qkv.dtype == torch.bfloat16
-    assert state.numel() >= state_capacity * heads * LA_HEAD_DIM ** 2
-    assert state_scales.numel() >= state_capacity * heads * LA_HEAD_DIM
-    assert qkv.numel() >= tokens * channels and out.numel() >= tokens * heads * LA_HEAD_DIM
-    assert out.dtype == torch.bfloat16 and alpha.dtype == torch.float32 and beta.dtype == torch.float32
-    assert alpha.numel() >= tokens * heads and beta.numel() >= tokens * heads
-    assert state_slots.numel() >= sequences and chunk_begins.numel() > sequences
-    assert continues is None or continues.numel() >= sequences
-    if gate is not None:
-        stride = gate_stride or heads * LA_HEAD_DIM
-        assert gate.dtype == torch.bfloat16 and norm_weight.numel() >= LA_HEAD_DIM
-        assert gate.numel() >= (tokens - 1) * stride + gate_offset + heads * LA_HEAD_DIM
-    _check_here(state, state_scales, state_slots, continues, chunk_begins, qkv, alpha, beta, out, workspace, gate,
-                norm_weight)
+    width = heads * LA_HEAD_DIM
+    assert gate_offset >= 0
+    stream = _check_operands(
+        (state, _I8, state_capacity * width * LA_HEAD_DIM), (state_scales, _F32, state_capacity * width),
+        (state_slots, _U32, sequences), (continues, _U32, sequences), (chunk_begins, _U32, sequences + 1),
+        (qkv, _BF16, tokens * channels), (alpha, _F32, tokens * heads), (beta, _F32, tokens * heads),
+        (out, _BF16, tokens * width), (norm_weight, _BF16, LA_HEAD_DIM),
+        (gate, _BF16, (tokens - 1) * (gate_stride or width) + gate_offset + width), (workspace, None, 0))
     workspace_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     abi.check(abi.lib.qwc_delta_chunk_int8(
-        _p(state), _p(state_scales), _p(state_slots), _p(continues), _p(chunk_begins), _p(qkv), _p(alpha), _p(beta),
-        _p(out), state_capacity, tokens, sequences, 0 if gate is None else gate.data_ptr() + 2 * gate_offset, gate_stride,
-        _p(norm_weight), epsilon, _p(workspace), workspace_bytes, _stream()), "qwc_delta_chunk_int8")
+        state.data_ptr(), state_scales.data_ptr(), state_slots.data_ptr(), _p(continues), chunk_begins.data_ptr(),
+        qkv.data_ptr(), alpha.data_ptr(), beta.data_ptr(), out.data_ptr(), state_capacity, tokens, sequences,
+        0 if gate is None else gate.data_ptr() + 2 * gate_offset, gate_stride, _p(norm_weight), epsilon, _p(workspace),
+        workspace_bytes, stream), "qwc_delta_chunk_int8")

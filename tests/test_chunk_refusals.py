@@ -146,3 +146,62 @@ def test_wrappers_refuse_what_does_not_fit(abi):
         ops.cache_copy(np.zeros((1, 3), dtype=np.int64), zeros(2, i32), 1)
     with pytest.raises(AssertionError):
         ops.cache_copy(np.zeros((1, 3), dtype=np.uint64), zeros(2, i32), 2)
+
+
+def test_wrappers_refuse_other_types(abi):
+    """Lists of anything but 32 bits would be read behind their ends or misread, weights of another type misread."""
+    import torch
+
+    from qwencore_b200 import ops
+
+    bf16, f32, i32 = torch.bfloat16, torch.float32, torch.int32
+    zeros = lambda n, dtype: torch.zeros(n, dtype=dtype)  # noqa: E731
+    before = abi.get_shape()
+    abi.configure(32, 64)
+    channels, width = 8192, 8192 + 4096 + 64
+
+    def attention(**other):
+        given = dict(query=zeros(2 * 6144, bf16), query_gate_projection=zeros(2 * 12288, bf16), key_cache=zeros(3 * 16384, torch.uint8),
+                     value_cache=zeros(3 * 16384, torch.uint8), block_tables=zeros(4, i32), context_lengths=zeros(1, i32),
+                     chunk_begins=zeros(2, i32), max_blocks_per_sequence=4, output=zeros(2 * 6144, bf16), tokens=2, sequences=1,
+                     workspace=zeros(16, torch.uint8), page_size=16, num_blocks=3)
+        ops.paged_attention_chunk(**{**given, **other})
+
+    def prepare(**other):
+        given = dict(mixed=zeros(2 * width, bf16), a_offset=width - 64, b_offset=width - 32, conv_weight=zeros(channels * 4, bf16),
+                     a_log=zeros(32, bf16), dt_bias=zeros(32, bf16), conv_state=zeros(2 * channels * 3, f32), state_slots=zeros(1, i32),
+                     continues=zeros(1, i32), chunk_begins=zeros(2, i32), qkv=zeros(2 * channels, bf16), alpha=zeros(64, f32),
+                     beta=zeros(64, f32), state_capacity=2, tokens=2, sequences=1, mixed_stride=width)
+        ops.delta_prepare_chunk(**{**given, **other})
+
+    def delta(**other):
+        given = dict(state=zeros(2 * 32 * 16384, torch.int8), state_scales=zeros(2 * 32 * 128, f32), state_slots=zeros(1, i32),
+                     continues=zeros(1, i32), chunk_begins=zeros(2, i32), qkv=zeros(2 * channels, bf16), alpha=zeros(64, f32),
+                     beta=zeros(64, f32), out=zeros(2 * 4096, bf16), state_capacity=2, tokens=2, sequences=1,
+                     workspace=zeros(16, torch.uint8), gate=zeros(2 * 4096, bf16), norm_weight=zeros(128, bf16))
+        ops.delta_chunk(**{**given, **other})
+
+    lists = {attention: dict(block_tables=4, context_lengths=1, chunk_begins=2),
+             prepare: dict(state_slots=1, continues=1, chunk_begins=2), delta: dict(state_slots=1, continues=1, chunk_begins=2)}
+    try:
+        for call, names in lists.items():
+            for name, count in names.items():
+                for dtype in (torch.int64, torch.bool, torch.uint8, torch.int16, f32):
+                    with pytest.raises(AssertionError):
+                        call(**{name: zeros(2 * count, dtype)})
+        for dtype in (torch.int64, f32):
+            with pytest.raises(AssertionError):
+                ops.cache_copy(np.zeros((1, 3), dtype=np.uint64), zeros(4, dtype), 1)
+        for other in (dict(key_cache=zeros(3 * 16384, bf16)), dict(value_cache=zeros(3 * 16384, torch.float8_e5m2)),
+                      dict(value_cache=zeros(3 * 16384, f32))):
+            with pytest.raises(AssertionError):
+                attention(**other)
+        for other in (dict(a_log=zeros(32, f32)), dict(a_log=zeros(31, bf16)), dict(dt_bias=zeros(32, f32)),
+                      dict(dt_bias=zeros(31, bf16)), dict(a_offset=-8), dict(b_offset=-8)):
+            with pytest.raises(AssertionError):
+                prepare(**other)
+        for other in (dict(norm_weight=zeros(128, f32)), dict(norm_weight=zeros(128, torch.float16)), dict(gate_offset=-8)):
+            with pytest.raises(AssertionError):
+                delta(**other)
+    finally:
+        abi.configure(*before)
