@@ -327,9 +327,12 @@ def _check_operands(*operands) -> int:
 
 
 def copy_table(tensors, units: int) -> np.ndarray:
-    """The arrays of `cache_copy`: one row (address, bytes of a unit, units) for each tensor of `units` units."""
+    """The arrays of `cache_copy`: one row (address, bytes of a unit, units) for each tensor of `units` units.
+
+    The tensors are on one GPU, which is the current device wherever the table is used."""
     for tensor in tensors:
         assert tensor.is_contiguous() and tensor.numel() % units == 0
+        assert tensor.is_cuda and tensor.get_device() == tensors[0].get_device()
     return np.array([[t.data_ptr(), t.numel() // units * t.element_size(), units] for t in tensors], dtype=np.uint64)
 
 

@@ -205,3 +205,12 @@ def test_wrappers_refuse_other_types(abi):
                 delta(**other)
     finally:
         abi.configure(*before)
+
+
+def test_copy_table_refuses_memory_of_the_host(built_library):
+    import torch
+
+    from qwencore_b200 import ops
+
+    with pytest.raises(AssertionError):
+        ops.copy_table([torch.zeros((4, 16))], 4)
