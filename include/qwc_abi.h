@@ -57,7 +57,8 @@ int qwc_device_status_reset(void);
  * tag it found instead (epoch << 10 | exchange number; 0 = never written).  Host-side, synchronising. */
 int qwc_device_status_detail(uint32_t* expected_and_found);
 /* Host-side fault injection: stores `code` in the status word as a bounded wait that gave up
- * would (every kernel that waits then returns at once and skips its stores).  Synchronises. */
+ * would (every kernel that waits then returns at once and skips its stores; those on chunks of new
+ * tokens go on after 0x105 and 0x107, which no wait leaves).  Synchronises. */
 int qwc_device_status_set(int code);
 /* Copies the status word to `destination` (device memory, 4 bytes) in stream order: no sync,
  * capture-legal.  A step that ends with this copy lets its caller read the word together with
@@ -527,6 +528,8 @@ int qwc_cache_copy(const qwc_copy_array* arrays, int array_count, const uint32_t
  * u32[sequences] names each chunk's slot, no slot twice; a slot beyond the pool leaves its chunk out and the
  * device status word reads 0x105.  continues u32[sequences] (NULL: all 1) is 0 where a sequence begins with its chunk:
  * what the slot holds from before then counts as zeros.  The number of value heads comes from qwc_configure.
+ * When the device status word holds the code of a wait that gave up (any but 0x105 and 0x107), attention and delta rule do
+ * nothing: outputs, states and scales stay as they were.  Their own codes are 0x108 and 0x109.
  */
 
 /*

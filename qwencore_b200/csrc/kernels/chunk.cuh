@@ -21,6 +21,23 @@ __device__ __forceinline__ ChunkSpan chunk_span(const uint32_t* begins, int sequ
     return {static_cast<int>(first), end > first ? static_cast<int>(end - first) : 0};
 }
 
+// The status word as the operators on chunks take it.  A wait that gave up, anywhere, leaves results that nobody should build
+// on: the kernels that wait do nothing then, and leave outputs and states as they were.  An id out of range (a slot, a unit of
+// a copy) has left out its own chunk or pair and nothing else, so it does not stop them.
+__device__ __forceinline__ bool is_range_code(int code) { return code == kStatusStateSlotRange || code == kStatusCopyRange; }
+
+__device__ __forceinline__ int status_code(const int* status) { return *reinterpret_cast<const volatile int*>(status); }
+
+__device__ __forceinline__ bool stops_chunks(int code) { return code != kStatusOk && !is_range_code(code); }
+
+// A wait gave up: its code takes the place of an id out of range, which would not stop the kernels behind this one.
+__device__ __forceinline__ void record_wait(int* status, int code) {
+    const int before = atomicCAS(status, kStatusOk, code);
+    if (is_range_code(before)) {
+        atomicCAS(status, before, code);
+    }
+}
+
 // 2^x and 1 / x of the unit for special functions, to 2^-22 of themselves, without the instructions that would save results
 // below 2^-126.
 __device__ __forceinline__ float exp2_fast(float x) {

@@ -95,7 +95,7 @@ struct Smem {
     ChunkWalk start;
     long long total;
     uint32_t tmem_base;
-    int stop;    // nothing is done: an earlier kernel has given up
+    int stop;    // nothing is done: a wait of an earlier kernel has given up
     int failed;  // a wait gave up
 };
 static_assert(sizeof(Smem) + 1024 <= 232448, "shared memory of a CTA");
@@ -191,7 +191,7 @@ __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, Smem& sm,
             break;
         }
     }
-    atomicCAS(status, 0, kStatusChunkAttentionWait);
+    record_wait(status, kStatusChunkAttentionWait);
     *reinterpret_cast<volatile int*>(&sm.failed) = 1;
     return false;
 }
@@ -536,7 +536,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     if (rank == 0 && threadIdx.x < 2) {
         // both CTAs of a pair go by what the first one finds in the status word
-        const uint32_t stop = status_is_set(p.status) ? 1u : 0u;
+        const uint32_t stop = stops_chunks(status_code(p.status)) ? 1u : 0u;
         asm volatile(
             "{\n"
             ".reg .b32 remote;\n"

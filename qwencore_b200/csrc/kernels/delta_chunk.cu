@@ -139,7 +139,7 @@ __device__ __noinline__ bool wait_slow(uint64_t* bar, uint32_t parity, int* fail
             break;
         }
     }
-    atomicCAS(status, 0, kStatusChunkDeltaWait);
+    record_wait(status, kStatusChunkDeltaWait);
     *reinterpret_cast<volatile int*>(failed) = 1;
     return false;
 }
@@ -192,6 +192,7 @@ struct FactorSmem {
     int length[kMaxChunkSequences];
     uint64_t done;
     uint32_t tmem_base;
+    int stop;  // nothing is done: a wait of an earlier kernel has given up
     int failed;
 };
 static_assert(offsetof(FactorSmem, m.product) % 1024 == 0, "an operand's alignment");
@@ -270,8 +271,9 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
             *images.taken = 0;
         }
     }
+    const int code = status_code(status);
     const ChunkTile tile = find_chunk_tile(begins, sequences, tokens, kBlock, block);
-    const bool here = tile.sequence >= 0;
+    bool here = tile.sequence >= 0;
     const int first = tile.index * kBlock;
     const int count = here ? min(kBlock, tile.span.length - first) : 0;
     const size_t row0 = static_cast<size_t>(tile.span.begin) + first;
@@ -324,9 +326,13 @@ __global__ void __launch_bounds__(kFactorThreads, 4) delta_factor_kernel(
         }
         asm volatile("cp.async.wait_group 0;" ::: "memory");
     }
+    if (tid == 0) {
+        sm.stop = stops_chunks(code) ? 1 : 0;
+    }
     fence_proxy_async();
     __syncthreads();
     pdl_launch_dependents();
+    here = here && *reinterpret_cast<volatile int*>(&sm.stop) == 0;
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&sm.tmem_base);
     const uint32_t tmem_row = tmem_base + (static_cast<uint32_t>(warp * 32) << 16);
@@ -615,6 +621,7 @@ struct ChainSmem {
     uint64_t job_full[2], job_empty[2];
     int job[2];
     uint32_t tmem_base;
+    int stop;  // as above; the first kernel of this call may have given up, too
     int failed;
 };
 static_assert(sizeof(ChainSmem) + 1024 <= 232448, "shared memory of a CTA");
@@ -682,6 +689,9 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
         }
         sm.chunk[threadIdx.x] = {chunk.x, chunk.y, there ? chunk.z : 0, chunk.w, static_cast<int>(slot)};
     }
+    if (threadIdx.x == kGateWarp * 32) {
+        sm.stop = stops_chunks(status_code(status)) ? 1 : 0;
+    }
     if (threadIdx.x == kMmaWarp * 32) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(&sm.qk_full[i], 1);
@@ -719,7 +729,7 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
     // A job is a chunk with a value head, the longest first.  A CTA's first one is its own, then whoever is done takes the next;
     // the warp that loads takes it, and says which to the others.  -1: there is none.  (40 chunks of 1000 tokens in all: 192 us
     // with a CTA for each job, 173 so; 128 chunks of 4000: 592 and 529; one chunk of 4096: 225 and 226.)
-    const int jobs = chunks * v_heads;
+    const int jobs = *reinterpret_cast<volatile int*>(&sm.stop) != 0 ? 0 : chunks * v_heads;
     int round = 0;
     const auto next_job = [&]() {
         const int slot = round & 1;

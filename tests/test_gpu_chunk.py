@@ -956,3 +956,37 @@ def test_attention_chunk_small_weights_decide(cuda, ops, tokens, past, at, lead)
     largest = float(values[case.table[0].long()].view(torch.float8_e4m3fn).float().max())
     bound = 2.0 ** -8 * want.abs() + 2.0 ** -10 * spread + 2.0 ** -36 * (tokens + past) * largest + 2.0 ** -32
     assert ((got - want).abs() <= bound).all(), float(((got - want).abs() / bound).max())
+
+
+@pytest.mark.parametrize("code", [0x103, 0x108, 0x109])
+def test_a_wait_that_gave_up_stops_the_operators_on_chunks(cuda, ops, code):
+    """Attention and delta rule leave everything as it was, and are right again behind a reset."""
+    from qwencore_b200 import abi
+    attention = Attention(cuda, 82, [100, 1, 30], [2000, 40, 0], 16)
+    delta = Delta(cuda, 83, [100, 1, 30], 32, normed=True)
+    codes, scales = delta.codes.clone(), delta.scales.clone()
+    abi.check(abi.lib.qwc_device_status_set(code), "set")
+    try:
+        attention.run(ops)
+        delta.run(ops)
+        assert abi.lib.qwc_device_status() == code
+    finally:
+        abi.check(abi.lib.qwc_device_status_reset(), "reset")
+    assert (attention.output == 7.0).all() and (delta.out == 7.0).all()
+    assert cuda.equal(delta.codes, codes) and cuda.equal(delta.scales, scales)
+    attention.check(ops, workspace=attention.workspace)
+    delta.check(ops)
+
+
+@pytest.mark.parametrize("code", [0x105, 0x107])
+def test_ids_out_of_range_do_not_stop_the_operators_on_chunks(cuda, ops, code):
+    from qwencore_b200 import abi
+    attention = Attention(cuda, 84, [100, 1, 30], [2000, 40, 0], 16)
+    delta = Delta(cuda, 85, [100, 1, 30], 32)
+    abi.check(abi.lib.qwc_device_status_set(code), "set")
+    try:
+        attention.check(ops)
+        delta.check(ops)
+        assert abi.lib.qwc_device_status() == code
+    finally:
+        abi.check(abi.lib.qwc_device_status_reset(), "reset")
