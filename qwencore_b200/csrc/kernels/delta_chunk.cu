@@ -966,6 +966,13 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
                 ok = issue_values(n + 1);
             }
         }
+        // the last commits that nobody else waits for have arrived in this CTA's shared memory before it ends
+        if (ok && n > 0) {
+            for (int i = n > 2 ? n - 2 : 0; i < n && ok; ++i) {
+                ok = wait(&sm.qk_empty[i & 1], (i >> 1) & 1, failed, status) && wait(&sm.w_empty[i & 1], (i >> 1) & 1, failed, status);
+            }
+            ok = ok && wait(&sm.v_empty, (n - 1) & 1, failed, status);
+        }
     } else if (warp < kChainWarps) {
         // ---------------- the chain --------------------------------------------------------------------
         const int quarter = warp & 3;
@@ -1276,6 +1283,10 @@ __global__ void __launch_bounds__(kChainThreads, 1) delta_chain_kernel(
             arrived(&sm.v_empty, n & 1);
             arrived(&sm.o_done, n & 1);
             arrived(&sm.s_done, n & 1);
+            for (int i = n > 1 ? n - 1 : 0; i <= n; ++i) {
+                arrived(&sm.qk_empty[i & 1], (i >> 1) & 1);
+                arrived(&sm.w_empty[i & 1], (i >> 1) & 1);
+            }
         }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
