@@ -557,7 +557,6 @@ int qwc_paged_attention_chunk_fp8(const void* query, const void* query_gate_proj
  * mixed_stride % 8 == 0); the convolution starts from the slot's history conv_state f32[capacity, channels, 3] and leaves
  * the chunk's last rows there.  qkv bf16[tokens, channels]: q [16][128] (scaled by 128^-1/2) | k [16][128] |
  * v [heads][128], each rounded once; alpha, beta f32[tokens, heads].  mixed_qkv, conv_weight, conv_state and qkv 16-byte aligned.
- * conv_weight must not be written by the kernel just before this one.
  */
 int qwc_delta_prepare_chunk(const void* mixed_qkv, const void* a_projection, const void* b_projection,
                             const void* conv_weight, const void* a_log, const void* dt_bias, void* conv_state,

@@ -61,9 +61,10 @@ __global__ void __launch_bounds__(kPrepareWarps * 32) delta_prepare_chunk_kernel
     const int head = blockIdx.x * kPrepareWarps + (threadIdx.x >> 5);
     const int channel = head * kDeltaHeadDim + (threadIdx.x & 31) * 4;
     const bool gates = blockIdx.x * kPrepareWarps >= heads;  // the last CTA of a tile
+    pdl_wait();
     Channels taps[kTaps];
     if (!gates) {
-        // never written during a step: fetched before the wait
+        // (on its way while the tile is looked for)
         const uint4* at = reinterpret_cast<const uint4*>(conv_weight + static_cast<size_t>(channel) * kTaps);
         const uint4 raw[2] = {at[0], at[1]};  // four taps of a channel are 8 bytes
         const Channels c0 = unpack4(make_uint2(raw[0].x, raw[0].y)), c1 = unpack4(make_uint2(raw[0].z, raw[0].w));
@@ -73,7 +74,6 @@ __global__ void __launch_bounds__(kPrepareWarps * 32) delta_prepare_chunk_kernel
         taps[2] = {make_float2(c0.hi.x, c1.hi.x), make_float2(c2.hi.x, c3.hi.x)};
         taps[3] = {make_float2(c0.hi.y, c1.hi.y), make_float2(c2.hi.y, c3.hi.y)};
     }
-    pdl_wait();
     const ChunkTile tile = find_chunk_tile(begins, sequences, tokens, kTileTokens, blockIdx.y);
     if (tile.sequence < 0) {
         return;

@@ -990,3 +990,27 @@ def test_ids_out_of_range_do_not_stop_the_operators_on_chunks(cuda, ops, code):
         assert abi.lib.qwc_device_status() == code
     finally:
         abi.check(abi.lib.qwc_device_status_reset(), "reset")
+
+
+def test_delta_prepare_chunk_behind_a_write_of_its_weights(cuda, ops):
+    """The kernel in front lets this one start early and writes the taps at its end."""
+    from qwencore_b200 import abi
+    torch = cuda
+    case = Prepare(torch, 86, [9, 100], 32)
+    taps = case.taps
+    big = torch.zeros((2, 1 << 28), dtype=torch.uint8, device="cuda")
+    held = torch.zeros((2,) + tuple(taps.shape), dtype=torch.bfloat16, device="cuda")
+    held[0] = taps
+    case.taps = held[1]
+    table, pairs = ops.copy_table([big, held], 2), i32(torch, [0, 1])
+    slots, begins, history = i32(torch, case.slots), i32(torch, case.first), case.history.clone()
+    qkv = torch.zeros_like(case.qkv)
+    abi.configure(case.heads, 64)
+    torch.cuda.synchronize()
+    ops.cache_copy(table, pairs, 1)
+    ops.delta_prepare_chunk(case.mixed, case.channels, case.channels + case.heads, case.taps, case.a_log, case.dt_bias,
+                            case.history, slots, None, begins, qkv, case.alpha, case.beta, case.capacity, case.tokens, 2,
+                            case.width)
+    case.history.copy_(history)
+    case.check(ops)
+    assert torch.equal(qkv, case.qkv)
