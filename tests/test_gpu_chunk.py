@@ -1014,3 +1014,78 @@ def test_delta_prepare_chunk_behind_a_write_of_its_weights(cuda, ops):
     case.history.copy_(history)
     case.check(ops)
     assert torch.equal(qkv, case.qkv)
+
+
+@pytest.mark.parametrize("std", [1e-3, 30.0, 3000.0])
+def test_attention_chunk_scores_as_steep_as_they_are(cuda, ops, std):
+    """A score s_j is a sum of 256 products in fp32, 16 steps of the tensor cores: each cuts off less than 2^-23 of what it has
+    summed up, twice that with the alignment of its products, so s_j is off by d_j <= 2^-18 sum |q||k_j| / 16.  To first
+    order that moves the result by sum_j w_j (d_j - mean) (v_j - o), 2 max d sum_j w_j |v_j - o| at most: nothing where
+    one weight is 1.  (e^(2 d) - 1 in place of 2 d for those that are large.)  And where a weight is 1 and its value 0, what
+    is left of the others: a probability is an f16 whose row's largest is 2^11 or more, off by half of its smallest step of 2^-24, so
+    a weight is off by 2^-36; a partial result is an f16 of 2^7 times the value over its scale, off by 2^-32 scales."""
+    torch = cuda
+    case = Attention(torch, 87, [70, 3], [500, 900], 16, query_std=std)
+    got = case.run(ops).double()
+    want, spread = case.want()
+    winners = 0
+    for s, n in enumerate(case.lengths):
+        context = case.contexts[s]
+        ids = case.table[s, :-(-context // case.page)].long()
+        k, v = (c[ids].view(torch.float8_e4m3fn).double().transpose(0, 1).reshape(KV, -1, WIDE)[:, :context].repeat_interleave(GROUP, 0) *
+                case.scale.double().repeat_interleave(GROUP)[:, None, None] for c in case.caches)
+        for i in range(n):
+            row, seen = case.first[s] + i, context - n + i + 1
+            q = case.query[row].double()[:, None]
+            weights = torch.softmax(q @ k[:, :seen].transpose(1, 2) / 16.0, -1)
+            off = 2.0 ** -18 * (q.abs() @ k[:, :seen].abs().transpose(1, 2)).amax((1, 2)) / 16.0
+            result = (weights @ v[:, :seen])[:, 0]
+            around = (weights.transpose(1, 2) * (v[:, :seen] - result[:, None]).abs()).sum(1)
+            gate = torch.sigmoid(case.gate[row].double().reshape(HEADS, 2 * WIDE)[:, WIDE:])
+            bound = 2.0 ** -8 * want[row].abs() + 2.0 ** -10 * spread[row] + torch.expm1(2 * off)[:, None] * around * gate
+            bound += 2.0 ** -36 * seen * v[:, :seen].abs().amax(1) + 2.0 ** -32 * case.scale.repeat_interleave(GROUP)[:, None]
+            assert ((got[row] - want[row]).abs() <= bound).all(), (row, float(((got[row] - want[row]).abs() / bound).max()))
+            winners += int((weights.amax(-1) > 0.9999).sum())
+    assert winners > 1000 or std < 1000.0
+
+
+@pytest.mark.parametrize("lengths,past", [([100, 3], [0, 40]), ([20], [3000])])
+def test_attention_chunk_scales_of_keys_and_values(cuda, ops, lengths, past):
+    """Different ones, in items of one piece and in items that are cut."""
+    torch = cuda
+    case = Attention(torch, 88, lengths, past, 16)
+    ratio = torch.tensor([0.5, 3.0, 8.0, 0.125], device="cuda")
+    workspace = torch.zeros(ops.attention_chunk_workspace_bytes(), dtype=torch.uint8, device="cuda")
+    ops.paged_attention_chunk(case.query, case.gate, *case.caches, case.table, i32(torch, case.contexts), i32(torch, case.first),
+                              case.widest, case.output, case.tokens, len(lengths), workspace, case.page, case.pool,
+                              key_scales=case.scale, value_scales=case.scale * ratio)
+    want, spread = (x * ratio.double().repeat_interleave(GROUP)[None, :, None] for x in case.want())
+    assert ((case.output.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -10 * spread).all()
+
+
+@pytest.mark.parametrize("heads", [32, 48])
+def test_delta_chunk_norm_of_exact_results(cuda, ops, heads):
+    """Keys that are unit vectors, one for each token, and no decay: o_t = v_t / 8 without any rounding, so what is off is the
+    norm's: fp32 sums of 128 squares, a root, two products and a sigmoid (2^-19 together) and half a bf16 step."""
+    torch = cuda
+    lengths = [100, 1, 64, 128, 30]
+    case = Delta(torch, 89, lengths, heads, continues=[0] * 5, normed=True)
+    place = torch.cat([torch.arange(n, device="cuda") for n in lengths])
+    keys = torch.nn.functional.one_hot(place, DIM).bfloat16()[:, None].expand(-1, KEY_HEADS, -1).reshape(case.tokens, -1)
+    case.qkv[:, :KEY_HEADS * DIM] = keys / 8
+    case.qkv[:, KEY_HEADS * DIM:2 * KEY_HEADS * DIM] = keys
+    case.alpha.fill_(1.0)
+    case.beta.fill_(1.0)
+    case.run(ops)
+    o = case.qkv[:, 2 * KEY_HEADS * DIM:].double().reshape(case.tokens, heads, DIM) / 8
+    gate = case.gate.double().reshape(case.tokens, heads, DIM)
+    want = o / torch.sqrt(o.square().mean(-1, keepdim=True) + EPS) * case.weight.double() * torch.nn.functional.silu(gate)
+    assert ((case.out.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -19) * want.abs()).all()
+
+
+@pytest.mark.parametrize("tokens,strength", [(2048, 1.0), (8192, 1.0), (8192, 0.02)])
+def test_delta_chunk_states_that_last(cuda, ops, tokens, strength):
+    """Hardly any decay over 32 and 128 blocks; with weak writes the state keeps what thousands of tokens have put there."""
+    case = Delta(cuda, 90, [tokens, 65], 32, rate=(1e-6, 1e-3))
+    case.beta *= strength
+    case.check(ops)
