@@ -224,15 +224,16 @@ extern "C" int qwc_delta_prepare_chunk(const void* mixed_qkv, const void* a_proj
             static_cast<const uint32_t*>(chunk_begins), static_cast<__nv_bfloat16*>(qkv), static_cast<float*>(alpha),
             static_cast<float*>(beta), tokens, sequences, mixed_stride, gate_stride, v_heads, state_capacity, status);
     };
-    // The shortest tile with no more than 1500 CTAs (three to four rounds of what is resident at once), or the longest.
-    // Measured (us, tiles of 8 / 16 / 32 / 64): 17 tokens, 32 heads 4.4 / 6.3 / 8.1 / 8.1; 256 tokens, 48 heads 6.6 / 8.4 /
-    // 11.0 / 17.0; 1024 tokens 13.8 / 14.5 / 15.6 / 23.0; 2048 tokens 25.4 / 23.4 / 24.6 / 28.0; 8192 tokens 95.0 / 81.3 /
-    // 77.9 / 80.7 (4.4 TB/s).
+    // The shortest tile with no more than 1500 CTAs (three to four rounds of what is resident at once; a chunk's last tile
+    // counts as one, however short it is), or the longest.
+    // Measured (us, tiles of 8 / 16 / 32): 17 tokens, 32 heads 4.5 / 6.5 / 8.2; with 48 heads 512 tokens 9.6 / 9.8 / 13.7, 1088
+    // tokens 15.2 / 15.3 / 15.9, 2100 tokens 27.1 / 24.6 / 25.4, 8192 tokens 96 / 82 / 79 (4.3 TB/s); 1088 tokens in 64 chunks
+    // 27.3 / 23.3 / 22.4, in 128 chunks 40.5 / 32.4 / 31.1.
     const int ctas_per_tile = (2 * kDeltaKeyHeads + v_heads) / kPrepareWarps + 1;
-    if (tokens / 8 * ctas_per_tile <= 1500) {
+    if (most_chunk_tiles(tokens, sequences, 8) * ctas_per_tile <= 1500) {
         return launch(delta_prepare_chunk_kernel<8>, 8);
     }
-    if (tokens / 16 * ctas_per_tile <= 1500) {
+    if (most_chunk_tiles(tokens, sequences, 16) * ctas_per_tile <= 1500) {
         return launch(delta_prepare_chunk_kernel<16>, 16);
     }
     return launch(delta_prepare_chunk_kernel<32>, 32);
