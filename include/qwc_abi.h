@@ -525,9 +525,9 @@ int qwc_cache_copy(const qwc_copy_array* arrays, int array_count, const uint32_t
  * The operators below take a ragged batch of chunks of new tokens, `sequences` of them (1..128), in
  * `tokens` rows (1..65536): chunk s is rows chunk_begins[s] .. chunk_begins[s + 1] (u32[sequences + 1], device,
  * ascending, cut at `tokens`; empty chunks are fine).  Rows of no chunk are left as they were.  state_slots
- * u32[sequences] names each chunk's slot, no slot twice; a slot beyond the pool leaves its chunk out and the
- * device status word reads 0x105.  continues u32[sequences] (NULL: all 1) is 0 where a sequence begins with its chunk:
- * what the slot holds from before then counts as zeros.  The number of value heads comes from qwc_configure.
+ * u32[sequences] names each chunk's slot, no slot twice (an empty chunk's is not looked at; state_capacity is `sequences` or
+ * more all the same); a slot beyond the pool leaves its chunk out and the device status word reads 0x105.  continues
+ * u32[sequences] (NULL: all 1) is 0 where a sequence begins with its chunk: what the slot holds from before then counts as zeros.  The number of value heads comes from qwc_configure.
  * When the device status word holds the code of a wait that gave up (any but 0x105 and 0x107), attention and delta rule do
  * nothing: outputs, states and scales stay as they were.  Their own codes are 0x108 and 0x109.
  */
@@ -539,7 +539,8 @@ int qwc_cache_copy(const qwc_copy_array* arrays, int array_count, const uint32_t
  * and gate_stride as qwc_paged_attention_packed_fp8_scaled, except that block_tables u32[sequences, max_blocks] has a
  * row for each sequence.  query, output bf16[tokens, 24, 256].  num_blocks: pages of the cache; a page
  * beyond it reads as zeros.  Scales are positive.  A value code that is no number (0x7f, 0xff) counts as 480 times the
- * scale, a key code makes its row NaN where it is seen.  workspace: qwc_paged_attention_chunk_workspace_bytes() bytes; calls that overlap on
+ * scale, a key code makes its row NaN where it is seen.  Scores are right to 2^-13 or to what fp32 sums
+ * of their terms are, weights to 2^-12 of themselves and, below 2^-25 of a row's largest weight, to 2^-36 of that.  workspace: qwc_paged_attention_chunk_workspace_bytes() bytes (25.6 MB); calls that overlap on
  * the device must not share one.  Pointers of rows, caches and workspace 16-byte aligned.
  * The segment shapes of crates/qwc-cuda/src/ffi.rs:520-537, for a whole batch.
  */
@@ -570,8 +571,11 @@ int qwc_delta_prepare_chunk(const void* mixed_qkv, const void* a_projection, con
  * The state is read from its eight bits at the start of a chunk, carried in fp32, and written back at its end.
  * qkv, alpha (none negative), beta: what qwc_delta_prepare_chunk wrote.  out bf16[tokens, heads, 128].  With norm_weight
  * bf16[128] and gate bf16 rows of gate_stride elements (0 = heads * 128; both or neither NULL), out is
- * rmsnorm(o) * norm_weight * silu(gate) instead.  workspace: qwc_delta_chunk_workspace_bytes(tokens, sequences) bytes;
- * calls that overlap on the device must not share one.  Row pointers, state and workspace 16-byte aligned.
+ * rmsnorm(o) * norm_weight * silu(gate) instead.  workspace: qwc_delta_chunk_workspace_bytes(tokens, sequences) bytes, 2.1 MB
+ * (48 heads; 1.6 MB with 32) for each 64 tokens begun and for each sequence: 70 MB for 2048 tokens of one sequence, 2.4 GB for
+ * 65536 of 128, which a caller with less memory takes in several calls; calls that overlap on the device must not share one.
+ * An element that is no number reaches its chunk's rows from the block of 64 tokens that holds it on, rows of that block in
+ * front of it too.  Row pointers, state and workspace 16-byte aligned.
  */
 size_t qwc_delta_chunk_workspace_bytes(int tokens, int sequences);
 int qwc_delta_chunk_int8(void* state, float* state_scales, const void* state_slots, const void* continues,
