@@ -539,8 +539,9 @@ int qwc_cache_copy(const qwc_copy_array* arrays, int array_count, const uint32_t
  * and gate_stride as qwc_paged_attention_packed_fp8_scaled, except that block_tables u32[sequences, max_blocks] has a
  * row for each sequence.  query, output bf16[tokens, 24, 256].  num_blocks: pages of the cache; a page
  * beyond it reads as zeros.  Scales are positive.  A value code that is no number (0x7f, 0xff) counts as 480 times the
- * scale, a key code makes its row NaN where it is seen.  Scores are right to 2^-13 or to what fp32 sums
- * of their terms are, weights to 2^-12 of themselves and, below 2^-25 of a row's largest weight, to 2^-36 of that.  workspace: qwc_paged_attention_chunk_workspace_bytes() bytes (25.6 MB); calls that overlap on
+ * scale, a key code makes its row NaN where it is seen.  Scores are right to 2^-13, or to what fp32 sums
+ * of their terms leave of queries whose elements count to 2^-39 of their row's largest; weights to 2^-12 of themselves and, below
+ * 2^-25 of a row's largest weight, to 2^-36 of that.  workspace: qwc_paged_attention_chunk_workspace_bytes() bytes (25.6 MB); calls that overlap on
  * the device must not share one.  Pointers of rows, caches and workspace 16-byte aligned.
  * The segment shapes of crates/qwc-cuda/src/ffi.rs:520-537, for a whole batch.
  */
